@@ -117,6 +117,19 @@ int tfjs_cuda_sync(tfjs_cuda_ctx* ctx);
 int tfjs_cuda_size_of(tfjs_cuda_ctx* ctx, int32_t id, uint64_t* out_nbytes);
 /* Raw device address of a tensor, for interop (profilers, other libraries). */
 int tfjs_cuda_device_ptr(tfjs_cuda_ctx* ctx, int32_t id, void** out_ptr);
+/* A tensor over device memory that belongs to the caller (another library's buffer), without
+ * a copy: the device half of creating a tensor from GPU data.  `ptr` must be device memory of
+ * the context's GPU, 16-byte aligned, and stay valid until the id has been freed and the work
+ * that reads it has run (tfjs_cuda_signal_stream orders its next user behind that work).
+ * tfjs_cuda_free forgets the id and leaves the memory alone; tfjs_cuda_memory does not count
+ * its bytes. */
+int tfjs_cuda_from_device(tfjs_cuda_ctx* ctx, void* ptr, uint64_t nbytes, int32_t* out_id);
+/* Order against a stream of the caller's (a cudaStream_t, 0 = the legacy default stream):
+ * wait_stream makes everything this context launches from now on run after the work already
+ * queued on `stream`; signal_stream makes everything queued on `stream` from now on run after
+ * the work this context has launched.  Neither blocks the host. */
+int tfjs_cuda_wait_stream(tfjs_cuda_ctx* ctx, void* stream);
+int tfjs_cuda_signal_stream(tfjs_cuda_ctx* ctx, void* stream);
 /* backend.memory() (tfjs-core/src/engine.ts:959-974). */
 int tfjs_cuda_memory(tfjs_cuda_ctx* ctx, uint64_t* bytes_in_use,
                      uint64_t* bytes_reserved, uint64_t* high_water,
@@ -438,6 +451,91 @@ int tfjs_cuda_fused_attention(tfjs_cuda_ctx* ctx, int32_t q_id, int32_t k_id, in
                               int32_t mask_id, int32_t has_scale, float scale, int32_t batch,
                               int32_t heads, int32_t seq, int32_t head_dim,
                               int32_t units_per_mask, int32_t out_id);
+
+/* ---- A paged key-value cache and attention of one new token over it ----------------------
+ * What a decoder keeps between tokens.  Keys and values live in two pools of pages,
+ *   k_cache, v_cache  float32 [num_pages, kv_heads, page_size, head_dim]
+ * and row b of a batch owns the pages that page_table[b, :] (int32 [batch, max_pages]) lists:
+ * its slot j, 0 <= j < lengths[b] (int32 [batch]), is place j % page_size of page
+ * page_table[b, j / page_size].  A row's capacity is max_pages * page_size slots.  Entries of
+ * the table behind a row's last slot are not read and may hold anything.  The pools are updated
+ * in place; every other tensor is a value that the calls read or write whole.
+ *
+ * A page number outside [0, num_pages) that a call needs and a length outside [0, capacity]
+ * are skipped on the device (the slots of such a page count as absent, the length is clamped)
+ * and reported by the next blocking call (read, read_wait, sync) as TFJS_CUDA_INVALID_ARG.
+ * No counterpart in the reference's kernel set. */
+typedef struct tfjs_cuda_paged_params {
+  int32_t batch, heads, kv_heads, head_dim; /* heads: attention only, a multiple of kv_heads */
+  int32_t num_pages, page_size, max_pages;
+  int32_t tokens;            /* append: tokens per row of k and v */
+  int32_t budget, recent;    /* evict */
+  int32_t has_scale;         /* attention */
+  float scale;
+} tfjs_cuda_paged_params;
+
+/* Writes k[b, h, t, :] and v[b, h, t, :] (float32 [batch, kv_heads, tokens, head_dim], the
+ * heads-split store of a projection) into slot lengths[b] + t for every t < counts[b]
+ * (int32 [batch]; counts_id 0: all tokens) and out_lengths[b] = lengths[b] + counts[b].
+ * Tokens that do not fit a row's capacity are dropped and reported.  The pages written must
+ * not be shared between rows. */
+int tfjs_cuda_paged_cache_append(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params* p,
+                                 int32_t k_cache_id, int32_t v_cache_id, int32_t k_id,
+                                 int32_t v_id, int32_t page_table_id, int32_t lengths_id,
+                                 int32_t counts_id, int32_t out_lengths_id);
+
+/* out[b, 0, h, :] = sum_j p_j v_j with p = softmax_j(fl32(q[b, h, 0, :] . k_j * scale) + mask[b, j])
+ * over the slots of row b; query head h reads key-value head h / (heads / kv_heads).
+ * q is [batch, heads, 1, head_dim], out [batch, 1, heads, head_dim]; has_scale = 0 skips the
+ * product.  mask (float32 [batch, capacity], 0: none) is added to the scores; -infinity hides
+ * a slot, and nothing is read of slots behind a row's length.  A row that has no slot, or only
+ * hidden ones, gives zeros.  weights (float32 [batch, kv_heads, capacity], 0: none) accumulates
+ * attention: out_weights[b, g, j] = weights[b, g, j] + the sum of p_j over the query heads of
+ * key-value head g, and 0 behind the row's length. */
+int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params* p, int32_t q_id,
+                              int32_t k_cache_id, int32_t v_cache_id, int32_t page_table_id,
+                              int32_t lengths_id, int32_t mask_id, int32_t weights_id,
+                              int32_t out_id, int32_t out_weights_id);
+
+/* Keeps m = min(lengths[b], budget) slots of every row and key-value head and moves them to
+ * the front.  Slot j holds the token of position positions[b, g, j] (int32 [batch, kv_heads,
+ * capacity]; a negative entry, and every entry when positions_id is 0: total[b] -
+ * (lengths[b] - j)), where total[b] (int32 [batch], 0: the lengths) counts all tokens the row
+ * has seen.  Kept are first the slots of the `recent` latest positions, then those of the
+ * largest weights; NaN counts as the largest weight, and among equals the lower slot stays.
+ * Kept slots below m stay where they are; the kept slots from m on move into the places that
+ * became free, both in ascending order (attention does not depend on the order of the slots).
+ *   out_weights, out_positions  the slots' weights and positions after the move, 0 and -1
+ *                               from slot m on
+ *   out_lengths                 m
+ *   out_kept                    int32 [batch, kv_heads, budget]: the slot each one came from,
+ *                               -1 from slot m on
+ * Pages of rows that lose slots must not be shared between rows. */
+int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params* p,
+                                int32_t k_cache_id, int32_t v_cache_id, int32_t weights_id,
+                                int32_t page_table_id, int32_t lengths_id, int32_t positions_id,
+                                int32_t total_id, int32_t out_weights_id,
+                                int32_t out_positions_id, int32_t out_lengths_id,
+                                int32_t out_kept_id);
+
+/* ---- Linear attention with a decay for each head -------------------------------------------
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   out_t = scale * q_t S_t
+ * for q, k [batch, heads, seq, dim_k], v [batch, heads, seq, dim_v], log_decay [heads] (at most
+ * 0 in a useful model, not checked), state [batch, heads, dim_k, dim_v] (state_id 0: zeros).
+ * out is [batch, seq, heads, dim_v] (heads merged, as tfjs_cuda_fused_attention stores it) and
+ * out_state the state behind each row's last token.  lengths (int32 [batch], 0: all of seq)
+ * gives the tokens of each row: what is behind them does not enter, and their out is zero.
+ * has_scale = 0 skips the product.  One token is one step of the recurrence; prompts run in
+ * chunks.  dim_k and dim_v up to 256.  No counterpart in the reference's kernel set. */
+typedef struct tfjs_cuda_linear_attention_params {
+  int32_t batch, heads, seq, dim_k, dim_v;
+  int32_t has_scale;
+  float scale;
+} tfjs_cuda_linear_attention_params;
+int tfjs_cuda_linear_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_linear_attention_params* p,
+                               int32_t q_id, int32_t k_id, int32_t v_id, int32_t log_decay_id,
+                               int32_t state_id, int32_t lengths_id, int32_t out_id,
+                               int32_t out_state_id);
 
 /* ---- Layer normalisation over the last axis of a [rows, cols] view, in the decomposed
  * form a converted graph holds: y = ((x - mean) * rsqrt(var + epsilon)) * gamma + beta with

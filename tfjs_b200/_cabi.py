@@ -60,6 +60,17 @@ class MatMulParams(Structure):
             ("gelu_one", c_float), ("gelu_divide", c_int32)]
 
 
+class PagedParams(Structure):
+    _fields_ = [(n, c_int32) for n in (
+        "batch", "heads", "kv_heads", "head_dim", "num_pages", "page_size", "max_pages",
+        "tokens", "budget", "recent", "has_scale")] + [("scale", c_float)]
+
+
+class LinearAttentionParams(Structure):
+    _fields_ = [(n, c_int32) for n in (
+        "batch", "heads", "seq", "dim_k", "dim_v", "has_scale")] + [("scale", c_float)]
+
+
 STORED_RAW, STORED_UINT8, STORED_UINT16, STORED_FLOAT16 = 0, 1, 2, 3
 
 
@@ -85,6 +96,9 @@ SIGNATURES = {
     "tfjs_cuda_sync": (c_int, [_CTX]),
     "tfjs_cuda_size_of": (c_int, [_CTX, c_int32, POINTER(c_uint64)]),
     "tfjs_cuda_device_ptr": (c_int, [_CTX, c_int32, POINTER(c_void_p)]),
+    "tfjs_cuda_from_device": (c_int, [_CTX, c_void_p, c_uint64, POINTER(c_int32)]),
+    "tfjs_cuda_wait_stream": (c_int, [_CTX, c_void_p]),
+    "tfjs_cuda_signal_stream": (c_int, [_CTX, c_void_p]),
     "tfjs_cuda_memory": (c_int, [_CTX] + [POINTER(c_uint64)] * 4),
     "tfjs_cuda_trim": (c_int, [_CTX]),
     "tfjs_cuda_host_alloc": (c_int, [_CTX, c_uint64, POINTER(c_void_p)]),
@@ -132,6 +146,10 @@ SIGNATURES = {
     "tfjs_cuda_fused_attention": (c_int, [_CTX, c_int32, c_int32, c_int32, c_int32, c_int32,
                                           c_float, c_int32, c_int32, c_int32, c_int32, c_int32,
                                           c_int32]),
+    "tfjs_cuda_paged_cache_append": (c_int, [_CTX, POINTER(PagedParams)] + [c_int32] * 8),
+    "tfjs_cuda_paged_attention": (c_int, [_CTX, POINTER(PagedParams)] + [c_int32] * 9),
+    "tfjs_cuda_paged_cache_evict": (c_int, [_CTX, POINTER(PagedParams)] + [c_int32] * 11),
+    "tfjs_cuda_linear_attention": (c_int, [_CTX, POINTER(LinearAttentionParams)] + [c_int32] * 8),
     "tfjs_cuda_layer_norm": (c_int, [_CTX, c_int32, c_int32, c_int32, c_int32, c_uint64, c_uint64,
                                      c_float, c_int32]),
     "tfjs_cuda_reduce": (c_int, [_CTX, c_int32, c_int32, c_uint64, c_uint64,

@@ -75,8 +75,40 @@ class TensorInfo(object):
         return "TensorInfo(%r, %s, %s)" % (self.dataId, self.shape, self.dtype)
 
 
+class GPUData(object):
+    """A tensor's device memory (tfjs-core's GPUData, the result of tensor.dataToGPU()):
+    `buffer` is the address, `bufSize` its bytes, `tensorRef` a tensor that keeps it alive.
+    Libraries that read __cuda_array_interface__ take it without a copy.  When the last
+    reference is gone the tensor is disposed, behind the work queued on `stream` by then."""
+    __slots__ = ("backend", "tensorRef", "buffer", "bufSize", "shape", "dtype", "stream")
+    _TYPESTR = {"float32": "<f4", "int32": "<i4", "bool": "|b1"}
+
+    def __init__(self, backend, tensorRef, buffer, bufSize, stream):
+        self.backend, self.tensorRef, self.stream = backend, tensorRef, stream
+        self.buffer, self.bufSize = buffer, bufSize
+        self.shape, self.dtype = list(tensorRef.shape), tensorRef.dtype
+
+    @property
+    def __cuda_array_interface__(self):
+        return {"shape": tuple(self.shape), "typestr": self._TYPESTR[self.dtype],
+                "data": (self.buffer, False), "strides": None, "version": 2}
+
+    def dispose(self):
+        ref, self.tensorRef = self.tensorRef, None
+        if ref is not None and self.backend.ctx:
+            if self.stream is not None:
+                self.backend.wait_stream(self.stream)
+            ref.dispose()
+
+    def __del__(self):
+        try:
+            self.dispose()
+        except Exception:      # the interpreter is going away, or the device is
+            pass
+
+
 class _Record(object):
-    __slots__ = ("dev", "nbytes", "dtype", "ref", "host", "pending", "held")
+    __slots__ = ("dev", "nbytes", "dtype", "ref", "host", "pending", "held", "foreign", "stream")
 
     def __init__(self, dev, nbytes, dtype, ref, host):
         self.dev = dev        # device buffer id, 0 = not uploaded / not launched yet
@@ -86,6 +118,8 @@ class _Record(object):
         self.host = host      # numpy copy for small host-written tensors
         self.pending = None   # PendingConv / PendingAdd until the launch happens
         self.held = 0         # how many of `ref` belong to pending launches
+        self.foreign = None   # the owner of device memory that is not the backend's
+        self.stream = None    # the stream its owner works on, if it is to be ordered
 
 
 class PendingConv(object):
@@ -549,6 +583,64 @@ class CudaBackend(object):
         self.data[dataId] = _Record(self._alloc(nbytes), nbytes, dtype, 1, None)
         return TensorInfo(dataId, shape, dtype)
 
+    # -------------------------------------------------- other libraries' memory --
+    def createTensorFromGPUData(self, values, shape=None, dtype=None, stream=None):
+        """A TensorInfo over device memory that another library holds, without a copy (the
+        KernelBackend method behind tf.tensor({buffer, zeroCopy: true})).  `values` has
+        __cuda_array_interface__: contiguous float32, int32 or bool memory of this GPU.
+        `stream` (a cudaStream_t as a number, 0 = the default stream): this backend's work
+        waits for what is queued there now, and what is queued there after the tensor is
+        disposed waits for this backend's work.  Without it the caller orders the two."""
+        info = values.__cuda_array_interface__
+        typestr, strides = info["typestr"], info.get("strides")
+        found = {"<f4": "float32", "<i4": "int32", "|b1": "bool"}.get(typestr)
+        have = [int(v) for v in info["shape"]]
+        if found is None or (dtype is not None and dtype != found):
+            raise ValueError("createTensorFromGPUData: dtype %s of the memory is not %s" %
+                             (typestr, dtype or "one of float32, int32, bool"))
+        nbytes = size_from_shape(have) * np.dtype(NP_DTYPES[found]).itemsize
+        if strides is not None and nbytes:
+            step = np.dtype(NP_DTYPES[found]).itemsize
+            for n, s in zip(reversed(have), reversed(list(strides))):
+                if n != 1 and s != step:
+                    raise ValueError("createTensorFromGPUData: the memory is not contiguous "
+                                     "(shape %s, strides %s)" % (have, list(strides)))
+                step *= n
+        shape = have if shape is None else [int(v) for v in shape]
+        if size_from_shape(shape) != size_from_shape(have):
+            raise ValueError("createTensorFromGPUData: %d values for shape %s" %
+                             (size_from_shape(have), shape))
+        if stream is not None:
+            self.wait_stream(stream)
+        dev = c_int32()
+        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes, byref(dev)))
+        dataId = DataId()
+        rec = _Record(dev.value, nbytes, found, 1, None)
+        rec.foreign, rec.stream = values, stream
+        self.data[dataId] = rec
+        return TensorInfo(dataId, shape, found)
+
+    def readToGPU(self, tensor, stream=None):
+        """GPUData over `tensor`'s device memory (the KernelBackend method behind
+        tensor.dataToGPU()), without a copy; launches a pending producer first.  With `stream`,
+        what is queued there from now on runs after this backend's work."""
+        dev = self.device_id(tensor.dataId)
+        ptr = c_void_p()
+        self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
+        if stream is not None:
+            self.signal_stream(stream)
+        rec = self.data[tensor.dataId]
+        rec.host = None        # whoever holds the memory may write to it
+        return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream)
+
+    def wait_stream(self, stream):
+        """This backend's work from now on runs after what is queued on `stream`."""
+        self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, c_void_p(int(stream))))
+
+    def signal_stream(self, stream):
+        """What is queued on `stream` from now on runs after this backend's work so far."""
+        self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, c_void_p(int(stream))))
+
     # ---------------------------------------------------- deferred launches --
     def _adjust(self, rec, dref, dheld):
         """Change a record's reference counts, tracking whether only pending launches
@@ -691,6 +783,22 @@ class CudaBackend(object):
                     self.ctx, rec.dev, rec.host.ctypes.data_as(c_void_p), rec.nbytes))
         return rec.dev
 
+    def _launch_readers(self, dataId, rec):
+        """Launches what is pending on a tensor's present contents."""
+        if rec.held:
+            for other in list(self.data.values()):
+                if other.pending is not None and dataId in other.pending.deps():
+                    self._resolve(other)
+
+    def device_id_for_update(self, dataId):
+        """Device buffer id of a tensor that a kernel is about to write in place: launches
+        that are pending on its present contents happen first, and a host copy is dropped."""
+        rec = self.data[dataId]
+        self._launch_readers(dataId, rec)
+        dev = self.device_id(dataId)
+        rec.host = None
+        return dev
+
     def host_values(self, dataId):
         """Host copy if the tensor is host-resident, else None (no sync)."""
         return self.data[dataId].host
@@ -747,6 +855,9 @@ class CudaBackend(object):
         rec = self.data.get(dataId)
         if rec is None:
             return False
+        if rec.foreign is not None and rec.ref - rec.held == 1:
+            # its owner may reuse the memory from here on: pending readers launch now
+            self._launch_readers(dataId, rec)
         self._adjust(rec, -1, 0)
         if rec.ref > 0 and (not force or rec.held > 0):
             return False
@@ -757,6 +868,8 @@ class CudaBackend(object):
         if rec.held > 0 and rec.ref <= rec.held:
             self._hidden -= 1
         del self.data[dataId]
+        if rec.stream is not None:     # its owner's next work waits for what reads it here
+            self.signal_stream(rec.stream)
         if rec.dev:
             self.check(self.lib.tfjs_cuda_free(self.ctx, rec.dev))
         if rec.pending is not None:

@@ -20,6 +20,7 @@ struct Buffer {
   cudaEvent_t ready = nullptr;  // set while an upload on the copy stream is pending
   bool uploaded = false;        // block came from tfjs_cuda_upload: recycled for uploads
   bool in_arena = false;        // lives in the arena of a captured graph
+  bool foreign = false;         // the caller's memory (tfjs_cuda_from_device): never freed here
 };
 
 // A captured step (tfjs_cuda_capture_begin .. _end): the instantiated graph and the
@@ -101,6 +102,7 @@ struct tfjs_cuda_ctx {
   long long* d_bad_index = nullptr;
   long long* h_bad_index = nullptr;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;
+  cudaEvent_t ev_order = nullptr;  // orders this context against a caller's stream
   std::vector<cudaEvent_t> prof_events;  // numbered events for per-kernel timing
   std::vector<cudaEvent_t> read_events;  // tickets of tfjs_cuda_read_begin (index + 1)
   std::vector<cudaEvent_t> read_order;   // per ticket: orders the read stream behind the compute stream
@@ -123,6 +125,29 @@ Buffer* ctx_buf(tfjs_cuda_ctx* ctx, int32_t id);
 int ctx_get(tfjs_cuda_ctx* ctx, int32_t id, uint64_t need, const char* name,
             Buffer** out);
 int ctx_scratch(tfjs_cuda_ctx* ctx, uint64_t bytes, void** out);
+
+// Values of the device error word from kBadInput on name inputs that only the device can
+// check; smaller ones are waits that gave up.
+enum { kBadInput = 1000, kBadPage = 1000, kBadLength = 1001 };
+
+// A workspace of one call, from the pool (or from the arena of the step being captured): it
+// goes back in stream order when the call returns, so that nothing outside the call, a
+// captured step included, carries its address.
+struct TempBuffer {
+  tfjs_cuda_ctx* ctx;
+  int32_t id = 0;
+  explicit TempBuffer(tfjs_cuda_ctx* c) : ctx(c) {}
+  TempBuffer(const TempBuffer&) = delete;
+  TempBuffer& operator=(const TempBuffer&) = delete;
+  ~TempBuffer() {
+    if (id) tfjs_cuda_free(ctx, id);
+  }
+  int get(uint64_t bytes, void** out) {
+    int rc = tfjs_cuda_alloc(ctx, bytes, &id);
+    if (rc == TFJS_CUDA_OK) *out = ctx_buf(ctx, id)->ptr;
+    return rc;
+  }
+};
 void ctx_mark_written(tfjs_cuda_ctx* ctx, int32_t id);
 void ctx_drop_packed(tfjs_cuda_ctx* ctx, int32_t id);
 // Marks captured steps that read the packed copy of weight `id` as stale (no memory call).

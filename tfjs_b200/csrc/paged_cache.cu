@@ -1,0 +1,388 @@
+// Writing to a paged key-value cache and keeping it bounded: appending new tokens, and
+// eviction by accumulated attention weight.  Both move rows of head_dim values and compute
+// nothing, so bytes bound them: a row is read once and written once.
+#include "paged.cuh"
+
+namespace {
+
+// ---- append ------------------------------------------------------------------------------
+// k and v are [batch, kv_heads, tokens, head_dim]; the tokens of one row and head are
+// contiguous at the source, and in runs of a page's places at the destination.  V values at a
+// time: 4 where head_dim and the addresses allow 16-byte accesses, else 1.
+template <int V>
+__global__ void __launch_bounds__(256)
+paged_append_kernel(const PagedLayout g, const float* __restrict__ k, const float* __restrict__ v,
+                    const int* __restrict__ counts, float* __restrict__ k_cache,
+                    float* __restrict__ v_cache, int* __restrict__ out_lengths, int batch,
+                    int tokens, int blocks_per_head) {
+  const int unit = blockIdx.x / blocks_per_head;           // row * kv_heads + head
+  const int part = blockIdx.x - unit * blocks_per_head;
+  const int b = unit / g.kv_heads, h = unit - b * g.kv_heads;
+  const int n = paged_length(g, b);
+  int c = counts ? __ldg(counts + b) : tokens;
+  const bool bad = c < 0 || c > tokens || c > g.capacity - n;
+  if (bad) c = c < 0 ? 0 : min(min(c, tokens), g.capacity - n);
+  if (h == 0 && part == 0 && threadIdx.x == 0) {
+    if (bad) atomicExch(g.flag, kBadLength);
+    out_lengths[b] = n + c;
+  }
+  const int per_row = g.head_dim / V;
+  const uint64_t total = (uint64_t)c * per_row;
+  const uint64_t src0 = (uint64_t)unit * tokens * g.head_dim;
+  for (uint64_t i = (uint64_t)part * 256 + threadIdx.x; i < total; i += (uint64_t)blocks_per_head * 256) {
+    const int t = (int)(i / per_row);
+    const int d = (int)(i - (uint64_t)t * per_row) * V;
+    const uint32_t row = paged_row(g, b, h, n + t);
+    if (row == kNoRow) continue;
+    const uint64_t src = src0 + (uint64_t)t * g.head_dim + d;
+    const uint64_t dst = (uint64_t)row * g.head_dim + d;
+    if (V == 4) {
+      *reinterpret_cast<float4*>(k_cache + dst) = __ldg(reinterpret_cast<const float4*>(k + src));
+      *reinterpret_cast<float4*>(v_cache + dst) = __ldg(reinterpret_cast<const float4*>(v + src));
+    } else {
+      k_cache[dst] = __ldg(k + src);
+      v_cache[dst] = __ldg(v + src);
+    }
+  }
+}
+
+// ---- evict -------------------------------------------------------------------------------
+constexpr int kSelThreads = 1024;
+
+struct EvictArgs {
+  const float* weights;     // [batch, kv_heads, capacity]
+  const int* positions;     // or null
+  const int* total;         // [batch], or null
+  float* out_weights;
+  int* out_positions;
+  int* out_lengths;
+  int* out_kept;            // [batch, kv_heads, budget]
+  int* moves;               // [units]: how many slots move
+  int* holes;               // [units][list]: where to, ascending
+  int* tails;               // [units][list]: where from, ascending
+  int list;                 // min(budget, capacity)
+  int budget, recent;
+};
+
+// Weights as unsigned numbers of the same order: NaN above all, -0 equal to +0.
+__device__ __forceinline__ uint32_t ordered(float w) {
+  if (w != w) return 0xfffffffeu;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+
+struct SlotView {
+  const float* w;
+  const int* pos;     // null: by the slot
+  long long total, n, first_recent;
+  __device__ __forceinline__ long long position(int j) const {
+    if (pos) {
+      const int p = __ldg(pos + j);
+      if (p >= 0) return p;
+    }
+    return total - (n - j);
+  }
+  // The recent ones first, whatever their weight.
+  __device__ __forceinline__ uint32_t key(int j) const {
+    return position(j) >= first_recent ? 0xffffffffu : ordered(__ldg(w + j));
+  }
+};
+
+// Exclusive sum over the block of one value a thread, and the block's total.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t mine = warp_sums[lane];
+    uint32_t t = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += u;
+    }
+    warp_sums[lane] = t - mine;
+    if (lane == 31) warp_sums[32] = t;
+  }
+  __syncthreads();
+  const uint32_t r = warp_sums[warp] + s - v;
+  *total = warp_sums[32];
+  __syncthreads();   // warp_sums is reused by the next call
+  return r;
+}
+
+// One block decides for one row and head which slots stay: the m-th largest key by a radix
+// select of 8 bits a pass (counting, no sorting), then one pass in slot order that ranks the
+// slots equal to it, the free places below m and the kept slots from m on.
+__global__ void __launch_bounds__(kSelThreads)
+paged_evict_select_kernel(const PagedLayout g, const EvictArgs a) {
+  __shared__ uint32_t hist[256];
+  __shared__ uint32_t warp_sums[33];
+  __shared__ uint32_t pick[2];
+  const int unit = blockIdx.x;
+  const int b = unit / g.kv_heads;
+  const int tid = threadIdx.x;
+  const int n = paged_length(g, b);
+  const int m = min(n, a.budget);
+  const uint64_t base = (uint64_t)unit * g.capacity;
+  SlotView s;
+  s.w = a.weights + base;
+  s.pos = a.positions ? a.positions + base : nullptr;
+  s.n = n;
+  s.total = a.total ? __ldg(a.total + b) : n;
+  s.first_recent = s.total - a.recent;
+  float* ow = a.out_weights + base;
+  int* op = a.out_positions + base;
+  int* ok = a.out_kept + (uint64_t)unit * a.budget;
+  if (unit == b * g.kv_heads && tid == 0) a.out_lengths[b] = m;
+  for (int j = m + tid; j < g.capacity; j += kSelThreads) {
+    ow[j] = 0.0f;
+    op[j] = -1;
+  }
+  for (int j = m + tid; j < a.budget; j += kSelThreads) ok[j] = -1;
+  if (n <= m) {   // nothing to lose
+    for (int j = tid; j < m; j += kSelThreads) {
+      ow[j] = __ldg(s.w + j);
+      op[j] = (int)s.position(j);
+      ok[j] = j;
+    }
+    if (tid == 0) a.moves[unit] = 0;
+    return;
+  }
+  // the key that the m-th largest has, and how many of the slots that have it stay
+  uint32_t prefix = 0, mask = 0;
+  uint32_t want = (uint32_t)m;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    for (int j = tid; j < n; j += kSelThreads) {
+      const uint32_t key = s.key(j);
+      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+    }
+    __syncthreads();
+    if (tid < 32) {
+      // lane l: the eight digits below 256 - 8 l, from the top
+      uint32_t c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        c[i] = hist[255 - (tid * 8 + i)];
+        sum += c[i];
+      }
+      uint32_t before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, before, o);
+        if (tid >= o) before += u;
+      }
+      before -= sum;
+      if (before < want && want <= before + sum) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (before < want && want <= before + c[i]) {
+            pick[0] = 255u - (uint32_t)(tid * 8 + i);
+            pick[1] = want - before;
+          }
+          before += c[i];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= pick[0] << shift;
+    want = pick[1];
+    mask |= 255u << shift;
+  }
+  // in slot order: slots equal to the threshold stay while `want` lasts
+  uint32_t equal_seen = 0, holes = 0, tails = 0;
+  int* hole_list = a.holes + (uint64_t)unit * a.list;
+  int* tail_list = a.tails + (uint64_t)unit * a.list;
+  for (int j0 = 0; j0 < n; j0 += kSelThreads) {
+    const int j = j0 + tid;
+    const uint32_t key = j < n ? s.key(j) : 0u;
+    const bool equal = j < n && key == prefix;
+    uint32_t all;
+    const uint32_t rank = equal_seen + block_scan(equal, warp_sums, &all);
+    equal_seen += all;
+    const bool keep = j < n && (key > prefix || (equal && rank < want));
+    const bool hole = j < m && !keep, tail = j >= m && keep;
+    const uint32_t r = block_scan((hole ? 1u : 0u) | (tail ? 0x10000u : 0u), warp_sums, &all);
+    if (hole) hole_list[holes + (r & 0xffffu)] = j;
+    if (tail) tail_list[tails + (r >> 16)] = j;
+    if (keep && j < m) {
+      ow[j] = __ldg(s.w + j);
+      op[j] = (int)s.position(j);
+      ok[j] = j;
+    }
+    holes += all & 0xffffu;
+    tails += all >> 16;
+  }
+  __syncthreads();   // the lists of this block, written above, are read by other threads below
+  for (uint32_t r = tid; r < holes; r += kSelThreads) {
+    const int to = hole_list[r], from = tail_list[r];
+    ow[to] = __ldg(s.w + from);
+    op[to] = (int)s.position(from);
+    ok[to] = from;
+  }
+  if (tid == 0) a.moves[unit] = (int)holes;
+}
+
+// The rows of the kept slots: sources are slots from m on, destinations slots below m, so no
+// move touches another's source.
+template <int V>
+__global__ void __launch_bounds__(256)
+paged_evict_move_kernel(const PagedLayout g, const int* __restrict__ moves,
+                        const int* __restrict__ holes, const int* __restrict__ tails, int list,
+                        float* __restrict__ k_cache, float* __restrict__ v_cache,
+                        int blocks_per_unit) {
+  const int unit = blockIdx.x / blocks_per_unit;
+  const int part = blockIdx.x - unit * blocks_per_unit;
+  const int b = unit / g.kv_heads, h = unit - b * g.kv_heads;
+  const int count = __ldg(moves + unit);
+  const int lane = threadIdx.x & 31;
+  for (int r = part * 8 + (threadIdx.x >> 5); r < count; r += blocks_per_unit * 8) {
+    const uint32_t from = paged_row(g, b, h, __ldg(tails + (uint64_t)unit * list + r));
+    const uint32_t to = paged_row(g, b, h, __ldg(holes + (uint64_t)unit * list + r));
+    if (from == kNoRow || to == kNoRow) continue;
+    for (int d = lane * V; d < g.head_dim; d += 32 * V) {
+      const uint64_t src = (uint64_t)from * g.head_dim + d, dst = (uint64_t)to * g.head_dim + d;
+      if (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(k_cache + src);
+        const float4 y = *reinterpret_cast<const float4*>(v_cache + src);
+        *reinterpret_cast<float4*>(k_cache + dst) = x;
+        *reinterpret_cast<float4*>(v_cache + dst) = y;
+      } else {
+        const float x = k_cache[src], y = v_cache[src];
+        k_cache[dst] = x;
+        v_cache[dst] = y;
+      }
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int tfjs_cuda_paged_cache_append(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params* p,
+                                 int32_t k_cache_id, int32_t v_cache_id, int32_t k_id,
+                                 int32_t v_id, int32_t page_table_id, int32_t lengths_id,
+                                 int32_t counts_id, int32_t out_lengths_id) {
+  if (!ctx) return TFJS_CUDA_INVALID_ARG;
+  const char* who = "paged cache append";
+  PagedLayout g;
+  Buffer *kc, *vc, *k, *v, *counts = nullptr, *ol;
+  int rc = paged_layout(ctx, p, who, k_cache_id, v_cache_id, page_table_id, lengths_id, &g, &kc, &vc);
+  if (rc) return rc;
+  if (p->tokens <= 0)
+    return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: dimensions must be positive", who);
+  const uint64_t units = (uint64_t)p->batch * p->kv_heads;
+  const uint64_t n = units * p->tokens * (uint64_t)p->head_dim;
+  if ((rc = ctx_get(ctx, k_id, n * 4, who, &k))) return rc;
+  if ((rc = ctx_get(ctx, v_id, n * 4, who, &v))) return rc;
+  if (counts_id && (rc = ctx_get(ctx, counts_id, (uint64_t)p->batch * 4, who, &counts))) return rc;
+  if ((rc = ctx_get(ctx, out_lengths_id, (uint64_t)p->batch * 4, who, &ol))) return rc;
+  if (out_lengths_id == lengths_id || k_id == k_cache_id || k_id == v_cache_id ||
+      v_id == k_cache_id || v_id == v_cache_id)
+    return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is also an input", who);
+  cudaSetDevice(ctx->device);
+  const bool wide = p->head_dim % 4 == 0 &&
+                    (((uintptr_t)kc->ptr | (uintptr_t)vc->ptr | (uintptr_t)k->ptr | (uintptr_t)v->ptr) & 15) == 0;
+  const uint64_t items = (uint64_t)p->tokens * (p->head_dim / (wide ? 4 : 1));
+  // a block handles up to four items a thread of one row and head
+  uint64_t per = (items + 1023) / 1024;
+  if (per > 0x7fffffffull / units) per = 0x7fffffffull / units;
+  const unsigned grid = (unsigned)(units * per);
+  const int* ct = counts ? (const int*)counts->ptr : nullptr;
+  if (wide)
+    paged_append_kernel<4><<<grid, 256, 0, ctx->stream>>>(
+        g, (const float*)k->ptr, (const float*)v->ptr, ct, (float*)kc->ptr, (float*)vc->ptr,
+        (int*)ol->ptr, p->batch, p->tokens, (int)per);
+  else
+    paged_append_kernel<1><<<grid, 256, 0, ctx->stream>>>(
+        g, (const float*)k->ptr, (const float*)v->ptr, ct, (float*)kc->ptr, (float*)vc->ptr,
+        (int*)ol->ptr, p->batch, p->tokens, (int)per);
+  LAUNCH_CHECK(ctx, wide ? "paged_append_kernel<4>" : "paged_append_kernel<1>");
+  ctx_mark_written(ctx, k_cache_id);
+  ctx_mark_written(ctx, v_cache_id);
+  ctx_mark_written(ctx, out_lengths_id);
+  return TFJS_CUDA_OK;
+}
+
+int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params* p,
+                                int32_t k_cache_id, int32_t v_cache_id, int32_t weights_id,
+                                int32_t page_table_id, int32_t lengths_id, int32_t positions_id,
+                                int32_t total_id, int32_t out_weights_id,
+                                int32_t out_positions_id, int32_t out_lengths_id,
+                                int32_t out_kept_id) {
+  if (!ctx) return TFJS_CUDA_INVALID_ARG;
+  const char* who = "paged cache evict";
+  PagedLayout g;
+  Buffer *kc, *vc, *w, *pos = nullptr, *tot = nullptr, *ow, *op, *ol, *ok;
+  int rc = paged_layout(ctx, p, who, k_cache_id, v_cache_id, page_table_id, lengths_id, &g, &kc, &vc);
+  if (rc) return rc;
+  if (p->budget <= 0 || p->recent < 0 || p->recent > p->budget)
+    return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG,
+                    "%s: the budget must be positive and hold the recent slots", who);
+  const uint64_t units = (uint64_t)p->batch * p->kv_heads;
+  const uint64_t slots = units * (uint64_t)g.capacity * 4;
+  if ((rc = ctx_get(ctx, weights_id, slots, who, &w))) return rc;
+  if (positions_id && (rc = ctx_get(ctx, positions_id, slots, who, &pos))) return rc;
+  if (total_id && (rc = ctx_get(ctx, total_id, (uint64_t)p->batch * 4, who, &tot))) return rc;
+  if ((rc = ctx_get(ctx, out_weights_id, slots, who, &ow))) return rc;
+  if ((rc = ctx_get(ctx, out_positions_id, slots, who, &op))) return rc;
+  if ((rc = ctx_get(ctx, out_lengths_id, (uint64_t)p->batch * 4, who, &ol))) return rc;
+  if ((rc = ctx_get(ctx, out_kept_id, units * (uint64_t)p->budget * 4, who, &ok))) return rc;
+  const int32_t in[] = {k_cache_id, v_cache_id, weights_id, page_table_id, lengths_id, positions_id, total_id};
+  const int32_t out[] = {out_weights_id, out_positions_id, out_lengths_id, out_kept_id};
+  for (int i = 0; i < 4; ++i) {
+    for (int32_t x : in)
+      if (out[i] == x) return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is also an input", who);
+    for (int j = 0; j < i; ++j)
+      if (out[i] == out[j]) return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is given twice", who);
+  }
+  float *kp = (float*)kc->ptr, *vp = (float*)vc->ptr;
+  EvictArgs a;
+  a.weights = (const float*)w->ptr;
+  a.positions = pos ? (const int*)pos->ptr : nullptr;
+  a.total = tot ? (const int*)tot->ptr : nullptr;
+  a.out_weights = (float*)ow->ptr;
+  a.out_positions = (int*)op->ptr;
+  a.out_lengths = (int*)ol->ptr;
+  a.out_kept = (int*)ok->ptr;
+  a.budget = p->budget;
+  a.recent = p->recent;
+  a.list = p->budget < g.capacity ? p->budget : g.capacity;
+  cudaSetDevice(ctx->device);
+  TempBuffer ws(ctx);
+  void* mem;
+  if ((rc = ws.get(units * (1 + 2 * (uint64_t)a.list) * 4, &mem))) return rc;   // (Buffer pointers end here)
+  a.moves = (int*)mem;
+  a.holes = a.moves + units;
+  a.tails = a.holes + units * a.list;
+  paged_evict_select_kernel<<<(unsigned)units, kSelThreads, 0, ctx->stream>>>(g, a);
+  LAUNCH_CHECK(ctx, "paged_evict_select_kernel");
+  // at most min(budget, capacity - budget) slots of a row move
+  const int most = g.capacity - p->budget < a.list ? g.capacity - p->budget : a.list;
+  if (most > 0) {
+    uint64_t per = ((uint64_t)most + 31) / 32;
+    if (per * units > (uint64_t)ctx->sm_count * 32) per = ((uint64_t)ctx->sm_count * 32 + units - 1) / units;
+    const bool wide = p->head_dim % 4 == 0 && (((uintptr_t)kp | (uintptr_t)vp) & 15) == 0;
+    const unsigned grid = (unsigned)(units * per);
+    if (wide)
+      paged_evict_move_kernel<4><<<grid, 256, 0, ctx->stream>>>(g, a.moves, a.holes, a.tails, a.list, kp, vp, (int)per);
+    else
+      paged_evict_move_kernel<1><<<grid, 256, 0, ctx->stream>>>(g, a.moves, a.holes, a.tails, a.list, kp, vp, (int)per);
+    LAUNCH_CHECK(ctx, wide ? "paged_evict_move_kernel<4>" : "paged_evict_move_kernel<1>");
+  }
+  ctx_mark_written(ctx, k_cache_id);
+  ctx_mark_written(ctx, v_cache_id);
+  for (int32_t id : out) ctx_mark_written(ctx, id);
+  return TFJS_CUDA_OK;
+}
+
+}  // extern "C"

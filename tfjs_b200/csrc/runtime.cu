@@ -231,6 +231,7 @@ int tfjs_cuda_create(int device_ordinal, tfjs_cuda_ctx** out_ctx) {
   ok = ok && cudaMallocHost(&ctx->h_bad_index, sizeof(long long)) == cudaSuccess;
   ok = ok && cudaEventCreate(&ctx->ev0) == cudaSuccess;
   ok = ok && cudaEventCreate(&ctx->ev1) == cudaSuccess;
+  ok = ok && cudaEventCreateWithFlags(&ctx->ev_order, cudaEventDisableTiming) == cudaSuccess;
   if (!ok) {
     fprintf(stderr, "tfjs_cuda: context setup failed: %s\n",
             cudaGetErrorString(cudaGetLastError()));
@@ -250,7 +251,7 @@ void tfjs_cuda_destroy(tfjs_cuda_ctx* ctx) {
   for (auto& kv : ctx->packed)
     if (kv.second.ptr) cudaFreeAsync(kv.second.ptr, ctx->stream);
   for (auto& b : ctx->bufs)
-    if (b.live && b.ptr) cudaFreeAsync(b.ptr, ctx->stream);
+    if (b.live && b.ptr && !b.foreign) cudaFreeAsync(b.ptr, ctx->stream);
   cache_flush(ctx);
   if (ctx->scratch) cudaFreeAsync(ctx->scratch, ctx->stream);
   if (ctx->l2_scratch) cudaFreeAsync(ctx->l2_scratch, ctx->stream);
@@ -284,6 +285,7 @@ void tfjs_cuda_destroy(tfjs_cuda_ctx* ctx) {
   }
   if (ctx->ev0) cudaEventDestroy(ctx->ev0);
   if (ctx->ev1) cudaEventDestroy(ctx->ev1);
+  if (ctx->ev_order) cudaEventDestroy(ctx->ev_order);
   if (ctx->stream) cudaStreamDestroy(ctx->stream);
   delete ctx;
 }
@@ -344,6 +346,15 @@ int tfjs_cuda_free(tfjs_cuda_ctx* ctx, int32_t id) {
     cudaStreamWaitEvent(ctx->stream, b->ready, 0);
     ctx->event_pool.push_back(b->ready);
     b->ready = nullptr;
+  }
+  if (b->foreign) {
+    b->foreign = false;
+    b->ptr = nullptr;
+    b->live = false;
+    b->bytes = 0;
+    ctx->n_live--;
+    ctx->free_ids.push_back(id);
+    return TFJS_CUDA_OK;
   }
   uint64_t padded = ((b->bytes + 255) / 256) * 256;
   if (padded == 0) padded = 256;
@@ -498,6 +509,12 @@ static int report_flag(tfjs_cuda_ctx* ctx, int* host_word) {
   if (*host_word != 0) {
     int v = *host_word;
     *host_word = 0;
+    if (v >= kBadInput)
+      return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s",
+                      v == kBadPage ? "a kernel needed a page that its page table does not name "
+                                      "(outside the pool); the slots of that page were left out"
+                                    : "a row's length is outside what its tensors hold; it was "
+                                      "clamped");
     // a K-split GEMM that gave up may have left partial-tile flags raised
     if (ctx->sk_flags) cudaMemsetAsync(ctx->sk_flags, 0, 4096 * sizeof(unsigned), ctx->stream);
     return ctx_fail(ctx, TFJS_CUDA_DEVICE_TIMEOUT,
@@ -656,6 +673,69 @@ int tfjs_cuda_device_ptr(tfjs_cuda_ctx* ctx, int32_t id, void** out_ptr) {
   if (!b) return ctx_fail(ctx, TFJS_CUDA_UNKNOWN_ID, "device_ptr: unknown tensor id %d", id);
   *out_ptr = b->ptr;
   return TFJS_CUDA_OK;
+}
+
+int tfjs_cuda_from_device(tfjs_cuda_ctx* ctx, void* ptr, uint64_t nbytes, int32_t* out_id) {
+  if (!ctx || !out_id) return TFJS_CUDA_INVALID_ARG;
+  *out_id = 0;
+  if (nbytes && !ptr) return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "from_device: null pointer");
+  if ((uintptr_t)ptr & 15)
+    return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "from_device: the memory is not 16-byte aligned");
+  cudaSetDevice(ctx->device);
+  if (nbytes) {
+    cudaPointerAttributes at;
+    CUDA_TRY(ctx, cudaPointerGetAttributes(&at, ptr));
+    if ((at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ||
+        at.device != ctx->device)
+      return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG,
+                      "from_device: not device memory of GPU %d", ctx->device);
+  }
+  int32_t id;
+  if (!ctx->free_ids.empty()) {
+    id = ctx->free_ids.back();
+    ctx->free_ids.pop_back();
+  } else {
+    id = (int32_t)ctx->bufs.size();
+    ctx->bufs.emplace_back();
+  }
+  Buffer& b = ctx->bufs[id];
+  b.ptr = ptr;
+  b.bytes = nbytes;
+  b.live = true;
+  b.from_host = false;   // its owner may rewrite it at any time: never packed once and kept
+  b.foreign = true;
+  b.version++;
+  ctx->n_live++;
+  *out_id = id;
+  return TFJS_CUDA_OK;
+}
+
+// `before` is recorded and `after` made to wait for that point.
+static int order_streams(tfjs_cuda_ctx* ctx, cudaStream_t before, cudaStream_t after,
+                         cudaStream_t foreign) {
+  cudaSetDevice(ctx->device);
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(foreign, &st);
+  if (e != cudaSuccess || st != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return ctx_fail(ctx, TFJS_CUDA_UNSUPPORTED,
+                    "the caller's stream is unusable or being captured");
+  }
+  CUDA_TRY(ctx, cudaEventRecord(ctx->ev_order, before));
+  CUDA_TRY(ctx, cudaStreamWaitEvent(after, ctx->ev_order, 0));
+  return TFJS_CUDA_OK;
+}
+
+int tfjs_cuda_wait_stream(tfjs_cuda_ctx* ctx, void* stream) {
+  if (!ctx) return TFJS_CUDA_INVALID_ARG;
+  NOT_WHILE_CAPTURING(ctx, "waiting for a caller's stream");
+  return order_streams(ctx, (cudaStream_t)stream, ctx->stream, (cudaStream_t)stream);
+}
+
+int tfjs_cuda_signal_stream(tfjs_cuda_ctx* ctx, void* stream) {
+  if (!ctx) return TFJS_CUDA_INVALID_ARG;
+  NOT_WHILE_CAPTURING(ctx, "signalling a caller's stream");
+  return order_streams(ctx, ctx->stream, (cudaStream_t)stream, (cudaStream_t)stream);
 }
 
 int tfjs_cuda_memory(tfjs_cuda_ctx* ctx, uint64_t* bytes_in_use,

@@ -51,6 +51,20 @@ class Tensor(object):
     def arraySync(self):
         return self.dataSync().reshape(self.shape)
 
+    def dataToGPU(self, stream=None):
+        """tensor.dataToGPU(): the tensor's device memory as GPUData, without a copy.  The
+        result keeps the memory alive on its own; this handle may be disposed.  `stream`:
+        what is queued on that stream from now on runs after the kernels launched so far."""
+        self._check()
+        info = self.info()
+        self._engine.backend.incRef(self.dataId)
+        ref = self._engine.make_tensor_from_info(info)
+        try:
+            return self._engine.backend.readToGPU(ref, stream)
+        except Exception:
+            ref.dispose()
+            raise
+
     def dispose(self):
         """engine.ts:917-943."""
         if self.isDisposed:
@@ -125,9 +139,13 @@ class Engine(object):
             self.backend = None
 
     # ----------------------------------------------------------- tensors --
-    def make_tensor(self, values, shape=None, dtype=None):
-        """engine.ts:803-827 -> backend.write."""
+    def make_tensor(self, values, shape=None, dtype=None, stream=None):
+        """engine.ts:803-827 -> backend.write; device memory of another library (anything
+        with __cuda_array_interface__) becomes a tensor without a copy."""
         self.ready()
+        if hasattr(values, "__cuda_array_interface__"):
+            return self.make_tensor_from_info(
+                self.backend.createTensorFromGPUData(values, shape, dtype, stream))
         arr = np.asarray(values)
         if dtype is None:
             if arr.dtype == np.bool_:

@@ -13,8 +13,11 @@ from .engine import ENGINE, Tensor
 from .util import size_from_shape
 
 
-def tensor(values, shape=None, dtype=None):
-    return ENGINE.make_tensor(values, shape, dtype)
+def tensor(values, shape=None, dtype=None, stream=None):
+    """A tensor from host values, or over another library's device memory (anything with
+    __cuda_array_interface__) without a copy; `stream` orders the latter against the stream
+    its owner works on (CudaBackend.createTensorFromGPUData)."""
+    return ENGINE.make_tensor(values, shape, dtype, stream)
 
 
 def _t(x, dtype=None):
@@ -318,6 +321,73 @@ def fused_attention(q, k, v, scale=None, mask=None):
     reference's ops (the graph executor substitutes it for batchMatMul + mul + add + softmax
     + batchMatMul + transpose); raises CudaError(UNSUPPORTED) for shapes it does not take."""
     return _run("_FusedAttention", {"q": q, "k": k, "v": v, "mask": mask}, {"scale": scale})
+
+
+def paged_cache_append(kCache, vCache, k, v, pageTable, lengths, counts=None):
+    """Writes new tokens into a paged key-value cache, in place, and returns the rows' new
+    lengths.
+
+    kCache, vCache [numPages, kvHeads, pageSize, headDim] float32 are the pools; pageTable
+    [batch, maxPages] int32 lists each row's pages, lengths [batch] int32 how many slots it
+    fills.  k, v [batch, kvHeads, tokens, headDim] (the heads-split store of a projection) go
+    to the slots from lengths[b] on; counts [batch] int32 says how many tokens of each row
+    are real (a padded batch), all by default.  Tokens beyond maxPages * pageSize slots are
+    dropped, and places whose page is not in the pool skipped; the next blocking read reports
+    either.  A kernel of the 'cuda' backend with no counterpart among the reference's ops."""
+    return _run("_PagedCacheAppend", {"kCache": kCache, "vCache": vCache, "k": k, "v": v,
+                                      "pageTable": pageTable, "lengths": lengths,
+                                      "counts": counts})
+
+
+def paged_attention(q, kCache, vCache, pageTable, lengths, scale=None, mask=None, weights=None):
+    """softmax(q k^T * scale + mask) v of one new token over a paged key-value cache.
+
+    q [batch, heads, 1, headDim]; heads is a multiple of the pools' kvHeads, and query head h
+    reads key-value head h // (heads // kvHeads).  mask [batch, maxPages * pageSize] is added
+    to the scores; -infinity hides a slot.  Returns [batch, 1, heads, headDim] (as
+    fused_attention does for a sequence); a row with nothing to attend to gives zeros.  With
+    weights [batch, kvHeads, maxPages * pageSize], which accumulates each slot's attention for
+    paged_cache_evict, returns [out, newWeights]; newWeights is 0 behind a row's length.
+    The token's own key and value are appended before.  A kernel of the 'cuda' backend with
+    no counterpart among the reference's ops."""
+    return _run("_PagedAttention", {"q": q, "kCache": kCache, "vCache": vCache,
+                                    "pageTable": pageTable, "lengths": lengths, "mask": mask,
+                                    "weights": weights}, {"scale": scale})
+
+
+def paged_cache_evict(kCache, vCache, weights, pageTable, lengths, budget, recent=0,
+                      positions=None, total=None):
+    """Cuts every row and key-value head of a paged cache down to `budget` slots: the
+    `recent` latest tokens stay, then those of the largest accumulated weight (NaN counts as
+    the largest; among equals the lower slot stays).
+
+    The pools are updated in place: kept slots behind the budget move into the places that
+    become free, so slots are no longer in the order of their tokens.  positions [batch,
+    kvHeads, maxPages * pageSize] int32 says which token each slot holds; entries below 0
+    (and all of them when it is absent) stand for tokens appended in order: total[b] -
+    (lengths[b] - slot), with total [batch] int32 the tokens a row has seen (default: its
+    length).  Returns [weights, positions, lengths, kept]: the slots' weights and positions
+    after the move (0 and -1 behind the new length), the new lengths min(lengths, budget),
+    and kept [batch, kvHeads, budget] int32, the slot each one came from (-1 behind the new
+    length).  A kernel of the 'cuda' backend with no counterpart among the reference's ops."""
+    return _run("_PagedCacheEvict", {"kCache": kCache, "vCache": vCache, "weights": weights,
+                                     "pageTable": pageTable, "lengths": lengths,
+                                     "positions": positions, "total": total},
+                {"budget": budget, "recent": recent})
+
+
+def linear_attention(q, k, v, logDecay, state=None, scale=None, lengths=None):
+    """Linear attention with a decay for each head: S_t = exp(logDecay[h]) S_{t-1} + k_t v_t^T,
+    out_t = scale * q_t S_t.
+
+    q, k [batch, heads, seq, dimK], v [batch, heads, seq, dimV], logDecay [heads], state
+    [batch, heads, dimK, dimV] (zeros if absent).  lengths [batch] int32 gives the tokens of
+    each row of a padded batch; what is behind them does not enter and gives zeros.  Returns
+    [out, newState] with out [batch, seq, heads, dimV].  seq = 1 is one step of generation,
+    longer inputs are prompts, in one call or in pieces that hand the state on.  A kernel of
+    the 'cuda' backend with no counterpart among the reference's ops."""
+    return _run("_LinearAttention", {"q": q, "k": k, "v": v, "logDecay": logDecay,
+                                     "state": state, "lengths": lengths}, {"scale": scale})
 
 
 def fused_layer_norm(x, gamma, beta, epsilon, residual=None):
