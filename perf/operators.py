@@ -314,9 +314,18 @@ def _linear(s):
 
 
 # ------------------------------------------------------------ the framework's calls --
+class _Held(dict):
+    """The framework's tensors over device memory that a program keeps from step to step;
+    disposed with the program's state."""
+
+    def __del__(self):
+        for t in self.values():
+            if t is not None:
+                t.dispose()
+
+
 def _handle(tf, s, name):
-    """The framework's tensor over device memory that a program keeps from step to step."""
-    held = s.setdefault("held", {})
+    held = s.setdefault("held", _Held())
     if name not in held:
         held[name] = tf.tensor(s[name]) if s[name] is not None else None
     return held[name]
@@ -356,7 +365,7 @@ def _run_own(s):
                 *pools, _handle(tf, s, "weights"), table, lengths, case["budget"], case["recent"],
                 _handle(tf, s, "positions"), _handle(tf, s, "total"))
     result = {name: torch.as_tensor(t.dataToGPU(stream), device=DEV) for name, t in out.items()}
-    for t in new:
+    for t in new + list(out.values()):
         t.dispose()
     if case["op"] in ("append", "evict"):
         result["k_cache"], result["v_cache"] = s["k_cache"], s["v_cache"]
