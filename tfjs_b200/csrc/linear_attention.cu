@@ -1,30 +1,12 @@
 // Linear attention with a decay for each head:
 //   S_t = g S_{t-1} + k_t v_t^T,  out_t = scale q_t S_t,  g = exp(log_decay)
-// as a recurrence over the tokens, the state in registers.
-#include "common.cuh"
+// This file: the entry point and the recurrence over the tokens, the state in registers; prompts
+// run in chunks (linear_attention_sm100.cu).
+#include "linear_attention.h"
 
 namespace {
 
-struct LinearArgs {
-  const float *q, *k, *v, *log_decay, *state;   // state: or null
-  const int* lengths;                           // or null
-  float *out, *out_state;
-  int heads, seq, dk, dv, tiles;
-  int has_scale;
-  float scale;
-  int* flag;
-};
-
-__device__ __forceinline__ int linear_length(const LinearArgs& a, int b) {
-  if (!a.lengths) return a.seq;
-  const int n = __ldg(a.lengths + b);
-  if (n < 0 || n > a.seq) {
-    atomicExch(a.flag, kBadLength);
-    return n < 0 ? 0 : a.seq;
-  }
-  return n;
-}
-
+constexpr int kFewTokens = 8;   // up to here the recurrence, one dependent step a token
 constexpr int kTileV = 32;      // columns of the state that a block holds
 constexpr int kRowGroups = 32;  // threads that share a column's rows
 
@@ -33,9 +15,9 @@ constexpr int kRowGroups = 32;  // threads that share a column's rows
 // tokens, where reading and writing the state is all there is.
 template <int NR>
 __global__ void __launch_bounds__(256)
-linear_recurrent_kernel(const LinearArgs a) {
+linear_recurrent_kernel(const LinearArgs a, int tiles) {
   __shared__ __align__(16) float part[8][kTileV];
-  const int unit = blockIdx.x / a.tiles, tile = blockIdx.x - unit * a.tiles;
+  const int unit = blockIdx.x / tiles, tile = blockIdx.x - unit * tiles;
   const int b = unit / a.heads, h = unit - b * a.heads;
   const int n = linear_length(a, b);
   const int r = threadIdx.x >> 3, c0 = tile * kTileV + (threadIdx.x & 7) * 4;
@@ -138,6 +120,7 @@ extern "C" int tfjs_cuda_linear_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_li
   a.lengths = n ? (const int*)n->ptr : nullptr;
   a.out = (float*)out->ptr;
   a.out_state = (float*)os->ptr;
+  a.batch = p->batch;
   a.heads = p->heads;
   a.seq = p->seq;
   a.dk = p->dim_k;
@@ -145,15 +128,22 @@ extern "C" int tfjs_cuda_linear_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_li
   a.has_scale = p->has_scale;
   a.scale = p->scale;
   a.flag = ctx->d_flag;
-  a.tiles = (p->dim_v + kTileV - 1) / kTileV;
   cudaSetDevice(ctx->device);
-  const unsigned grid = (unsigned)(units * a.tiles);
+  if (p->seq > kFewTokens) {
+    rc = launch_linear_chunked(ctx, a);
+    if (rc) return rc;
+    ctx_mark_written(ctx, out_id);
+    ctx_mark_written(ctx, out_state_id);
+    return TFJS_CUDA_OK;
+  }
+  const int tiles = (p->dim_v + kTileV - 1) / kTileV;
+  const unsigned grid = (unsigned)(units * tiles);
   if (p->dim_k <= 64)
-    linear_recurrent_kernel<2><<<grid, 256, 0, ctx->stream>>>(a);
+    linear_recurrent_kernel<2><<<grid, 256, 0, ctx->stream>>>(a, tiles);
   else if (p->dim_k <= 128)
-    linear_recurrent_kernel<4><<<grid, 256, 0, ctx->stream>>>(a);
+    linear_recurrent_kernel<4><<<grid, 256, 0, ctx->stream>>>(a, tiles);
   else
-    linear_recurrent_kernel<8><<<grid, 256, 0, ctx->stream>>>(a);
+    linear_recurrent_kernel<8><<<grid, 256, 0, ctx->stream>>>(a, tiles);
   LAUNCH_CHECK(ctx, "linear_recurrent_kernel");
   ctx_mark_written(ctx, out_id);
   ctx_mark_written(ctx, out_state_id);

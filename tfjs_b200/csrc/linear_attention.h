@@ -1,0 +1,36 @@
+// What the two forms of linear attention (linear_attention.cu: one token after the other;
+// linear_attention_sm100.cu: chunks of 128 tokens on the tensor cores) share.
+#pragma once
+#include "common.cuh"
+
+struct LinearArgs {
+  const float *q, *k, *v, *log_decay, *state;   // state: or null
+  const int* lengths;                           // or null
+  float *out, *out_state;
+  int batch, heads, seq, dk, dv;
+  int has_scale;
+  float scale;
+  int* flag;
+};
+
+int launch_linear_chunked(tfjs_cuda_ctx* ctx, const LinearArgs& a);
+
+namespace {
+
+// Tokens of row b, clamped to [0, seq]; a length outside that is reported.
+__device__ __forceinline__ int linear_length(const LinearArgs& a, int b) {
+  if (!a.lengths) return a.seq;
+  const int n = __ldg(a.lengths + b);
+  if (n < 0 || n > a.seq) {
+    atomicExch(a.flag, kBadLength);
+    return n < 0 ? 0 : a.seq;
+  }
+  return n;
+}
+
+// decay^e for a whole number e >= 0 (decay 0 included: 0^0 = 1)
+__device__ __forceinline__ float decay_power(float log_decay, int e) {
+  return e == 0 ? 1.0f : expf(__fmul_rn(log_decay, (float)e));
+}
+
+}  // namespace

@@ -1,0 +1,733 @@
+// Linear attention with a decay for each head, in chunks of 128 tokens on the tensor cores.
+// With g = exp(log_decay) and S the state in front of a chunk, its tokens t = 0 .. 127 give
+//   out_t = scale * ( sum_{j <= t} g^(t-j) (q_t . k_j) v_j  +  g^(t+1) q_t S )
+// and the chunk leaves  g^128 S + A,  A = sum_j g^(127-j) k_j v_j^T.  Three launches:
+//   chunk_states   A^T of every chunk (tokens are the K dimension of the product)
+//   chunk_scan     A^T of chunk c is replaced by the state in front of it, chunk after chunk,
+//                  elementwise; what is left over is the new state
+//   chunk_outputs  Q [K; S^T]^T, the decayed lower triangle of its left half, times V, on top of
+//                  the decayed right half
+// so that all chunks of all rows and heads run at once; the states between them are kept
+// transposed, [dim_v][dim_k], which is what the last kernel's B operand wants.
+//
+// Products of fp32 values on TF32 tensor cores: every operand x is stored as hi = x rounded to
+// 11 bits and lo = x - hi, and hi hi + hi lo + lo hi is accumulated in fp32, which leaves out
+// about 2^-22 of each product.  The tensor core cuts its sums off instead of rounding them, a
+// bias of about 0.4 * 2^-24 of the accumulator for each MMA, so the small products have an
+// accumulator of their own (or come first) and only every third MMA meets the large sum.
+// Operands come through registers (load, split, swizzled store)
+// because the split has to happen on the way, so any size and alignment is a predicate there.
+//
+// Shared memory bounds it: the split doubles what is written, and each MMA reads its operands again:
+// 1.5 MB per chunk of 128 x 128 heads at 128 B a clock.
+#include "gemm_tf32_device.cuh"
+#include "linear_attention.h"
+
+namespace {
+
+constexpr int kC = 128;            // tokens of a chunk = rows of an MMA
+constexpr int kProducers = 8;      // warps
+constexpr int kMaxStages = 4;
+constexpr int kSmemCap = 232448;
+
+struct ChunkArgs {
+  LinearArgs a;
+  float* states;                   // [units][chunks][dv][dk]
+  int chunks, dv_tiles, items;
+  int dvp, dkp;                    // columns of a dim_v tile and dim_k, in whole blocks of 32
+  int stage_bytes, stages;
+};
+
+// a chunk's row, head, first token and tokens
+struct Item {
+  int unit, b, h, c, dv0;
+  int n;                           // tokens of the chunk, 0 behind the row's end
+};
+__device__ __forceinline__ Item item_of(const ChunkArgs& g, int i) {
+  Item t;
+  const int dvt = i % g.dv_tiles;
+  const int uc = i / g.dv_tiles;
+  t.c = uc % g.chunks;
+  t.unit = uc / g.chunks;
+  t.b = t.unit / g.a.heads;
+  t.h = t.unit - t.b * g.a.heads;
+  t.dv0 = dvt * 128;
+  const int left = linear_length(g.a, t.b) - t.c * kC;
+  t.n = left < 0 ? 0 : (left > kC ? kC : left);
+  return t;
+}
+
+// Four values of a row of `dim` from column d on, zeros outside.
+template <bool WIDE>
+__device__ __forceinline__ float4 load_cols(const float* row, int d, int dim) {
+  if (WIDE) return d < dim ? __ldg(reinterpret_cast<const float4*>(row + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 r;
+  r.x = d < dim ? __ldg(row + d) : 0.f;
+  r.y = d + 1 < dim ? __ldg(row + d + 1) : 0.f;
+  r.z = d + 2 < dim ? __ldg(row + d + 2) : 0.f;
+  r.w = d + 3 < dim ? __ldg(row + d + 3) : 0.f;
+  return r;
+}
+
+// x rounded to TF32's 11 bits, to nearest
+__device__ __forceinline__ float tf32_hi(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+}
+__device__ __forceinline__ void store_split(uint32_t hi_addr, uint32_t lo_addr, const float4& x) {
+  const float a = tf32_hi(x.x), b = tf32_hi(x.y), c = tf32_hi(x.z), d = tf32_hi(x.w);
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(hi_addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(lo_addr), "f"(x.x - a), "f"(x.y - b),
+               "f"(x.z - c), "f"(x.w - d) : "memory");
+}
+// Byte offsets of 16-byte piece c4 (of 8) of a row in the two swizzled layouts: K-major rows of
+// 32 values (16-byte pieces exchanged within eight rows), and MN-major blocks of 32 K rows x 32
+// columns (32-byte pieces exchanged within four rows).
+__device__ __forceinline__ uint32_t k_major(int row, int c4) {
+  return (uint32_t)row * 128u + (uint32_t)((c4 ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint32_t mn_major(int row, int c4) {
+  return (uint32_t)row * 128u + (uint32_t)((((c4 >> 1) ^ (row & 3)) << 5) | ((c4 & 1) << 4));
+}
+
+// mbar_wait for a whole warp: true only if no lane gave up, so that its lanes stay together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+__device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const float* f) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]),
+      "f"(f[8]), "f"(f[9]), "f"(f[10]), "f"(f[11]), "f"(f[12]), "f"(f[13]), "f"(f[14]), "f"(f[15]),
+      "f"(f[16]), "f"(f[17]), "f"(f[18]), "f"(f[19]), "f"(f[20]), "f"(f[21]), "f"(f[22]), "f"(f[23]),
+      "f"(f[24]), "f"(f[25]), "f"(f[26]), "f"(f[27]), "f"(f[28]), "f"(f[29]), "f"(f[30]), "f"(f[31])
+      : "memory");
+}
+
+// 32 x 32 values, one row a lane, through a swizzled 4 KB tile of the warp so that global
+// memory is written in rows of 128 bytes.  Row r goes to row_ptr(r) (null: not stored) at
+// columns col .. col + 31 of `dim`.
+template <bool WIDE, typename RowPtr>
+__device__ __forceinline__ void store_rows32(uint32_t tile, int lane, const float* v, int col, int dim, RowPtr row_ptr) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(tile + k_major(lane, j)), "f"(v[4 * j]),
+                 "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3]) : "memory");
+  __syncwarp();
+  const int c4 = lane & 7, d = col + c4 * 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    float4 x;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                 : "r"(tile + k_major(r, c4)) : "memory");
+    float* p = row_ptr(r);
+    if (p == nullptr) continue;
+    if (WIDE) {
+      if (d < dim) *reinterpret_cast<float4*>(p + d) = x;
+    } else {
+      if (d < dim) p[d] = x.x;
+      if (d + 1 < dim) p[d + 1] = x.y;
+      if (d + 2 < dim) p[d + 2] = x.z;
+      if (d + 3 < dim) p[d + 3] = x.w;
+    }
+  }
+}
+
+constexpr uint32_t kIdesc = (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(128 >> 4) << 24);  // f32 += tf32 x tf32, M = 128
+constexpr uint32_t kAMN = 1u << 15, kBMN = 1u << 16;
+__device__ __forceinline__ uint32_t n_field(int n) { return (uint32_t)(n >> 3) << 17; }
+
+// ---- A^T of every chunk: M = dim_v tile, N = dim_k, K = tokens ------------------------------
+// warps 0-7 producers, 8-11 epilogue, 12 MMA
+constexpr int kStateThreads = (kProducers + 4 + 1) * 32;
+
+template <bool WIDE>
+__global__ void __launch_bounds__(kStateThreads, 1)
+linear_chunk_states_kernel(const ChunkArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t tiles = base + (uint32_t)(g.stages * g.stage_bytes);
+  const uint32_t bars = tiles + 4 * 4096u;
+  auto full = [&](int s) { return bars + 8u * (uint32_t)s; };
+  auto empty = [&](int s) { return bars + 8u * (uint32_t)(kMaxStages + s); };
+  auto acc_full = [&](int s) { return bars + 8u * (uint32_t)(2 * kMaxStages + s); };
+  auto acc_empty = [&](int s) { return bars + 8u * (uint32_t)(2 * kMaxStages + 2 + s); };
+  const uint32_t tmem_slot = bars + 8u * (2 * kMaxStages + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.stages; ++s) {
+      mbar_init(full(s), kProducers);
+      mbar_init(empty(s), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(acc_full(s), 1);
+      mbar_init(acc_empty(s), 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+  // a stage: 32 tokens of V (four column blocks, hi then lo) and of decayed K
+  const int nbv = g.dvp / 32, nbk = g.dkp / 32;
+  const uint32_t k_off = 2 * 16384u, k_bytes = (uint32_t)nbk * 4096u;
+  // accumulators of hi hi and of the small products: twice where 512 columns hold that
+  const uint32_t bufs = g.dkp <= 128 ? 2u : 1u;
+  if (warp < kProducers) {
+    const int tid = threadIdx.x;
+    uint32_t st = 0;
+    bool alive = true;
+    for (int i = blockIdx.x; alive && i < g.items; i += gridDim.x) {
+      const Item t = item_of(g, i);
+      if (t.n == 0) continue;
+      const float ld = __ldg(g.a.log_decay + t.h);
+      const uint64_t row0 = (uint64_t)t.unit * g.a.seq + (uint64_t)t.c * kC;
+      const int steps = (t.n + 31) / 32;
+      for (int ks = 0; ks < steps; ++ks, ++st) {
+        const int s = st % g.stages;
+        const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+        // 32 rows x (nbv + nbk) blocks of eight 16-byte pieces; thread: row tid / 8, one piece
+        // of every block
+        const int r = tid >> 3, c4 = tid & 7;
+        const int j = ks * 32 + r;
+        const bool in = j < t.n;
+        float4 xv[4], xk[8];
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk)
+          if (blk < nbv)
+            xv[blk] = in ? load_cols<WIDE>(g.a.v + (row0 + j) * g.a.dv, t.dv0 + blk * 32 + c4 * 4, g.a.dv)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int blk = 0; blk < 8; ++blk)
+          if (blk < nbk)
+            xk[blk] = in ? load_cols<WIDE>(g.a.k + (row0 + j) * g.a.dk, blk * 32 + c4 * 4, g.a.dk)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float w = in ? decay_power(ld, t.n - 1 - j) : 0.f;
+        if (!warp_wait(empty(s), ((st / g.stages) & 1) ^ 1)) {
+          if (lane == 0) atomicExch(g.a.flag, 1);
+          alive = false;
+          break;
+        }
+        const uint32_t at = mn_major(r, c4);
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk)
+          if (blk < nbv) store_split(sb + blk * 4096u + at, sb + 16384u + blk * 4096u + at, xv[blk]);
+#pragma unroll
+        for (int blk = 0; blk < 8; ++blk)
+          if (blk < nbk) {
+            xk[blk].x *= w;
+            xk[blk].y *= w;
+            xk[blk].z *= w;
+            xk[blk].w *= w;
+            store_split(sb + k_off + blk * 4096u + at, sb + k_off + k_bytes + blk * 4096u + at, xk[blk]);
+          }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(s));
+      }
+    }
+  } else if (warp == 12) {
+    if (lane == 0) {
+      const uint32_t idesc = kIdesc | kAMN | kBMN | n_field(g.dkp);
+      uint32_t st = 0, done = 0;
+      bool alive = true;
+      for (int i = blockIdx.x; alive && i < g.items; i += gridDim.x) {
+        const Item t = item_of(g, i);
+        if (t.n == 0) continue;
+        const uint32_t buf = done % bufs;
+        if (!mbar_wait(acc_empty(buf), ((done / bufs) & 1) ^ 1)) {
+          atomicExch(g.a.flag, 2);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * 256u, acc_lo = acc + (bufs == 2 ? 128u : 256u);
+        const int steps = (t.n + 31) / 32;
+        for (int ks = 0; ks < steps; ++ks, ++st) {
+          const int s = st % g.stages;
+          if (!mbar_wait(full(s), (st / g.stages) & 1)) {
+            atomicExch(g.a.flag, 3);
+            alive = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t o = (uint32_t)kk * 1024u;
+            const uint64_t vh = desc_mn_major(sb + o), vl = desc_mn_major(sb + 16384u + o);
+            const uint64_t kh = desc_mn_major(sb + k_off + o), kl = desc_mn_major(sb + k_off + k_bytes + o);
+            tc_mma_tf32(acc_lo, vl, kh, idesc, (ks | kk) != 0);
+            tc_mma_tf32(acc_lo, vh, kl, idesc, 1);
+            tc_mma_tf32(acc, vh, kh, idesc, (ks | kk) != 0);
+          }
+          tc_commit(empty(s));
+        }
+        if (!alive) break;
+        tc_commit(acc_full(buf));
+        ++done;
+      }
+    }
+  } else {
+    const int q = warp & 3;
+    const uint32_t tile = tiles + (uint32_t)q * 4096u;
+    uint32_t done = 0;
+    for (int i = blockIdx.x; i < g.items; i += gridDim.x) {
+      const Item t = item_of(g, i);
+      if (t.n == 0) continue;
+      const uint32_t buf = done % bufs;
+      if (!warp_wait(acc_full(buf), (done / bufs) & 1)) {
+        if (lane == 0) atomicExch(g.a.flag, 4);
+        break;
+      }
+      tc_fence_after();
+      float* out = g.states + ((uint64_t)t.unit * g.chunks + t.c) * g.a.dv * g.a.dk;
+      if (q * 32 < g.dvp)
+        for (int cb = 0; cb < nbk; ++cb) {
+          float v[32], lo[32];
+          const uint32_t acc = tmem + buf * 256u + ((uint32_t)(q * 32) << 16) + (uint32_t)(cb * 32);
+          tc_ld32(acc, v);
+          tc_ld32(acc + (bufs == 2 ? 128u : 256u), lo);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += lo[j];
+          store_rows32<WIDE>(tile, lane, v, cb * 32, g.a.dk, [&](int r) -> float* {
+            const int row = t.dv0 + q * 32 + r;
+            return row < g.a.dv ? out + (uint64_t)row * g.a.dk : nullptr;
+          });
+        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(buf));
+      ++done;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ---- states between the chunks -----------------------------------------------------------
+// A thread carries one element of the (transposed) state through all chunks of its row; eight
+// chunks are in flight, since each is a dependent step of one multiply-add.
+__global__ void __launch_bounds__(256)
+linear_chunk_scan_kernel(const ChunkArgs g, int blocks_per_unit) {
+  const int unit = blockIdx.x / blocks_per_unit;
+  const int e = (blockIdx.x - unit * blocks_per_unit) * 256 + (int)threadIdx.x;
+  const int size = g.a.dv * g.a.dk;
+  if (e >= size) return;
+  const int b = unit / g.a.heads, h = unit - b * g.a.heads;
+  const int n = linear_length(g.a, b);
+  const int nc = (n + kC - 1) / kC;
+  const int row = e / g.a.dk, col = e - row * g.a.dk;      // dim_v, dim_k
+  const uint64_t at = (uint64_t)unit * size + (uint64_t)col * g.a.dv + row;
+  const float ld = __ldg(g.a.log_decay + h);
+  const float whole = decay_power(ld, kC), last = decay_power(ld, n - (nc - 1) * kC);
+  float s = g.a.state ? __ldg(g.a.state + at) : 0.f;
+  float* p = g.states + (uint64_t)unit * g.chunks * size + e;
+  constexpr int U = 8;
+  int c = 0;
+  for (; c + U < nc; c += U) {
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = p[(uint64_t)(c + u) * size];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      p[(uint64_t)(c + u) * size] = s;
+      s = fmaf(s, whole, x[u]);
+    }
+  }
+  for (; c < nc; ++c) {
+    const float x = p[(uint64_t)c * size];
+    p[(uint64_t)c * size] = s;
+    s = fmaf(s, c + 1 < nc ? whole : last, x);
+  }
+  g.a.out_state[at] = s;
+}
+
+// ---- outputs -------------------------------------------------------------------------------
+// warps 0-7 producers, 8-15 two per quarter of the tensor-memory lanes (scores to decayed
+// probabilities, then the result), 16 MMA.
+// Tensor memory, in columns (hi hi sums left, sums of the small products right):
+//   [0, 128) scores, later the probabilities' hi parts     [256, 384) scores, later their lo parts
+//   [128, 256) Q S, later decayed                          [384, 512) Q S, later P V
+constexpr int kOutThreads = (kProducers + 8 + 1) * 32;
+
+template <bool WIDE>
+__global__ void __launch_bounds__(kOutThreads, 1)
+linear_chunk_outputs_kernel(const ChunkArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t tiles = base + (uint32_t)(g.stages * g.stage_bytes);
+  const uint32_t bars = tiles + 8 * 4096u;
+  auto full = [&](int s) { return bars + 8u * (uint32_t)s; };
+  auto empty = [&](int s) { return bars + 8u * (uint32_t)(kMaxStages + s); };
+  const uint32_t s_full = bars + 8u * (2 * kMaxStages), p_full = s_full + 8u, o_full = s_full + 16u,
+                 o_empty = s_full + 24u;
+  const uint32_t tmem_slot = s_full + 32u;
+  const uint32_t power_s = tmem_slot + 8u;                 // float[kC + 1] per transforming warp set
+  float* power = reinterpret_cast<float*>(smem_raw + (power_s - smem_u32(smem_raw)));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.stages; ++s) {
+      mbar_init(full(s), kProducers);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 8);
+    mbar_init(o_full, 1);
+    mbar_init(o_empty, 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 16) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  const uint32_t t_s = tmem, t_inter = tmem + 128u, t_lo = tmem + 256u, t_out = tmem + 384u;
+
+  // a stage holds either 32 columns of Q (128 rows, hi then lo) and of [K; S^T] (128 + dvp rows,
+  // hi then lo), or 64 tokens of V (two groups of 32, each dvp / 32 column blocks; hi then lo)
+  const int nk = g.dkp / 32, nbv = g.dvp / 32;
+  const uint32_t b_off = 32768u, b_bytes = (uint32_t)(128 + g.dvp) * 128u;
+  const uint32_t v_bytes = 64u * (uint32_t)g.dvp * 4u;
+  if (warp < kProducers) {
+    const int tid = threadIdx.x;
+    const int r0 = tid >> 3, c4 = tid & 7;                 // 32 rows at a time, eight pieces each
+    uint32_t st = 0;
+    bool alive = true;
+    for (int i = blockIdx.x; alive && i < g.items; i += gridDim.x) {
+      const Item t = item_of(g, i);
+      if (t.n == 0) continue;
+      const uint64_t row0 = (uint64_t)t.unit * g.a.seq + (uint64_t)t.c * kC;
+      const float* sp = g.states + ((uint64_t)t.unit * g.chunks + t.c) * g.a.dv * g.a.dk;
+      for (int ks = 0; ks < nk; ++ks, ++st) {
+        const int s = st % g.stages;
+        const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+        const int d = ks * 32 + c4 * 4;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 xq[4], xk[4], xs[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = x * 32 + r0;
+          xq[x] = r < t.n ? load_cols<WIDE>(g.a.q + (row0 + r) * g.a.dk, d, g.a.dk) : zero;
+          xk[x] = r < t.n ? load_cols<WIDE>(g.a.k + (row0 + r) * g.a.dk, d, g.a.dk) : zero;
+          const int dv = t.dv0 + r;
+          xs[x] = x < nbv && dv < g.a.dv ? load_cols<WIDE>(sp + (uint64_t)dv * g.a.dk, d, g.a.dk) : zero;
+        }
+        if (!warp_wait(empty(s), ((st / g.stages) & 1) ^ 1)) {
+          if (lane == 0) atomicExch(g.a.flag, 1);
+          alive = false;
+          break;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t at = k_major(x * 32 + r0, c4);
+          store_split(sb + at, sb + 16384u + at, xq[x]);
+          store_split(sb + b_off + at, sb + b_off + b_bytes + at, xk[x]);
+          if (x < nbv) store_split(sb + b_off + 16384u + at, sb + b_off + b_bytes + 16384u + at, xs[x]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(s));
+      }
+      if (!alive) break;
+      const int vsteps = (t.n + 63) / 64;
+      for (int vs = 0; vs < vsteps; ++vs, ++st) {
+        const int s = st % g.stages;
+        const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+        float4 x[2][4];
+#pragma unroll
+        for (int tg = 0; tg < 2; ++tg) {
+          const int j = vs * 64 + tg * 32 + r0;
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb)
+            if (cb < nbv)
+              x[tg][cb] = j < t.n ? load_cols<WIDE>(g.a.v + (row0 + j) * g.a.dv, t.dv0 + cb * 32 + c4 * 4, g.a.dv)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (!warp_wait(empty(s), ((st / g.stages) & 1) ^ 1)) {
+          if (lane == 0) atomicExch(g.a.flag, 1);
+          alive = false;
+          break;
+        }
+        const uint32_t at = mn_major(r0, c4);
+#pragma unroll
+        for (int tg = 0; tg < 2; ++tg)
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb)
+            if (cb < nbv) {
+              const uint32_t o = sb + (uint32_t)(tg * nbv + cb) * 4096u + at;
+              store_split(o, o + v_bytes, x[tg][cb]);
+            }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(s));
+      }
+    }
+  } else if (warp == 16) {
+    if (lane == 0) {
+      const uint32_t idesc_s = kIdesc | n_field(128 + g.dvp);
+      const uint32_t idesc_o = kIdesc | kBMN | n_field(g.dvp);
+      uint32_t st = 0, done = 0;
+      bool alive = true;
+      for (int i = blockIdx.x; alive && i < g.items; i += gridDim.x) {
+        const Item t = item_of(g, i);
+        if (t.n == 0) continue;
+        // (the probabilities' place is free: the previous item's products, which read it, come first
+        // in this thread's order; the sums must have been read)
+        if (!mbar_wait(o_empty, (done & 1) ^ 1)) {
+          atomicExch(g.a.flag, 7);
+          break;
+        }
+        tc_fence_after();
+        for (int ks = 0; ks < nk; ++ks, ++st) {
+          const int s = st % g.stages;
+          if (!mbar_wait(full(s), (st / g.stages) & 1)) {
+            atomicExch(g.a.flag, 2);
+            alive = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t o = (uint32_t)kk * 32u;
+            const uint64_t qh = desc_k_major(sb + o), ql = desc_k_major(sb + 16384u + o);
+            const uint64_t bh = desc_k_major(sb + b_off + o), bl = desc_k_major(sb + b_off + b_bytes + o);
+            tc_mma_tf32(t_lo, ql, bh, idesc_s, (ks | kk) != 0);
+            tc_mma_tf32(t_lo, qh, bl, idesc_s, 1);
+            tc_mma_tf32(t_s, qh, bh, idesc_s, (ks | kk) != 0);
+          }
+          tc_commit(empty(s));
+        }
+        if (!alive) break;
+        tc_commit(s_full);
+        if (!mbar_wait(p_full, done & 1)) {
+          atomicExch(g.a.flag, 3);
+          break;
+        }
+        tc_fence_after();
+        // all small products first, while the sum is small: both halves of V are there by then
+        // (at least two stages)
+        const int vsteps = (t.n + 63) / 64;
+        for (int pass = 0; alive && pass < 2; ++pass)
+          for (int vs = 0; vs < vsteps; ++vs) {
+            const int s = (st + vs) % g.stages;
+            if (pass == 0) {
+              if (!mbar_wait(full(s), ((st + vs) / g.stages) & 1)) {
+                atomicExch(g.a.flag, 4);
+                alive = false;
+                break;
+              }
+              tc_fence_after();
+            }
+            const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t o = sb + (uint32_t)((kk >> 2) * nbv) * 4096u + (uint32_t)(kk & 3) * 1024u;
+              const uint32_t col = (uint32_t)(vs * 64 + kk * 8);
+              const uint64_t vh = desc_mn_major(o), vl = desc_mn_major(o + v_bytes);
+              if (pass == 0) {
+                mma_tmem_a(t_out, t_lo + col, vh, idesc_o, (vs | kk) != 0);
+                mma_tmem_a(t_out, t_s + col, vl, idesc_o, 1);
+              } else {
+                mma_tmem_a(t_out, t_s + col, vh, idesc_o, 1);
+              }
+            }
+            if (pass == 1) tc_commit(empty(s));
+          }
+        st += vsteps;
+        if (!alive) break;
+        tc_commit(o_full);
+        ++done;
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - kProducers) >> 2;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const uint32_t tile = tiles + (uint32_t)(warp - kProducers) * 4096u;
+    const int tok = q * 32 + lane;                         // this thread's row
+    uint32_t done = 0;
+    int powers_of = -1;
+    bool alive = true;
+    for (int i = blockIdx.x; i < g.items; i += gridDim.x) {
+      const Item t = item_of(g, i);
+      const uint64_t first = (uint64_t)t.b * g.a.seq + (uint64_t)t.c * kC;
+      auto out_row = [&](int r) -> float* {
+        const int token = q * 32 + r;
+        return t.c * kC + token < g.a.seq ? g.a.out + ((first + token) * g.a.heads + t.h) * g.a.dv + t.dv0 : nullptr;
+      };
+      const int cols = g.a.dv - t.dv0 < 128 ? g.a.dv - t.dv0 : 128;
+      if (t.n == 0) {
+        float z[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) z[x] = 0.f;
+        for (int cb = half; cb < nbv; cb += 2) store_rows32<WIDE>(tile, lane, z, cb * 32, cols, out_row);
+        continue;
+      }
+      if (t.h != powers_of) {                              // (the same for all eight warps)
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int e = (int)threadIdx.x - kProducers * 32;
+        if (e <= kC) power[e] = decay_power(__ldg(g.a.log_decay + t.h), e);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        powers_of = t.h;
+      }
+      if (!alive) continue;                                // (keeps the barriers above in step)
+      if (!warp_wait(s_full, done & 1)) {
+        if (lane == 0) atomicExch(g.a.flag, 5);
+        alive = false;
+        continue;
+      }
+      tc_fence_after();
+#pragma unroll 1
+      for (int cc = 0; cc < 2; ++cc) {
+        const int j0 = half * 64 + cc * 32;
+        float x[32], lo[32];
+        if (j0 <= q * 32 + 31) {
+          tc_ld32(t_s + lanes + (uint32_t)j0, x);
+          tc_ld32(t_lo + lanes + (uint32_t)j0, lo);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int ago = tok - (j0 + j);
+            const float p = ago >= 0 ? (x[j] + lo[j]) * power[ago < 0 ? 0 : ago] : 0.f;
+            x[j] = tf32_hi(p);
+            lo[j] = p - x[j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = lo[j] = 0.f;
+        }
+        tmem_store32(t_s + lanes + (uint32_t)j0, x);
+        tmem_store32(t_lo + lanes + (uint32_t)j0, lo);
+      }
+      const float w = power[tok + 1];
+#pragma unroll 1
+      for (int cb = half; cb < nbv; cb += 2) {
+        float x[32], lo[32];
+        tc_ld32(t_inter + lanes + (uint32_t)(cb * 32), x);
+        tc_ld32(t_out + lanes + (uint32_t)(cb * 32), lo);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = (x[j] + lo[j]) * w;
+        tmem_store32(t_inter + lanes + (uint32_t)(cb * 32), x);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+      if (!warp_wait(o_full, done & 1)) {
+        if (lane == 0) atomicExch(g.a.flag, 6);
+        alive = false;
+        continue;
+      }
+      tc_fence_after();
+      const bool real = tok < t.n;
+      float x[2][32];                                      // (both blocks first: the sums' place is needed)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int cb = half + 2 * y;
+        if (cb < nbv) {
+          float lo[32];
+          tc_ld32(t_out + lanes + (uint32_t)(cb * 32), x[y]);
+          tc_ld32(t_inter + lanes + (uint32_t)(cb * 32), lo);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float o = x[y][j] + lo[j];
+            x[y][j] = real ? (g.a.has_scale ? __fmul_rn(o, g.a.scale) : o) : 0.f;
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty);
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        if (half + 2 * y < nbv) store_rows32<WIDE>(tile, lane, x[y], (half + 2 * y) * 32, cols, out_row);
+      ++done;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 16) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+template <bool WIDE>
+int launch_chunks(tfjs_cuda_ctx* ctx, ChunkArgs& g) {
+  // chunk_states: 32 tokens of V (four blocks whatever dim_v, the MMA reads 128 columns) and K
+  ChunkArgs s = g;
+  s.stage_bytes = 2 * 16384 + 2 * (g.dkp / 32) * 4096;
+  const int s_fixed = 1024 + 4 * 4096 + 256;
+  s.stages = (kSmemCap - s_fixed) / s.stage_bytes;
+  if (s.stages > kMaxStages) s.stages = kMaxStages;
+  const int s_smem = s_fixed + s.stages * s.stage_bytes;
+  CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
+  const unsigned grid = (unsigned)(g.items < ctx->sm_count ? g.items : ctx->sm_count);
+  linear_chunk_states_kernel<WIDE><<<grid, kStateThreads, s_smem, ctx->stream>>>(s);
+  LAUNCH_CHECK(ctx, "linear_chunk_states_kernel");
+  const unsigned units = (unsigned)(g.a.batch * g.a.heads);
+  const int per = (g.a.dv * g.a.dk + 255) / 256;
+  linear_chunk_scan_kernel<<<units * per, 256, 0, ctx->stream>>>(g, per);
+  LAUNCH_CHECK(ctx, "linear_chunk_scan_kernel");
+  const int qk = 32768 + 2 * (128 + g.dvp) * 128, v = 2 * 64 * g.dvp * 4;
+  g.stage_bytes = qk > v ? qk : v;
+  const int o_fixed = 1024 + 8 * 4096 + 256 + (kC + 1) * 4;
+  g.stages = (kSmemCap - o_fixed) / g.stage_bytes;
+  if (g.stages > kMaxStages) g.stages = kMaxStages;
+  const int o_smem = o_fixed + g.stages * g.stage_bytes;
+  CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_outputs_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, o_smem));
+  linear_chunk_outputs_kernel<WIDE><<<grid, kOutThreads, o_smem, ctx->stream>>>(g);
+  LAUNCH_CHECK(ctx, "linear_chunk_outputs_kernel");
+  return TFJS_CUDA_OK;
+}
+
+}  // namespace
+
+int launch_linear_chunked(tfjs_cuda_ctx* ctx, const LinearArgs& a) {
+  ChunkArgs g;
+  g.a = a;
+  g.chunks = (a.seq + kC - 1) / kC;
+  g.dv_tiles = (a.dv + 127) / 128;
+  const uint64_t units = (uint64_t)a.batch * a.heads;
+  if (units * g.chunks * g.dv_tiles > 0x7fffffffull || units * ((uint64_t)a.dv * a.dk / 256 + 1) > 0x7fffffffull)
+    return ctx_fail(ctx, TFJS_CUDA_UNSUPPORTED, "linear attention: too many tokens for one call");
+  g.items = (int)(units * g.chunks * g.dv_tiles);
+  const int tile = a.dv < 128 ? a.dv : 128;
+  g.dvp = (tile + 31) / 32 * 32;
+  g.dkp = (a.dk + 31) / 32 * 32;
+  TempBuffer ws(ctx);
+  void* mem;
+  int rc = ws.get(units * g.chunks * (uint64_t)a.dv * a.dk * 4, &mem);
+  if (rc) return rc;
+  g.states = (float*)mem;
+  const bool wide = a.dk % 4 == 0 && a.dv % 4 == 0 &&
+                    (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0;
+  return wide ? launch_chunks<true>(ctx, g) : launch_chunks<false>(ctx, g);
+}
