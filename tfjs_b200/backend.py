@@ -39,6 +39,7 @@ from . import _cabi
 from ._cabi import CudaError
 
 NP_DTYPES = {"float32": np.float32, "int32": np.int32, "bool": np.uint8}
+_FOREIGN_TYPES = {"<f4": ("float32", 4), "<i4": ("int32", 4), "|b1": ("bool", 1)}
 HOST_RESIDENT_BYTES = 4096  # keep a host copy of tensors up to this size
 
 
@@ -584,32 +585,32 @@ class CudaBackend(object):
         return TensorInfo(dataId, shape, dtype)
 
     # -------------------------------------------------- other libraries' memory --
-    def createTensorFromGPUData(self, values, shape=None, dtype=None, stream=None):
+    def createTensorFromGPUData(self, values, shape=None, dtype=None, stream=None,
+                                interface=None):
         """A TensorInfo over device memory that another library holds, without a copy (the
         KernelBackend method behind tf.tensor({buffer, zeroCopy: true})).  `values` has
-        __cuda_array_interface__: contiguous float32, int32 or bool memory of this GPU.
-        `stream` (a cudaStream_t as a number, 0 = the default stream): this backend's work
-        waits for what is queued there now, and what is queued there after the tensor is
-        disposed waits for this backend's work.  Without it the caller orders the two."""
-        info = values.__cuda_array_interface__
-        typestr, strides = info["typestr"], info.get("strides")
-        found = {"<f4": "float32", "<i4": "int32", "|b1": "bool"}.get(typestr)
-        have = [int(v) for v in info["shape"]]
+        __cuda_array_interface__ (`interface`, if the caller has read it already): contiguous
+        float32, int32 or bool memory of this GPU.  `stream` (a cudaStream_t as a number, 0 = the
+        default stream): this backend's work waits for what is queued there now, and what is
+        queued there after the tensor is disposed waits for this backend's work.  Without it
+        the caller orders the two."""
+        info = interface if interface is not None else values.__cuda_array_interface__
+        found, step = _FOREIGN_TYPES.get(info["typestr"], (None, 0))
         if found is None or (dtype is not None and dtype != found):
             raise ValueError("createTensorFromGPUData: dtype %s of the memory is not %s" %
-                             (typestr, dtype or "one of float32, int32, bool"))
-        nbytes = size_from_shape(have) * np.dtype(NP_DTYPES[found]).itemsize
-        if strides is not None and nbytes:
-            step = np.dtype(NP_DTYPES[found]).itemsize
-            for n, s in zip(reversed(have), reversed(list(strides))):
-                if n != 1 and s != step:
+                             (info["typestr"], dtype or "one of float32, int32, bool"))
+        have = info["shape"]
+        n = size_from_shape(have)
+        nbytes = n * step
+        strides = info.get("strides")
+        if strides is not None and n:
+            for d, s in zip(reversed(have), reversed(strides)):
+                if d != 1 and s != step:
                     raise ValueError("createTensorFromGPUData: the memory is not contiguous "
-                                     "(shape %s, strides %s)" % (have, list(strides)))
-                step *= n
-        shape = have if shape is None else [int(v) for v in shape]
-        if size_from_shape(shape) != size_from_shape(have):
-            raise ValueError("createTensorFromGPUData: %d values for shape %s" %
-                             (size_from_shape(have), shape))
+                                     "(shape %s, strides %s)" % (list(have), list(strides)))
+                step *= d
+        if shape is not None and size_from_shape(shape) != n:
+            raise ValueError("createTensorFromGPUData: %d values for shape %s" % (n, list(shape)))
         if stream is not None:
             self.wait_stream(stream)
         dev = c_int32()
@@ -618,7 +619,7 @@ class CudaBackend(object):
         rec = _Record(dev.value, nbytes, found, 1, None)
         rec.foreign, rec.stream = values, stream
         self.data[dataId] = rec
-        return TensorInfo(dataId, shape, found)
+        return TensorInfo(dataId, have if shape is None else shape, found)
 
     def readToGPU(self, tensor, stream=None):
         """GPUData over `tensor`'s device memory (the KernelBackend method behind
@@ -635,11 +636,11 @@ class CudaBackend(object):
 
     def wait_stream(self, stream):
         """This backend's work from now on runs after what is queued on `stream`."""
-        self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, c_void_p(int(stream))))
+        self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, int(stream)))
 
     def signal_stream(self, stream):
         """What is queued on `stream` from now on runs after this backend's work so far."""
-        self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, c_void_p(int(stream))))
+        self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, int(stream)))
 
     # ---------------------------------------------------- deferred launches --
     def _adjust(self, rec, dref, dheld):

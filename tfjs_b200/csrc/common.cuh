@@ -103,6 +103,10 @@ struct tfjs_cuda_ctx {
   long long* h_bad_index = nullptr;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;
   cudaEvent_t ev_order = nullptr;  // orders this context against a caller's stream
+  // Counts what may have put work on the stream (every use of a tensor, every launch), so that a
+  // caller's stream that was signalled and has missed nothing since is not signalled again.
+  uint64_t work = 1, signalled_work = 0;
+  unsigned long long signalled_stream = 0;  // cudaStreamGetId: never given out twice
   std::vector<cudaEvent_t> prof_events;  // numbered events for per-kernel timing
   std::vector<cudaEvent_t> read_events;  // tickets of tfjs_cuda_read_begin (index + 1)
   std::vector<cudaEvent_t> read_order;   // per ticket: orders the read stream behind the compute stream
@@ -182,6 +186,7 @@ void loaders_drop(tfjs_cuda_ctx* ctx);
 #define LAUNCH_CHECK(ctx, name)                               \
   do {                                                        \
     (ctx)->launches++;                                        \
+    (ctx)->work++;                                            \
     if ((ctx)->log_launches) (ctx)->launch_log.push_back(name); \
     int _rc = ctx_check((ctx), cudaGetLastError(), name);     \
     if (_rc != TFJS_CUDA_OK) return _rc;                      \

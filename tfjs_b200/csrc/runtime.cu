@@ -44,6 +44,7 @@ Buffer* ctx_buf(tfjs_cuda_ctx* ctx, int32_t id) {
 int ctx_get(tfjs_cuda_ctx* ctx, int32_t id, uint64_t need, const char* name,
             Buffer** out) {
   Buffer* b = ctx_buf(ctx, id);
+  ctx->work++;
   if (!b) return ctx_fail(ctx, TFJS_CUDA_UNKNOWN_ID, "%s: unknown tensor id %d",
                           name, id);
   if (b->bytes < need)
@@ -735,7 +736,15 @@ int tfjs_cuda_wait_stream(tfjs_cuda_ctx* ctx, void* stream) {
 int tfjs_cuda_signal_stream(tfjs_cuda_ctx* ctx, void* stream) {
   if (!ctx) return TFJS_CUDA_INVALID_ARG;
   NOT_WHILE_CAPTURING(ctx, "signalling a caller's stream");
-  return order_streams(ctx, ctx->stream, (cudaStream_t)stream, (cudaStream_t)stream);
+  cudaSetDevice(ctx->device);
+  unsigned long long id = 0;
+  const bool known = cudaStreamGetId((cudaStream_t)stream, &id) == cudaSuccess;
+  if (!known) cudaGetLastError();
+  if (known && id == ctx->signalled_stream && ctx->work == ctx->signalled_work) return TFJS_CUDA_OK;
+  const int rc = order_streams(ctx, ctx->stream, (cudaStream_t)stream, (cudaStream_t)stream);
+  ctx->signalled_stream = id;
+  ctx->signalled_work = rc == TFJS_CUDA_OK && known ? ctx->work : 0;
+  return rc;
 }
 
 int tfjs_cuda_memory(tfjs_cuda_ctx* ctx, uint64_t* bytes_in_use,
@@ -937,6 +946,7 @@ int tfjs_cuda_graph_launch(tfjs_cuda_ctx* ctx, int32_t graph) {
                     "step again", graph);
   cudaSetDevice(ctx->device);
   CUDA_TRY(ctx, cudaGraphLaunch(g->exec, ctx->stream));
+  ctx->work++;
   ctx->launches += g->launches;
   return TFJS_CUDA_OK;
 }

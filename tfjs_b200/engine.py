@@ -17,6 +17,7 @@ class Tensor(object):
 
     def __init__(self, engine, info):
         self._engine = engine
+        self._info = info
         self.dataId = info.dataId
         self.shape = list(info.shape)
         self.dtype = info.dtype
@@ -34,7 +35,9 @@ class Tensor(object):
         return n
 
     def info(self):
-        return TensorInfo(self.dataId, self.shape, self.dtype)
+        if self._info.shape != self.shape:
+            return TensorInfo(self.dataId, self.shape, self.dtype)
+        return self._info
 
     def dataSync(self):
         """engine.ts:1218-1222 -> backend.readSync."""
@@ -56,11 +59,11 @@ class Tensor(object):
         result keeps the memory alive on its own; this handle may be disposed.  `stream`:
         what is queued on that stream from now on runs after the kernels launched so far."""
         self._check()
-        info = self.info()
-        self._engine.backend.incRef(self.dataId)
-        ref = self._engine.make_tensor_from_info(info)
+        backend = self._engine.backend
+        backend.incRef(self.dataId)
+        ref = self._engine.make_tensor_from_info(self.info())
         try:
-            return self._engine.backend.readToGPU(ref, stream)
+            return backend.readToGPU(ref, stream)
         except Exception:
             ref.dispose()
             raise
@@ -143,9 +146,10 @@ class Engine(object):
         """engine.ts:803-827 -> backend.write; device memory of another library (anything
         with __cuda_array_interface__) becomes a tensor without a copy."""
         self.ready()
-        if hasattr(values, "__cuda_array_interface__"):
+        interface = getattr(values, "__cuda_array_interface__", None)
+        if interface is not None:
             return self.make_tensor_from_info(
-                self.backend.createTensorFromGPUData(values, shape, dtype, stream))
+                self.backend.createTensorFromGPUData(values, shape, dtype, stream, interface))
         arr = np.asarray(values)
         if dtype is None:
             if arr.dtype == np.bool_:

@@ -16,28 +16,38 @@ from .common import BACKEND, dev
 
 def _want(name, what, info, shape, dtype):
     """`shape` holds sizes, or None where any size goes."""
-    if info.dtype != dtype or len(info.shape) != len(shape) or \
-            any(w is not None and int(g) != w for g, w in zip(info.shape, shape)):
-        raise ValueError("%s: %s must be %s %s, but got %s %s" %
-                         (name, what, dtype, ["any" if w is None else w for w in shape],
-                          info.dtype, list(info.shape)))
-    if any(int(d) <= 0 for d in info.shape):
-        raise ValueError("%s: %s has an empty dimension: %s" % (name, what, list(info.shape)))
+    got = info.shape
+    if info.dtype == dtype:
+        if got == shape:
+            if 0 not in got:
+                return
+        elif len(got) == len(shape):
+            for w, g in zip(shape, got):
+                if g <= 0 or (w is not None and g != w):
+                    break
+            else:
+                return
+    if 0 in got and info.dtype == dtype and len(got) == len(shape) and \
+            all(w is None or g == w for w, g in zip(shape, got)):
+        raise ValueError("%s: %s has an empty dimension: %s" % (name, what, list(got)))
+    raise ValueError("%s: %s must be %s %s, but got %s %s" %
+                     (name, what, dtype, ["any" if w is None else w for w in shape],
+                      info.dtype, list(got)))
 
 
 def _paged(name, inp):
     """Checks the pools, the table and the lengths; the parameters and the rows' capacity."""
     kc, vc, table, lengths = inp["kCache"], inp["vCache"], inp["pageTable"], inp["lengths"]
     _want(name, "kCache", kc, [None] * 4, "float32")
-    _want(name, "vCache", vc, [int(d) for d in kc.shape], "float32")
+    _want(name, "vCache", vc, kc.shape, "float32")
     if kc.dataId is vc.dataId:
         raise ValueError("%s: kCache and vCache are the same tensor" % name)
     _want(name, "lengths", lengths, [None], "int32")
-    batch = int(lengths.shape[0])
+    batch = lengths.shape[0]
     _want(name, "pageTable", table, [batch, None], "int32")
     p = _cabi.PagedParams()
-    p.batch, p.max_pages = batch, int(table.shape[1])
-    p.num_pages, p.kv_heads, p.page_size, p.head_dim = [int(d) for d in kc.shape]
+    p.batch, p.max_pages = batch, table.shape[1]
+    p.num_pages, p.kv_heads, p.page_size, p.head_dim = kc.shape
     return p, p.max_pages * p.page_size
 
 
@@ -74,11 +84,11 @@ def _paged_cache_append(args):
     p, _ = _paged(name, inp)
     k, v, counts = inp["k"], inp["v"], inp.get("counts")
     _want(name, "k", k, [p.batch, p.kv_heads, None, p.head_dim], "float32")
-    _want(name, "v", v, [int(d) for d in k.shape], "float32")
+    _want(name, "v", v, k.shape, "float32")
     if counts is not None:
         _want(name, "counts", counts, [p.batch], "int32")
     _not_a_pool(name, inp, ("k", "v"))
-    p.tokens = int(k.shape[2])
+    p.tokens = k.shape[2]
     reads = [dev(backend, t) for t in (k, v, inp["pageTable"], inp["lengths"], counts)]
     pools = [backend.device_id_for_update(inp[n].dataId) for n in ("kCache", "vCache")]
     return _outputs(backend, [([p.batch], "int32")],
@@ -92,7 +102,7 @@ def _paged_attention(args):
     p, capacity = _paged(name, inp)
     q, mask, weights = inp["q"], inp.get("mask"), inp.get("weights")
     _want(name, "q", q, [p.batch, None, 1, p.head_dim], "float32")
-    p.heads = int(q.shape[1])
+    p.heads = q.shape[1]
     if p.heads % p.kv_heads:
         raise ValueError("%s: %d query heads do not share %d key-value heads evenly" %
                          (name, p.heads, p.kv_heads))
@@ -143,10 +153,10 @@ def _linear_attention(args):
     state, lengths = inp.get("state"), inp.get("lengths")
     _want(name, "q", q, [None] * 4, "float32")
     p = _cabi.LinearAttentionParams()
-    p.batch, p.heads, p.seq, p.dim_k = [int(d) for d in q.shape]
-    _want(name, "k", k, [int(d) for d in q.shape], "float32")
+    p.batch, p.heads, p.seq, p.dim_k = q.shape
+    _want(name, "k", k, q.shape, "float32")
     _want(name, "v", v, [p.batch, p.heads, p.seq, None], "float32")
-    p.dim_v = int(v.shape[3])
+    p.dim_v = v.shape[3]
     _want(name, "logDecay", decay, [p.heads], "float32")
     states = [p.batch, p.heads, p.dim_k, p.dim_v]
     if state is not None:
