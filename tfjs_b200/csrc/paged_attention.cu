@@ -13,9 +13,10 @@
 // the four warps that compute: the bytes in flight do not depend on registers.  Head sizes that
 // are no multiple of four values (rows not on 16 bytes) take a kernel with plain loads.
 //
-// Arithmetic, for 1 or 2 query heads a key-value head: fp32 multiply-adds.  For more, the
+// Arithmetic, for up to 4 query heads a key-value head: fp32 multiply-adds.  For more, the
 // multiply-adds and the sums across lanes took four times as long as memory (8 heads of 64: 321 us
-// where the bytes take 83), so the products run as m16n8k8 TF32 MMAs with each operand split into
+// where the bytes take 83; 144 with MMAs, whose 16 rows half a group of 4 would leave empty:
+// 196 against 148 us with 4 heads of 128), so the products run as m16n8k8 TF32 MMAs with each operand split into
 // two TF32 parts and three products (fp32 accuracy; the single query row of a decode step has no
 // tile for the 128-row tcgen05 form).  Tensor cores cut sums off instead of rounding them, so
 // sums over a tile start from zero and are added to fp32 registers.
@@ -341,9 +342,15 @@ struct FmaState {
         v[r] = d < D && (all || (seen >> row & 1u)) ? *reinterpret_cast<const float4*>(vt + row * D + d)
                                                     : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+      float p_row[GT];
+      if constexpr (GT == 4)
+        *reinterpret_cast<float4*>(p_row) = *reinterpret_cast<const float4*>(p_s + row * GT);
+      else
+#pragma unroll
+        for (int gi = 0; gi < GT; ++gi) p_row[gi] = p_s[row * GT + gi];
 #pragma unroll
       for (int gi = 0; gi < GT; ++gi) {
-        const float p = p_s[row * GT + gi];
+        const float p = p_row[gi];
 #pragma unroll
         for (int r = 0; r < VR; ++r) {
           acc[gi][r].x = fmaf(p, v[r].x, acc[gi][r].x);
@@ -686,21 +693,26 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
     State::load_queries(g, a, pc, q_s, tid);
     st.reset();
     compute_barrier();
+    // lane j looks after slot t0 + j: its page, and what the mask adds to it (fetched a tile ahead)
+    auto look = [&](int t, int& page, float& add) {
+      const int mine = pc.begin + t * T + warp * TW + lane;
+      page = -1;
+      add = 0.f;
+      if (lane < TW && mine < pc.end) {
+        page = __ldg(g.table + (size_t)pc.b * g.max_pages + (g.page_shift >= 0 ? mine >> g.page_shift : mine / g.page_size));
+        if (a.mask) add = __ldg(a.mask + (uint64_t)pc.b * g.capacity + mine);
+      }
+    };
+    int page, next_page;
+    float add, next_add;
+    look(0, next_page, next_add);
     for (int t = 0; t < pc.tiles; ++t) {
       const int t0 = pc.begin + t * T + warp * TW;
-      // lane j looks after slot t0 + j: is it there, and what does the mask add to it
-      const int mine = t0 + lane;
-      float add = 0.f;
-      bool there = lane < TW && mine < pc.end;
-      if (there) {
-        const int pi = g.page_shift >= 0 ? mine >> g.page_shift : mine / g.page_size;
-        there = (unsigned)__ldg(g.table + (size_t)pc.b * g.max_pages + pi) < (unsigned)g.num_pages;
-        if (a.mask) {
-          add = __ldg(a.mask + (uint64_t)pc.b * g.capacity + mine);
-          there = there && add != -INFINITY;              // hidden: what it holds, NaN included, does not count
-        }
-      }
-      const uint32_t seen = __ballot_sync(0xffffffffu, there);
+      page = next_page;
+      add = next_add;
+      look(t + 1, next_page, next_add);
+      // (a slot hidden by the mask does not count, whatever it holds, NaN included)
+      const uint32_t seen = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)g.num_pages && add != -INFINITY);
       // (a wait that gives up marks the launch as failed; the rest runs through without waiting)
       if (alive && !warp_wait(full(slot), phase)) {
         alive = false;
@@ -942,12 +954,15 @@ paged_attention_loads_kernel(const PagedLayout g, const PagedAttnArgs a) {
 // A block takes query heads `part`, part + per, ... of a row and key-value head (results that
 // several blocks worked on) and, with weights, every per-th stretch of its slots: the accumulated
 // weights are the old ones plus the group's probabilities, summed in the order of the heads.
+// V slots a thread: 4 where the rows of the weights are on 16 bytes, else 1.
 constexpr int kJoinThreads = 256;
 
+template <int V>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_attention_join_kernel(const PagedLayout g, const PagedAttnArgs a, const float* __restrict__ weights,
                             float* __restrict__ out_weights, int per) {
   extern __shared__ float2 stat[];               // [group]: maximum, 1 / sum (0 for an empty row)
+  __shared__ float sums[kJoinThreads];
   __shared__ int part0_s, parts_s;
   const int unit = blockIdx.x / per;             // row * kv_heads + head
   const int part = blockIdx.x - unit * per;
@@ -955,10 +970,14 @@ paged_attention_join_kernel(const PagedLayout g, const PagedAttnArgs a, const fl
   const int n = paged_length(g, b);
   const uint64_t head0 = (uint64_t)b * a.heads + h * a.group;
   const int per_row = g.kv_heads * a.group_chunks;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // threads side by side along head_dim, `lines` parts at a time
+  const int width = g.head_dim <= 32 ? 32 : g.head_dim <= 64 ? 64 : g.head_dim <= 128 ? 128 : 256;
+  const int lines = kJoinThreads / width, d = tid & (width - 1), line = tid / width;
   Shares sh;
-  if (threadIdx.x < 32) sh = shares_of(g, a, b, -1);
+  if (warp == 0) sh = shares_of(g, a, b, -1);
   for (int gc = 0; gc < a.group_chunks; ++gc) {
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
       // the blocks among which this unit's tiles lie
       const int hc = h * a.group_chunks + gc;
       const long long t = row_tiles(g, a, b), first = sh.before * per_row + hc * t;
@@ -969,50 +988,73 @@ paged_attention_join_kernel(const PagedLayout g, const PagedAttnArgs a, const fl
     __syncthreads();
     const int part0 = part0_s, parts = parts_s;
     const int heads = min(a.chunk, a.group - gc * a.chunk);
-    for (int gi = threadIdx.x; gi < heads; gi += kJoinThreads) {
+    for (int gi = warp; gi < heads; gi += kJoinThreads / 32) {
       const float2* ml = a.part_ml + (uint64_t)part0 * a.chunk + gi;
       float mx = -INFINITY, sum = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < parts; ++i) mx = fmaxf(mx, ml[(uint64_t)i * a.chunk].x);
-#pragma unroll 4
-      for (int i = 0; i < parts; ++i)
-        sum = fmaf(ml[(uint64_t)i * a.chunk].y, exp_from(ml[(uint64_t)i * a.chunk].x, mx), sum);
-      stat[gc * a.chunk + gi] = make_float2(mx, sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum));
+      for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, ml[(uint64_t)i * a.chunk].x);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      for (int i = lane; i < parts; i += 32) {
+        const float2 x = ml[(uint64_t)i * a.chunk];
+        sum = fmaf(x.y, exp_from(x.x, mx), sum);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) stat[gc * a.chunk + gi] = make_float2(mx, sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum));
     }
     __syncthreads();
     if (parts > 1)
       for (int gi = part; gi < heads; gi += per) {
         const float2* ml = a.part_ml + (uint64_t)part0 * a.chunk + gi;
-        const float mx = stat[gc * a.chunk + gi].x;
-        for (int d = threadIdx.x; d < g.head_dim; d += kJoinThreads) {
-          float o = 0.f, sum = 0.f;
+        const float* acc = a.part_acc + ((uint64_t)part0 * a.chunk + gi) * g.head_dim + d;
+        const float2 st = stat[gc * a.chunk + gi];
+        float o = 0.f;
+        if (d < g.head_dim) {
 #pragma unroll 8
-          for (int i = 0; i < parts; ++i) {
-            const float2 x = ml[(uint64_t)i * a.chunk];
-            const float f = exp_from(x.x, mx);
-            o = fmaf(a.part_acc[((uint64_t)(part0 + i) * a.chunk + gi) * g.head_dim + d], f, o);
-            sum = fmaf(x.y, f, sum);
-          }
-          a.out[(head0 + gc * a.chunk + gi) * g.head_dim + d] = sum == 0.f ? 0.f : __fdiv_rn(o, sum);
+          for (int i = line; i < parts; i += lines)
+            o = fmaf(acc[(uint64_t)i * a.chunk * g.head_dim], exp_from(ml[(uint64_t)i * a.chunk].x, st.x), o);
         }
+        sums[tid] = o;
+        __syncthreads();
+        if (line == 0 && d < g.head_dim) {
+          for (int x = 1; x < lines; ++x) o += sums[x * width + d];
+          a.out[(head0 + gc * a.chunk + gi) * g.head_dim + d] = __fmul_rn(o, st.y);
+        }
+        __syncthreads();
       }
-    __syncthreads();
   }
   if (out_weights == nullptr) return;
   const float* sc = a.scores + head0 * g.capacity;
-  for (int j = part * kJoinThreads + (int)threadIdx.x; j < g.capacity; j += per * kJoinThreads) {
-    float w = 0.f;
+  const float* old = weights + (uint64_t)unit * g.capacity;
+  for (int j = (part * kJoinThreads + tid) * V; j < g.capacity; j += per * kJoinThreads * V) {
+    float w[V], o[V];
+#pragma unroll
+    for (int x = 0; x < V; ++x) w[x] = o[x] = 0.f;
     if (j < n) {
-      const float old = __ldg(weights + (uint64_t)unit * g.capacity + j);
-#pragma unroll 8
+      if constexpr (V == 4)
+        *reinterpret_cast<float4*>(o) = __ldg(reinterpret_cast<const float4*>(old + j));
+      else
+        o[0] = __ldg(old + j);
+#pragma unroll 4
       for (int gi = 0; gi < a.group; ++gi) {
         const float2 st = stat[gi];
+        float s[V];
+        if constexpr (V == 4)
+          *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sc + (uint64_t)gi * g.capacity + j);
+        else
+          s[0] = sc[(uint64_t)gi * g.capacity + j];
         // (an empty row has 1 / sum = 0 and scores of -infinity only)
-        w = fmaf(exp_from(sc[(uint64_t)gi * g.capacity + j], st.x), st.y, w);
+#pragma unroll
+        for (int x = 0; x < V; ++x) w[x] = fmaf(exp_from(s[x], st.x), st.y, w[x]);
       }
-      w += old;
+      // (what lies behind the row's end was never written and is dropped here)
+#pragma unroll
+      for (int x = 0; x < V; ++x) w[x] = j + x < n ? w[x] + o[x] : 0.f;
     }
-    out_weights[(uint64_t)unit * g.capacity + j] = w;
+    if constexpr (V == 4)
+      *reinterpret_cast<float4*>(out_weights + (uint64_t)unit * g.capacity + j) = *reinterpret_cast<float4*>(w);
+    else
+      out_weights[(uint64_t)unit * g.capacity + j] = w[0];
   }
 }
 
@@ -1081,9 +1123,9 @@ struct Form {
     {plan_loads<32, GT>, launch_loads<32, GT>}, {plan_loads<64, GT>, launch_loads<64, GT>}, \
     {plan_loads<128, GT>, launch_loads<128, GT>}, {plan_loads<256, GT>, launch_loads<256, GT>} \
   }
-// [query heads of a key-value head: 1, 2, to 8, more; plain loads: 1, more][head size]
-const Form kForms[6][4] = {BULK_FORMS(1, false), BULK_FORMS(2, false), BULK_FORMS(8, true), BULK_FORMS(16, true),
-                           LOAD_FORMS(1), LOAD_FORMS(8)};
+// [query heads of a key-value head: 1, 2, to 4, to 8, more; plain loads: 1, more][head size]
+const Form kForms[7][4] = {BULK_FORMS(1, false), BULK_FORMS(2, false), BULK_FORMS(4, false), BULK_FORMS(8, true),
+                           BULK_FORMS(16, true), LOAD_FORMS(1), LOAD_FORMS(8)};
 
 }  // namespace
 
@@ -1134,7 +1176,8 @@ extern "C" int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_pag
   float* owp = ow ? (float*)ow->ptr : nullptr;
 
   const bool wide = p->head_dim % 4 == 0 && (((uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0;
-  const int by_group = !wide ? (a.group == 1 ? 4 : 5) : a.group == 1 ? 0 : a.group == 2 ? 1 : a.group <= 8 ? 2 : 3;
+  const int by_group = !wide ? (a.group == 1 ? 5 : 6)
+                             : a.group <= 2 ? a.group - 1 : a.group <= 4 ? 2 : a.group <= 8 ? 3 : 4;
   const int by_dim = p->head_dim <= 32 ? 0 : p->head_dim <= 64 ? 1 : p->head_dim <= 128 ? 2 : 3;
   const Form& form = kForms[by_group][by_dim];
   const Plan plan = form.plan(ctx, p->head_dim);
@@ -1163,10 +1206,16 @@ extern "C" int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_pag
   if (weights_id || !a.whole) {
     // blocks for the heads to join, and one for every four slots a thread
     uint64_t per = a.whole ? 1 : a.group;
-    if (weights_id && per < (cap + 1023) / 1024) per = (cap + 1023) / 1024;
+    const bool four = weights_id && cap % 4 == 0 && (((uintptr_t)wp | (uintptr_t)owp) & 15) == 0;
+    const uint64_t stretch = kJoinThreads * 4;
+    if (weights_id && per < (cap + stretch - 1) / stretch) per = (cap + stretch - 1) / stretch;
     if (per * kv_units > 0x7fffffffull) per = 0x7fffffffull / kv_units;
-    paged_attention_join_kernel<<<(unsigned)(kv_units * per), kJoinThreads, a.group * sizeof(float2), ctx->stream>>>(
-        g, a, wp, owp, (int)per);
+    const unsigned grid = (unsigned)(kv_units * per);
+    const unsigned stat = a.group * sizeof(float2);
+    if (four)
+      paged_attention_join_kernel<4><<<grid, kJoinThreads, stat, ctx->stream>>>(g, a, wp, owp, (int)per);
+    else
+      paged_attention_join_kernel<1><<<grid, kJoinThreads, stat, ctx->stream>>>(g, a, wp, owp, (int)per);
     LAUNCH_CHECK(ctx, "paged_attention_join_kernel");
     if (weights_id) ctx_mark_written(ctx, out_weights_id);
   }
