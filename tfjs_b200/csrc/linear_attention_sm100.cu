@@ -26,7 +26,9 @@
 namespace {
 
 constexpr int kC = 128;            // tokens of a chunk = rows of an MMA
-constexpr int kProducers = 8;      // warps
+constexpr int kProducers = 8;      // warps 0-7: load, split, store operands; 8-11: one per quarter of
+                                   // the tensor-memory lanes
+constexpr int kThreads = (kProducers + 4) * 32;
 constexpr int kMaxStages = 4;
 constexpr int kSmemCap = 232448;
 
@@ -57,16 +59,30 @@ __device__ __forceinline__ Item item_of(const ChunkArgs& g, int i) {
   return t;
 }
 
-// Four values of a row of `dim` from column d on, zeros outside.
-template <bool WIDE>
-__device__ __forceinline__ float4 load_cols(const float* row, int d, int dim) {
-  if (WIDE) return d < dim ? __ldg(reinterpret_cast<const float4*>(row + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+// Four values of a row of `dim` from column d on (p points there), zeros outside and where !in.
+// Volatile, so that a stage's loads are issued together and early: left to itself the compiler
+// moves each one down to its use.  Predicated, since a branch a load costs as much as the rest.
+__device__ __forceinline__ float4 load16(const float* p, bool in) {
   float4 r;
-  r.x = d < dim ? __ldg(row + d) : 0.f;
-  r.y = d + 1 < dim ? __ldg(row + d + 1) : 0.f;
-  r.z = d + 2 < dim ? __ldg(row + d + 2) : 0.f;
-  r.w = d + 3 < dim ? __ldg(row + d + 3) : 0.f;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\tmov.f32 %2, 0f00000000;\n\tmov.f32 %3, 0f00000000;\n\t"
+      "@q ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "l"(p), "r"((int)in));
   return r;
+}
+__device__ __forceinline__ float load1(const float* p, bool in) {
+  float r;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@q ld.global.nc.f32 %0, [%1];\n\t}"
+      : "=f"(r) : "l"(p), "r"((int)in));
+  return r;
+}
+template <bool WIDE>
+__device__ __forceinline__ float4 load_cols(const float* p, int d, int dim, bool in) {
+  if (WIDE) return load16(p, in && d < dim);
+  return make_float4(load1(p, in && d < dim), load1(p + 1, in && d + 1 < dim), load1(p + 2, in && d + 2 < dim),
+                     load1(p + 3, in && d + 3 < dim));
 }
 
 // x rounded to TF32's 11 bits, to nearest
@@ -151,11 +167,9 @@ constexpr uint32_t kAMN = 1u << 15, kBMN = 1u << 16;
 __device__ __forceinline__ uint32_t n_field(int n) { return (uint32_t)(n >> 3) << 17; }
 
 // ---- A^T of every chunk: M = dim_v tile, N = dim_k, K = tokens ------------------------------
-// warps 0-7 producers, 8-11 epilogue, 12 MMA
-constexpr int kStateThreads = (kProducers + 4 + 1) * 32;
-
-template <bool WIDE>
-__global__ void __launch_bounds__(kStateThreads, 1)
+// Warp 12's first thread issues the MMAs.  NK: at most that many blocks of 32 columns of K.
+template <bool WIDE, int NK>
+__global__ void __launch_bounds__(kThreads + 32, 1)
 linear_chunk_states_kernel(const ChunkArgs g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -194,57 +208,84 @@ linear_chunk_states_kernel(const ChunkArgs g) {
   // accumulators of hi hi and of the small products: twice where 512 columns hold that
   const uint32_t bufs = g.dkp <= 128 ? 2u : 1u;
   if (warp < kProducers) {
-    const int tid = threadIdx.x;
-    uint32_t st = 0;
-    bool alive = true;
-    for (int i = blockIdx.x; alive && i < g.items; i += gridDim.x) {
-      const Item t = item_of(g, i);
-      if (t.n == 0) continue;
-      const float ld = __ldg(g.a.log_decay + t.h);
-      const uint64_t row0 = (uint64_t)t.unit * g.a.seq + (uint64_t)t.c * kC;
-      const int steps = (t.n + 31) / 32;
-      for (int ks = 0; ks < steps; ++ks, ++st) {
-        const int s = st % g.stages;
-        const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
-        // 32 rows x (nbv + nbk) blocks of eight 16-byte pieces; thread: row tid / 8, one piece
-        // of every block
-        const int r = tid >> 3, c4 = tid & 7;
-        const int j = ks * 32 + r;
-        const bool in = j < t.n;
-        float4 xv[4], xk[8];
-#pragma unroll
-        for (int blk = 0; blk < 4; ++blk)
-          if (blk < nbv)
-            xv[blk] = in ? load_cols<WIDE>(g.a.v + (row0 + j) * g.a.dv, t.dv0 + blk * 32 + c4 * 4, g.a.dv)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int blk = 0; blk < 8; ++blk)
-          if (blk < nbk)
-            xk[blk] = in ? load_cols<WIDE>(g.a.k + (row0 + j) * g.a.dk, blk * 32 + c4 * 4, g.a.dk)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float w = in ? decay_power(ld, t.n - 1 - j) : 0.f;
-        if (!warp_wait(empty(s), ((st / g.stages) & 1) ^ 1)) {
-          if (lane == 0) atomicExch(g.a.flag, 1);
-          alive = false;
-          break;
-        }
-        const uint32_t at = mn_major(r, c4);
-#pragma unroll
-        for (int blk = 0; blk < 4; ++blk)
-          if (blk < nbv) store_split(sb + blk * 4096u + at, sb + 16384u + blk * 4096u + at, xv[blk]);
-#pragma unroll
-        for (int blk = 0; blk < 8; ++blk)
-          if (blk < nbk) {
-            xk[blk].x *= w;
-            xk[blk].y *= w;
-            xk[blk].z *= w;
-            xk[blk].w *= w;
-            store_split(sb + k_off + blk * 4096u + at, sb + k_off + k_bytes + blk * 4096u + at, xk[blk]);
-          }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full(s));
+    // A thread has a token of the stage and a 16-byte piece of each of its blocks.  Two stages are
+    // in flight: the next one's loads are issued before this one's values are split and stored.
+    const int r0 = (int)threadIdx.x >> 3, c4 = (int)threadIdx.x & 7;
+    constexpr int S = 4 + NK;
+    struct Stage {
+      int i, ks;
+      Item t;
+      float ld;
+    };
+    auto settle = [&](Stage& s) {                  // the next item that has tokens, from s.i on
+      for (; s.i < g.items; s.i += gridDim.x) {
+        s.t = item_of(g, s.i);
+        if (s.t.n > 0) break;
       }
+      s.ks = 0;
+      if (s.i < g.items) s.ld = __ldg(g.a.log_decay + s.t.h);
+    };
+    auto next = [&](Stage& s) {
+      if ((++s.ks) * 32 >= s.t.n) {
+        s.i += gridDim.x;
+        settle(s);
+      }
+    };
+    auto load = [&](const Stage& s, float4 (&x)[S]) {
+      if (s.i >= g.items) return;
+      const int j = s.ks * 32 + r0;
+      const bool in = j < s.t.n;
+      const uint64_t row = (uint64_t)s.t.unit * g.a.seq + (uint64_t)s.t.c * kC + (in ? j : 0);
+      const float* pv = g.a.v + row * g.a.dv + s.t.dv0 + c4 * 4;
+      const float* pk = g.a.k + row * g.a.dk + c4 * 4;
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (y < nbv) x[y] = load_cols<WIDE>(pv + y * 32, s.t.dv0 + y * 32 + c4 * 4, g.a.dv, in);
+#pragma unroll
+      for (int y = 0; y < NK; ++y)
+        if (y < nbk) x[4 + y] = load_cols<WIDE>(pk + y * 32, y * 32 + c4 * 4, g.a.dk, in);
+    };
+    uint32_t slot = 0, phase = 1;
+    auto store = [&](const Stage& s, float4 (&x)[S]) -> bool {
+      const uint32_t at = base + slot * (uint32_t)g.stage_bytes + mn_major(r0, c4);
+      const int j = s.ks * 32 + r0;
+      const float w = j < s.t.n ? decay_power(s.ld, s.t.n - 1 - j) : 0.f;
+      if (!warp_wait(empty(slot), phase)) {
+        if (lane == 0) atomicExch(g.a.flag, 1);
+        return false;
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (y < nbv) store_split(at + y * 4096u, at + 16384u + y * 4096u, x[y]);
+      const uint32_t k_hi = at + k_off, k_lo = k_hi + k_bytes;
+#pragma unroll
+      for (int y = 0; y < NK; ++y)
+        if (y < nbk)
+          store_split(k_hi + y * 4096u, k_lo + y * 4096u,
+                      make_float4(x[4 + y].x * w, x[4 + y].y * w, x[4 + y].z * w, x[4 + y].w * w));
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full(slot));
+      if (++slot == (uint32_t)g.stages) {
+        slot = 0;
+        phase ^= 1;
+      }
+      return true;
+    };
+    Stage a, b;
+    float4 xa[S], xb[S];
+    a.i = blockIdx.x;
+    settle(a);
+    load(a, xa);
+    while (a.i < g.items) {
+      b = a;
+      next(b);
+      load(b, xb);
+      if (!store(a, xa) || b.i >= g.items) break;
+      a = b;
+      next(a);
+      load(a, xa);
+      if (!store(b, xb)) break;
     }
   } else if (warp == 12) {
     if (lane == 0) {
@@ -329,64 +370,62 @@ linear_chunk_states_kernel(const ChunkArgs g) {
 }
 
 // ---- states between the chunks -----------------------------------------------------------
-// A thread carries one element of the (transposed) state through all chunks of its row; eight
-// chunks are in flight, since each is a dependent step of one multiply-add.
+// A thread carries V neighbouring elements of the (transposed) state through all chunks of its
+// row; eight chunks are in flight, since each is a dependent step of one multiply-add.
+template <int V>
 __global__ void __launch_bounds__(256)
 linear_chunk_scan_kernel(const ChunkArgs g, int blocks_per_unit) {
   const int unit = blockIdx.x / blocks_per_unit;
-  const int e = (blockIdx.x - unit * blocks_per_unit) * 256 + (int)threadIdx.x;
+  const int e = ((blockIdx.x - unit * blocks_per_unit) * 256 + (int)threadIdx.x) * V;
   const int size = g.a.dv * g.a.dk;
   if (e >= size) return;
   const int b = unit / g.a.heads, h = unit - b * g.a.heads;
   const int n = linear_length(g.a, b);
   const int nc = (n + kC - 1) / kC;
-  const int row = e / g.a.dk, col = e - row * g.a.dk;      // dim_v, dim_k
+  const int row = e / g.a.dk, col = e - row * g.a.dk;      // dim_v, dim_k (V divides dim_k)
   const uint64_t at = (uint64_t)unit * size + (uint64_t)col * g.a.dv + row;
   const float ld = __ldg(g.a.log_decay + h);
   const float whole = decay_power(ld, kC), last = decay_power(ld, n - (nc - 1) * kC);
-  float s = g.a.state ? __ldg(g.a.state + at) : 0.f;
+  struct __align__(V * 4) Vec { float x[V]; };
+  Vec s;
+#pragma unroll
+  for (int v = 0; v < V; ++v) s.x[v] = g.a.state ? __ldg(g.a.state + at + (uint64_t)v * g.a.dv) : 0.f;
   float* p = g.states + (uint64_t)unit * g.chunks * size + e;
   constexpr int U = 8;
-  int c = 0;
-  for (; c + U < nc; c += U) {
-    float x[U];
+  for (int c = 0; c < nc; c += U) {
+    Vec x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = p[(uint64_t)(c + u) * size];
+    for (int u = 0; u < U; ++u)
+      if (c + u < nc) x[u] = *reinterpret_cast<const Vec*>(p + (uint64_t)(c + u) * size);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      p[(uint64_t)(c + u) * size] = s;
-      s = fmaf(s, whole, x[u]);
-    }
+    for (int u = 0; u < U; ++u)
+      if (c + u < nc) {
+        *reinterpret_cast<Vec*>(p + (uint64_t)(c + u) * size) = s;
+        const float w = c + u + 1 < nc ? whole : last;
+#pragma unroll
+        for (int v = 0; v < V; ++v) s.x[v] = fmaf(s.x[v], w, x[u].x[v]);
+      }
   }
-  for (; c < nc; ++c) {
-    const float x = p[(uint64_t)c * size];
-    p[(uint64_t)c * size] = s;
-    s = fmaf(s, c + 1 < nc ? whole : last, x);
-  }
-  g.a.out_state[at] = s;
+#pragma unroll
+  for (int v = 0; v < V; ++v) g.a.out_state[at + (uint64_t)v * g.a.dv] = s.x[v];
 }
 
 // ---- outputs -------------------------------------------------------------------------------
-// warps 0-7 producers, 8-15 two per quarter of the tensor-memory lanes (scores to decayed
-// probabilities, then the result), 16 MMA.
 // Tensor memory, in columns (hi hi sums left, sums of the small products right):
 //   [0, 128) scores, later the probabilities' hi parts     [256, 384) scores, later their lo parts
 //   [128, 256) Q S, later decayed                          [384, 512) Q S, later P V
-constexpr int kOutThreads = (kProducers + 8 + 1) * 32;
-
 template <bool WIDE>
-__global__ void __launch_bounds__(kOutThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 linear_chunk_outputs_kernel(const ChunkArgs g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t tiles = base + (uint32_t)(g.stages * g.stage_bytes);
-  const uint32_t bars = tiles + 8 * 4096u;
+  const uint32_t bars = tiles + 4 * 4096u;
   auto full = [&](int s) { return bars + 8u * (uint32_t)s; };
   auto empty = [&](int s) { return bars + 8u * (uint32_t)(kMaxStages + s); };
-  const uint32_t s_full = bars + 8u * (2 * kMaxStages), p_full = s_full + 8u, o_full = s_full + 16u,
-                 o_empty = s_full + 24u;
-  const uint32_t tmem_slot = s_full + 32u;
-  const uint32_t power_s = tmem_slot + 8u;                 // float[kC + 1] per transforming warp set
+  const uint32_t s_full = bars + 8u * (2 * kMaxStages), o_full = s_full + 8u;
+  const uint32_t tmem_slot = s_full + 16u;
+  const uint32_t power_s = tmem_slot + 8u;                 // float[kC + 1]
   float* power = reinterpret_cast<float*>(smem_raw + (power_s - smem_u32(smem_raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -395,12 +434,10 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       mbar_init(empty(s), 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_full, 8);
     mbar_init(o_full, 1);
-    mbar_init(o_empty, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 16) {
+  if (warp == kProducers) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -417,104 +454,129 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
   const uint32_t b_off = 32768u, b_bytes = (uint32_t)(128 + g.dvp) * 128u;
   const uint32_t v_bytes = 64u * (uint32_t)g.dvp * 4u;
   if (warp < kProducers) {
-    const int tid = threadIdx.x;
-    const int r0 = tid >> 3, c4 = tid & 7;                 // 32 rows at a time, eight pieces each
-    uint32_t st = 0;
-    bool alive = true;
-    for (int i = blockIdx.x; alive && i < g.items; i += gridDim.x) {
-      const Item t = item_of(g, i);
-      if (t.n == 0) continue;
-      const uint64_t row0 = (uint64_t)t.unit * g.a.seq + (uint64_t)t.c * kC;
-      const float* sp = g.states + ((uint64_t)t.unit * g.chunks + t.c) * g.a.dv * g.a.dk;
-      for (int ks = 0; ks < nk; ++ks, ++st) {
-        const int s = st % g.stages;
-        const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
-        const int d = ks * 32 + c4 * 4;
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        float4 xq[4], xk[4], xs[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = x * 32 + r0;
-          xq[x] = r < t.n ? load_cols<WIDE>(g.a.q + (row0 + r) * g.a.dk, d, g.a.dk) : zero;
-          xk[x] = r < t.n ? load_cols<WIDE>(g.a.k + (row0 + r) * g.a.dk, d, g.a.dk) : zero;
-          const int dv = t.dv0 + r;
-          xs[x] = x < nbv && dv < g.a.dv ? load_cols<WIDE>(sp + (uint64_t)dv * g.a.dk, d, g.a.dk) : zero;
-        }
-        if (!warp_wait(empty(s), ((st / g.stages) & 1) ^ 1)) {
-          if (lane == 0) atomicExch(g.a.flag, 1);
-          alive = false;
-          break;
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t at = k_major(x * 32 + r0, c4);
-          store_split(sb + at, sb + 16384u + at, xq[x]);
-          store_split(sb + b_off + at, sb + b_off + b_bytes + at, xk[x]);
-          if (x < nbv) store_split(sb + b_off + 16384u + at, sb + b_off + b_bytes + 16384u + at, xs[x]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full(s));
+    // A thread has a 16-byte piece of every 32nd operand row: of 128 of Q, 128 of K, dvp of S^T; or of
+    // each column block of two tokens of V.  Two stages are in flight, as above.
+    const int r0 = (int)threadIdx.x >> 3, c4 = (int)threadIdx.x & 7;
+    constexpr int S = 12;
+    struct Stage {
+      int i, ks;                                   // ks: nk stages of Q, K, S, then those of V
+      Item t;
+    };
+    auto settle = [&](Stage& s) {
+      for (; s.i < g.items; s.i += gridDim.x) {
+        s.t = item_of(g, s.i);
+        if (s.t.n > 0) break;
       }
-      if (!alive) break;
-      const int vsteps = (t.n + 63) / 64;
-      for (int vs = 0; vs < vsteps; ++vs, ++st) {
-        const int s = st % g.stages;
-        const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
-        float4 x[2][4];
+      s.ks = 0;
+    };
+    auto next = [&](Stage& s) {
+      if (++s.ks >= nk + (s.t.n + 63) / 64) {
+        s.i += gridDim.x;
+        settle(s);
+      }
+    };
+    auto load = [&](const Stage& s, float4 (&x)[S]) {
+      if (s.i >= g.items) return;
+      const uint64_t row0 = (uint64_t)s.t.unit * g.a.seq + (uint64_t)s.t.c * kC;
+      if (s.ks < nk) {
+        const int d = s.ks * 32 + c4 * 4;
+        const uint64_t at = (row0 + r0) * g.a.dk + d;
+        const float *pq = g.a.q + at, *pk = g.a.k + at;
+        const float* ps = g.states + (((uint64_t)s.t.unit * g.chunks + s.t.c) * g.a.dv + s.t.dv0 + r0) * g.a.dk + d;
+        const uint32_t by = 32u * (uint32_t)g.a.dk;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const bool in = y * 32 + r0 < s.t.n;
+          x[y] = load_cols<WIDE>(pq + y * by, d, g.a.dk, in);
+          x[4 + y] = load_cols<WIDE>(pk + y * by, d, g.a.dk, in);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (y < nbv) x[8 + y] = load_cols<WIDE>(ps + y * by, d, g.a.dk, s.t.dv0 + y * 32 + r0 < g.a.dv);
+      } else {
 #pragma unroll
         for (int tg = 0; tg < 2; ++tg) {
-          const int j = vs * 64 + tg * 32 + r0;
+          const int j = (s.ks - nk) * 64 + tg * 32 + r0;
+          const bool in = j < s.t.n;
+          const float* pv = g.a.v + (row0 + (in ? j : 0)) * g.a.dv + s.t.dv0 + c4 * 4;
 #pragma unroll
           for (int cb = 0; cb < 4; ++cb)
-            if (cb < nbv)
-              x[tg][cb] = j < t.n ? load_cols<WIDE>(g.a.v + (row0 + j) * g.a.dv, t.dv0 + cb * 32 + c4 * 4, g.a.dv)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (cb < nbv) x[tg * 4 + cb] = load_cols<WIDE>(pv + cb * 32, s.t.dv0 + cb * 32 + c4 * 4, g.a.dv, in);
         }
-        if (!warp_wait(empty(s), ((st / g.stages) & 1) ^ 1)) {
-          if (lane == 0) atomicExch(g.a.flag, 1);
-          alive = false;
-          break;
-        }
-        const uint32_t at = mn_major(r0, c4);
+      }
+    };
+    uint32_t slot = 0, phase = 1;
+    const uint32_t at_k = k_major(r0, c4), at_mn = mn_major(r0, c4);
+    auto store = [&](const Stage& s, float4 (&x)[S]) -> bool {
+      const uint32_t sb = base + slot * (uint32_t)g.stage_bytes;
+      if (!warp_wait(empty(slot), phase)) {
+        if (lane == 0) atomicExch(g.a.flag, 1);
+        return false;
+      }
+      if (s.ks < nk) {
+        const uint32_t q_at = sb + at_k, b_at = q_at + b_off, b_lo = b_at + b_bytes;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) store_split(q_at + y * 4096u, q_at + 16384u + y * 4096u, x[y]);
+#pragma unroll
+        for (int y = 0; y < 8; ++y)                // rows 128 on of B are those of S^T
+          if (y < 4 + nbv) store_split(b_at + y * 4096u, b_lo + y * 4096u, x[4 + y]);
+      } else {
 #pragma unroll
         for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
           for (int cb = 0; cb < 4; ++cb)
             if (cb < nbv) {
-              const uint32_t o = sb + (uint32_t)(tg * nbv + cb) * 4096u + at;
-              store_split(o, o + v_bytes, x[tg][cb]);
+              const uint32_t at = sb + at_mn + (uint32_t)(tg * nbv + cb) * 4096u;
+              store_split(at, at + v_bytes, x[tg * 4 + cb]);
             }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full(s));
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full(slot));
+      if (++slot == (uint32_t)g.stages) {
+        slot = 0;
+        phase ^= 1;
+      }
+      return true;
+    };
+    Stage a, b;
+    float4 xa[S], xb[S];
+    a.i = blockIdx.x;
+    settle(a);
+    load(a, xa);
+    while (a.i < g.items) {
+      b = a;
+      next(b);
+      load(b, xb);
+      if (!store(a, xa) || b.i >= g.items) break;
+      a = b;
+      next(a);
+      load(a, xa);
+      if (!store(b, xb)) break;
     }
-  } else if (warp == 16) {
-    if (lane == 0) {
-      const uint32_t idesc_s = kIdesc | n_field(128 + g.dvp);
-      const uint32_t idesc_o = kIdesc | kBMN | n_field(g.dvp);
-      uint32_t st = 0, done = 0;
-      bool alive = true;
-      for (int i = blockIdx.x; alive && i < g.items; i += gridDim.x) {
-        const Item t = item_of(g, i);
-        if (t.n == 0) continue;
-        // (the probabilities' place is free: the previous item's products, which read it, come first
-        // in this thread's order; the sums must have been read)
-        if (!mbar_wait(o_empty, (done & 1) ^ 1)) {
-          atomicExch(g.a.flag, 7);
-          break;
+  } else {
+    // The first of these warps also issues the MMAs, of which its first thread: the four have nothing
+    // else to do while the scores are formed.
+    const bool issuer = warp == kProducers;
+    const uint32_t idesc_s = kIdesc | n_field(128 + g.dvp);
+    const uint32_t idesc_o = kIdesc | kBMN | n_field(g.dvp);
+    uint32_t slot = 0, phase = 0;
+    auto advance = [&](uint32_t& s, uint32_t& p) {
+      if (++s == (uint32_t)g.stages) {
+        s = 0;
+        p ^= 1;
+      }
+    };
+    // scores (and Q S) of an item, stage by stage
+    auto issue_scores = [&]() -> bool {
+      for (int ks = 0; ks < nk; ++ks) {
+        if (!warp_wait(full(slot), phase)) {
+          if (lane == 0) atomicExch(g.a.flag, 2);
+          return false;
         }
         tc_fence_after();
-        for (int ks = 0; ks < nk; ++ks, ++st) {
-          const int s = st % g.stages;
-          if (!mbar_wait(full(s), (st / g.stages) & 1)) {
-            atomicExch(g.a.flag, 2);
-            alive = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+        if (lane == 0) {
+          const uint32_t sb = base + slot * (uint32_t)g.stage_bytes;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             const uint32_t o = (uint32_t)kk * 32u;
@@ -524,30 +586,30 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
             tc_mma_tf32(t_lo, qh, bl, idesc_s, 1);
             tc_mma_tf32(t_s, qh, bh, idesc_s, (ks | kk) != 0);
           }
-          tc_commit(empty(s));
+          tc_commit(empty(slot));
+          if (ks == nk - 1) tc_commit(s_full);
         }
-        if (!alive) break;
-        tc_commit(s_full);
-        if (!mbar_wait(p_full, done & 1)) {
-          atomicExch(g.a.flag, 3);
-          break;
-        }
-        tc_fence_after();
-        // all small products first, while the sum is small: both halves of V are there by then
-        // (at least two stages)
-        const int vsteps = (t.n + 63) / 64;
-        for (int pass = 0; alive && pass < 2; ++pass)
-          for (int vs = 0; vs < vsteps; ++vs) {
-            const int s = (st + vs) % g.stages;
-            if (pass == 0) {
-              if (!mbar_wait(full(s), ((st + vs) / g.stages) & 1)) {
-                atomicExch(g.a.flag, 4);
-                alive = false;
-                break;
-              }
-              tc_fence_after();
+        __syncwarp();
+        advance(slot, phase);
+      }
+      return true;
+    };
+    // P V: all small products first, while the sum is small; both halves of V are there by then (at
+    // least two stages)
+    auto issue_values = [&](int n) -> bool {
+      const int vsteps = (n + 63) / 64;
+      for (int pass = 0; pass < 2; ++pass) {
+        uint32_t s = slot, p = phase;
+        for (int vs = 0; vs < vsteps; ++vs) {
+          if (pass == 0) {
+            if (!warp_wait(full(s), p)) {
+              if (lane == 0) atomicExch(g.a.flag, 4);
+              return false;
             }
-            const uint32_t sb = base + (uint32_t)(s * g.stage_bytes);
+            tc_fence_after();
+          }
+          if (lane == 0) {
+            const uint32_t sb = base + s * (uint32_t)g.stage_bytes;
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
               const uint32_t o = sb + (uint32_t)((kk >> 2) * nbv) * 4096u + (uint32_t)(kk & 3) * 1024u;
@@ -560,18 +622,25 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
                 mma_tmem_a(t_out, t_s + col, vh, idesc_o, 1);
               }
             }
-            if (pass == 1) tc_commit(empty(s));
+            if (pass == 1) {
+              tc_commit(empty(s));
+              if (vs == vsteps - 1) tc_commit(o_full);
+            }
           }
-        st += vsteps;
-        if (!alive) break;
-        tc_commit(o_full);
-        ++done;
+          __syncwarp();
+          advance(s, p);
+        }
+        if (pass == 1) {
+          slot = s;
+          phase = p;
+        }
       }
-    }
-  } else {
-    const int q = warp & 3, half = (warp - kProducers) >> 2;
+      return true;
+    };
+    auto four_warps = []() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    const int q = warp & 3;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    const uint32_t tile = tiles + (uint32_t)(warp - kProducers) * 4096u;
+    const uint32_t tile = tiles + (uint32_t)q * 4096u;
     const int tok = q * 32 + lane;                         // this thread's row
     uint32_t done = 0;
     int powers_of = -1;
@@ -588,28 +657,28 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
         float z[32];
 #pragma unroll
         for (int x = 0; x < 32; ++x) z[x] = 0.f;
-        for (int cb = half; cb < nbv; cb += 2) store_rows32<WIDE>(tile, lane, z, cb * 32, cols, out_row);
+        for (int cb = 0; cb < nbv; ++cb) store_rows32<WIDE>(tile, lane, z, cb * 32, cols, out_row);
         continue;
       }
-      if (t.h != powers_of) {                              // (the same for all eight warps)
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const int e = (int)threadIdx.x - kProducers * 32;
-        if (e <= kC) power[e] = decay_power(__ldg(g.a.log_decay + t.h), e);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (t.h != powers_of) {                              // (the same for all four warps)
+        four_warps();
+        const float ld = __ldg(g.a.log_decay + t.h);
+        for (int e = (int)threadIdx.x - kProducers * 32; e <= kC; e += 128) power[e] = decay_power(ld, e);
+        four_warps();
         powers_of = t.h;
       }
-      if (!alive) continue;                                // (keeps the barriers above in step)
-      if (!warp_wait(s_full, done & 1)) {
+      // (a warp that gave up takes part in the barriers alone)
+      if (issuer && alive) alive = issue_scores();
+      if (alive && !warp_wait(s_full, done & 1)) {
         if (lane == 0) atomicExch(g.a.flag, 5);
         alive = false;
-        continue;
       }
       tc_fence_after();
+      if (alive) {
 #pragma unroll 1
-      for (int cc = 0; cc < 2; ++cc) {
-        const int j0 = half * 64 + cc * 32;
+      for (int j0 = 0; j0 < kC; j0 += 32) {
         float x[32], lo[32];
-        if (j0 <= q * 32 + 31) {
+        if (j0 <= q * 32) {
           tc_ld32(t_s + lanes + (uint32_t)j0, x);
           tc_ld32(t_lo + lanes + (uint32_t)j0, lo);
 #pragma unroll
@@ -628,7 +697,7 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       }
       const float w = power[tok + 1];
 #pragma unroll 1
-      for (int cb = half; cb < nbv; cb += 2) {
+      for (int cb = 0; cb < nbv; ++cb) {
         float x[32], lo[32];
         tc_ld32(t_inter + lanes + (uint32_t)(cb * 32), x);
         tc_ld32(t_out + lanes + (uint32_t)(cb * 32), lo);
@@ -637,43 +706,38 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
         tmem_store32(t_inter + lanes + (uint32_t)(cb * 32), x);
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      }
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-      if (!warp_wait(o_full, done & 1)) {
+      four_warps();                                        // the probabilities of all rows are there
+      tc_fence_after();
+      if (issuer && alive) alive = issue_values(t.n);
+      if (alive && !warp_wait(o_full, done & 1)) {
         if (lane == 0) atomicExch(g.a.flag, 6);
         alive = false;
-        continue;
       }
       tc_fence_after();
+      if (alive) {
       const bool real = tok < t.n;
-      float x[2][32];                                      // (both blocks first: the sums' place is needed)
+      const float scale = g.a.has_scale ? g.a.scale : 1.0f;
+#pragma unroll 1
+      for (int cb = 0; cb < nbv; ++cb) {
+        float x[32], lo[32];
+        tc_ld32(t_out + lanes + (uint32_t)(cb * 32), x);
+        tc_ld32(t_inter + lanes + (uint32_t)(cb * 32), lo);
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int cb = half + 2 * y;
-        if (cb < nbv) {
-          float lo[32];
-          tc_ld32(t_out + lanes + (uint32_t)(cb * 32), x[y]);
-          tc_ld32(t_inter + lanes + (uint32_t)(cb * 32), lo);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float o = x[y][j] + lo[j];
-            x[y][j] = real ? (g.a.has_scale ? __fmul_rn(o, g.a.scale) : o) : 0.f;
-          }
-        }
+        for (int j = 0; j < 32; ++j) x[j] = real ? __fmul_rn(x[j] + lo[j], scale) : 0.0f;
+        store_rows32<WIDE>(tile, lane, x, cb * 32, cols, out_row);
+      }
       }
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(o_empty);
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-        if (half + 2 * y < nbv) store_rows32<WIDE>(tile, lane, x[y], (half + 2 * y) * 32, cols, out_row);
+      four_warps();                                        // all sums are read: the next products may come
+      tc_fence_after();
       ++done;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == kProducers) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
@@ -688,22 +752,30 @@ int launch_chunks(tfjs_cuda_ctx* ctx, ChunkArgs& g) {
   s.stages = (kSmemCap - s_fixed) / s.stage_bytes;
   if (s.stages > kMaxStages) s.stages = kMaxStages;
   const int s_smem = s_fixed + s.stages * s.stage_bytes;
-  CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
   const unsigned grid = (unsigned)(g.items < ctx->sm_count ? g.items : ctx->sm_count);
-  linear_chunk_states_kernel<WIDE><<<grid, kStateThreads, s_smem, ctx->stream>>>(s);
+  if (g.dkp <= 128) {
+    CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
+    linear_chunk_states_kernel<WIDE, 4><<<grid, kThreads + 32, s_smem, ctx->stream>>>(s);
+  } else {
+    CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
+    linear_chunk_states_kernel<WIDE, 8><<<grid, kThreads + 32, s_smem, ctx->stream>>>(s);
+  }
   LAUNCH_CHECK(ctx, "linear_chunk_states_kernel");
   const unsigned units = (unsigned)(g.a.batch * g.a.heads);
-  const int per = (g.a.dv * g.a.dk + 255) / 256;
-  linear_chunk_scan_kernel<<<units * per, 256, 0, ctx->stream>>>(g, per);
+  const int V = g.a.dk % 4 == 0 ? 4 : 1, per = (g.a.dv * g.a.dk / V + 255) / 256;
+  if (V == 4)
+    linear_chunk_scan_kernel<4><<<units * per, 256, 0, ctx->stream>>>(g, per);
+  else
+    linear_chunk_scan_kernel<1><<<units * per, 256, 0, ctx->stream>>>(g, per);
   LAUNCH_CHECK(ctx, "linear_chunk_scan_kernel");
   const int qk = 32768 + 2 * (128 + g.dvp) * 128, v = 2 * 64 * g.dvp * 4;
   g.stage_bytes = qk > v ? qk : v;
-  const int o_fixed = 1024 + 8 * 4096 + 256 + (kC + 1) * 4;
+  const int o_fixed = 1024 + 4 * 4096 + 256 + (kC + 1) * 4;
   g.stages = (kSmemCap - o_fixed) / g.stage_bytes;
   if (g.stages > kMaxStages) g.stages = kMaxStages;
   const int o_smem = o_fixed + g.stages * g.stage_bytes;
   CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_outputs_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, o_smem));
-  linear_chunk_outputs_kernel<WIDE><<<grid, kOutThreads, o_smem, ctx->stream>>>(g);
+  linear_chunk_outputs_kernel<WIDE><<<grid, kThreads, o_smem, ctx->stream>>>(g);
   LAUNCH_CHECK(ctx, "linear_chunk_outputs_kernel");
   return TFJS_CUDA_OK;
 }
