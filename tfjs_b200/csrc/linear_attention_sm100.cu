@@ -391,20 +391,31 @@ linear_chunk_scan_kernel(const ChunkArgs g, int blocks_per_unit) {
 #pragma unroll
   for (int v = 0; v < V; ++v) s.x[v] = g.a.state ? __ldg(g.a.state + at + (uint64_t)v * g.a.dv) : 0.f;
   float* p = g.states + (uint64_t)unit * g.chunks * size + e;
+  // (two batches: loads behind a batch's stores would otherwise wait for them; 2 x 16 heads of
+  // 128 x 128, 128 chunks: 210 us with one batch of eight in flight)
   constexpr int U = 8;
-  for (int c = 0; c < nc; c += U) {
-    Vec x[U];
+  Vec x[2][U];
+  auto load = [&](int c, Vec (&y)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (c + u < nc) x[u] = *reinterpret_cast<const Vec*>(p + (uint64_t)(c + u) * size);
+      if (c + u < nc) y[u] = *reinterpret_cast<const Vec*>(p + (uint64_t)(c + u) * size);
+  };
+  auto step = [&](int c, const Vec (&y)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (c + u < nc) {
         *reinterpret_cast<Vec*>(p + (uint64_t)(c + u) * size) = s;
         const float w = c + u + 1 < nc ? whole : last;
 #pragma unroll
-        for (int v = 0; v < V; ++v) s.x[v] = fmaf(s.x[v], w, x[u].x[v]);
+        for (int v = 0; v < V; ++v) s.x[v] = fmaf(s.x[v], w, y[u].x[v]);
       }
+  };
+  load(0, x[0]);
+  for (int c = 0; c < nc; c += 2 * U) {
+    load(c + U, x[1]);
+    step(c, x[0]);
+    load(c + 2 * U, x[0]);
+    step(c + U, x[1]);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) g.a.out_state[at + (uint64_t)v * g.a.dv] = s.x[v];
