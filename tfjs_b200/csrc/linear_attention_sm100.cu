@@ -606,46 +606,54 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       return true;
     };
     // P V: all small products first, while the sum is small; both halves of V are there by then (at
-    // least two stages)
+    // least two stages).  (Straight code for each half: a branch an MMA makes one take 140 cycles to
+    // issue, twice what it takes to run.)
     auto issue_values = [&](int n) -> bool {
-      const int vsteps = (n + 63) / 64;
-      for (int pass = 0; pass < 2; ++pass) {
-        uint32_t s = slot, p = phase;
-        for (int vs = 0; vs < vsteps; ++vs) {
-          if (pass == 0) {
-            if (!warp_wait(full(s), p)) {
-              if (lane == 0) atomicExch(g.a.flag, 4);
-              return false;
-            }
-            tc_fence_after();
-          }
-          if (lane == 0) {
-            const uint32_t sb = base + s * (uint32_t)g.stage_bytes;
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk) {
-              const uint32_t o = sb + (uint32_t)((kk >> 2) * nbv) * 4096u + (uint32_t)(kk & 3) * 1024u;
-              const uint32_t col = (uint32_t)(vs * 64 + kk * 8);
-              const uint64_t vh = desc_mn_major(o), vl = desc_mn_major(o + v_bytes);
-              if (pass == 0) {
-                mma_tmem_a(t_out, t_lo + col, vh, idesc_o, (vs | kk) != 0);
-                mma_tmem_a(t_out, t_s + col, vl, idesc_o, 1);
-              } else {
-                mma_tmem_a(t_out, t_s + col, vh, idesc_o, 1);
-              }
-            }
-            if (pass == 1) {
-              tc_commit(empty(s));
-              if (vs == vsteps - 1) tc_commit(o_full);
-            }
-          }
-          __syncwarp();
-          advance(s, p);
-        }
-        if (pass == 1) {
-          slot = s;
-          phase = p;
-        }
+      const bool two = n > 64;
+      const uint32_t s0 = slot, sb0 = base + s0 * (uint32_t)g.stage_bytes;
+      if (!warp_wait(full(slot), phase)) {
+        if (lane == 0) atomicExch(g.a.flag, 4);
+        return false;
       }
+      advance(slot, phase);
+      uint32_t s1 = s0;
+      if (two) {
+        s1 = slot;
+        if (!warp_wait(full(slot), phase)) {
+          if (lane == 0) atomicExch(g.a.flag, 4);
+          return false;
+        }
+        advance(slot, phase);
+      }
+      const uint32_t sb1 = base + s1 * (uint32_t)g.stage_bytes;
+      const uint32_t group = (uint32_t)nbv * 4096u;
+      auto small = [&](uint32_t sb, uint32_t col0, uint32_t begun) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t o = sb + (kk >= 4 ? group : 0u) + (uint32_t)(kk & 3) * 1024u, col = col0 + (uint32_t)(kk * 8);
+          mma_tmem_a(t_out, t_lo + col, desc_mn_major(o), idesc_o, kk ? 1u : begun);
+          mma_tmem_a(t_out, t_s + col, desc_mn_major(o + v_bytes), idesc_o, 1u);
+        }
+      };
+      auto large = [&](uint32_t sb, uint32_t col0) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_tmem_a(t_out, t_s + col0 + (uint32_t)(kk * 8),
+                     desc_mn_major(sb + (kk >= 4 ? group : 0u) + (uint32_t)(kk & 3) * 1024u), idesc_o, 1u);
+      };
+      tc_fence_after();
+      if (lane == 0) {
+        small(sb0, 0u, 0u);
+        if (two) small(sb1, 64u, 1u);
+        large(sb0, 0u);
+        tc_commit(empty(s0));
+        if (two) {
+          large(sb1, 64u);
+          tc_commit(empty(s1));
+        }
+        tc_commit(o_full);
+      }
+      __syncwarp();
       return true;
     };
     auto four_warps = []() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
