@@ -240,10 +240,10 @@ linear_chunk_states_kernel(const ChunkArgs g) {
       const float* pk = g.a.k + row * g.a.dk + c4 * 4;
 #pragma unroll
       for (int y = 0; y < 4; ++y)
-        if (y < nbv) x[y] = load_cols<WIDE>(pv + y * 32, s.t.dv0 + y * 32 + c4 * 4, g.a.dv, in);
+        x[y] = load_cols<WIDE>(pv + y * 32, s.t.dv0 + y * 32 + c4 * 4, g.a.dv, in && y < nbv);
 #pragma unroll
       for (int y = 0; y < NK; ++y)
-        if (y < nbk) x[4 + y] = load_cols<WIDE>(pk + y * 32, y * 32 + c4 * 4, g.a.dk, in);
+        x[4 + y] = load_cols<WIDE>(pk + y * 32, y * 32 + c4 * 4, g.a.dk, in && y < nbk);
     };
     uint32_t slot = 0, phase = 1;
     auto store = [&](const Stage& s, float4 (&x)[S]) -> bool {
@@ -488,32 +488,31 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
     };
     auto load = [&](const Stage& s, float4 (&x)[S]) {
       if (s.i >= g.items) return;
+      // (One load a place whichever kind of stage it is: with two, the compiler copies what one of them
+      // brings, which waits for it, and nothing is in flight any more.)
       const uint64_t row0 = (uint64_t)s.t.unit * g.a.seq + (uint64_t)s.t.c * kC;
-      if (s.ks < nk) {
-        const int d = s.ks * 32 + c4 * 4;
-        const uint64_t at = (row0 + r0) * g.a.dk + d;
-        const float *pq = g.a.q + at, *pk = g.a.k + at;
-        const float* ps = g.states + (((uint64_t)s.t.unit * g.chunks + s.t.c) * g.a.dv + s.t.dv0 + r0) * g.a.dk + d;
-        const uint32_t by = 32u * (uint32_t)g.a.dk;
+      const bool is_v = s.ks >= nk;
+      const int d = s.ks * 32 + c4 * 4;
+      const uint64_t at = (row0 + r0) * g.a.dk + d;
+      const float *pq = g.a.q + at, *pk = g.a.k + at;
+      const float* ps = g.states + (((uint64_t)s.t.unit * g.chunks + s.t.c) * g.a.dv + s.t.dv0 + r0) * g.a.dk + d;
+      const uint32_t by = 32u * (uint32_t)g.a.dk;
+      const int j0 = (s.ks - nk) * 64 + r0;                // V: this thread's tokens are j0 and j0 + 32
+      const float* pv = g.a.v + (row0 + j0) * g.a.dv + s.t.dv0 + c4 * 4;
+      const uint32_t by_v = 32u * (uint32_t)g.a.dv;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const bool in = y * 32 + r0 < s.t.n;
-          x[y] = load_cols<WIDE>(pq + y * by, d, g.a.dk, in);
-          x[4 + y] = load_cols<WIDE>(pk + y * by, d, g.a.dk, in);
+      for (int y = 0; y < 12; ++y) {
+        const int tg = y >> 2, cb = y & 3;                 // V: places 0 to 7
+        const float* p = y < 4 ? pq + y * by : y < 8 ? pk + (y - 4) * by : ps + (y - 8) * by;
+        bool in = y < 8 ? cb * 32 + r0 < s.t.n : cb < nbv && s.t.dv0 + cb * 32 + r0 < g.a.dv;
+        int col = d, dim = g.a.dk;
+        if (is_v) {
+          p = pv + (tg == 1 ? by_v : 0u) + cb * 32;
+          in = y < 8 && cb < nbv && j0 + tg * 32 < s.t.n;
+          col = s.t.dv0 + cb * 32 + c4 * 4;
+          dim = g.a.dv;
         }
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-          if (y < nbv) x[8 + y] = load_cols<WIDE>(ps + y * by, d, g.a.dk, s.t.dv0 + y * 32 + r0 < g.a.dv);
-      } else {
-#pragma unroll
-        for (int tg = 0; tg < 2; ++tg) {
-          const int j = (s.ks - nk) * 64 + tg * 32 + r0;
-          const bool in = j < s.t.n;
-          const float* pv = g.a.v + (row0 + (in ? j : 0)) * g.a.dv + s.t.dv0 + c4 * 4;
-#pragma unroll
-          for (int cb = 0; cb < 4; ++cb)
-            if (cb < nbv) x[tg * 4 + cb] = load_cols<WIDE>(pv + cb * 32, s.t.dv0 + cb * 32 + c4 * 4, g.a.dv, in);
-        }
+        x[y] = load_cols<WIDE>(p, col, dim, in);
       }
     };
     uint32_t slot = 0, phase = 1;
