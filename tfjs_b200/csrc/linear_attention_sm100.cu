@@ -131,6 +131,31 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const float* f) {
       : "memory");
 }
 
+// 32 columns of this thread's lane from two places at once: one wait for both.
+__device__ __forceinline__ void tmem_load32_nowait(uint32_t taddr, float* f) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]),
+        "=f"(f[8]), "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]),
+        "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]), "=f"(f[21]), "=f"(f[22]), "=f"(f[23]),
+        "=f"(f[24]), "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]), "=f"(f[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load_sum32(uint32_t at, uint32_t at_lo, float* x) {
+  float lo[32];
+  tmem_load32_nowait(at, x);
+  tmem_load32_nowait(at_lo, lo);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  // (the registers are there only now: nothing that reads them may come earlier)
+#pragma unroll
+  for (int j = 0; j < 32; ++j) asm volatile("" : "+f"(x[j]), "+f"(lo[j]));
+#pragma unroll
+  for (int j = 0; j < 32; ++j) x[j] += lo[j];
+}
+
 // 32 x 32 values, one row a lane, through a swizzled 4 KB tile of the warp so that global
 // memory is written in rows of 128 bytes.  Row r goes to row_ptr(r) (null: not stored) at
 // columns col .. col + 31 of `dim`.
@@ -344,12 +369,9 @@ linear_chunk_states_kernel(const ChunkArgs g) {
       float* out = g.states + ((uint64_t)t.unit * g.chunks + t.c) * g.a.dv * g.a.dk;
       if (q * 32 < g.dvp)
         for (int cb = 0; cb < nbk; ++cb) {
-          float v[32], lo[32];
+          float v[32];
           const uint32_t acc = tmem + buf * 256u + ((uint32_t)(q * 32) << 16) + (uint32_t)(cb * 32);
-          tc_ld32(acc, v);
-          tc_ld32(acc + (bufs == 2 ? 128u : 256u), lo);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += lo[j];
+          tmem_load_sum32(acc, acc + (bufs == 2 ? 128u : 256u), v);
           store_rows32<WIDE>(tile, lane, v, cb * 32, g.a.dk, [&](int r) -> float* {
             const int row = t.dv0 + q * 32 + r;
             return row < g.a.dv ? out + (uint64_t)row * g.a.dk : nullptr;
@@ -697,12 +719,11 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       for (int j0 = 0; j0 < kC; j0 += 32) {
         float x[32], lo[32];
         if (j0 <= q * 32) {
-          tc_ld32(t_s + lanes + (uint32_t)j0, x);
-          tc_ld32(t_lo + lanes + (uint32_t)j0, lo);
+          tmem_load_sum32(t_s + lanes + (uint32_t)j0, t_lo + lanes + (uint32_t)j0, x);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const int ago = tok - (j0 + j);
-            const float p = ago >= 0 ? (x[j] + lo[j]) * power[ago < 0 ? 0 : ago] : 0.f;
+            const float p = ago >= 0 ? x[j] * power[ago < 0 ? 0 : ago] : 0.f;
             x[j] = tf32_hi(p);
             lo[j] = p - x[j];
           }
@@ -716,11 +737,10 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       const float w = power[tok + 1];
 #pragma unroll 1
       for (int cb = 0; cb < nbv; ++cb) {
-        float x[32], lo[32];
-        tc_ld32(t_inter + lanes + (uint32_t)(cb * 32), x);
-        tc_ld32(t_out + lanes + (uint32_t)(cb * 32), lo);
+        float x[32];
+        tmem_load_sum32(t_inter + lanes + (uint32_t)(cb * 32), t_out + lanes + (uint32_t)(cb * 32), x);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = (x[j] + lo[j]) * w;
+        for (int j = 0; j < 32; ++j) x[j] *= w;
         tmem_store32(t_inter + lanes + (uint32_t)(cb * 32), x);
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -739,11 +759,10 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       const float scale = g.a.has_scale ? g.a.scale : 1.0f;
 #pragma unroll 1
       for (int cb = 0; cb < nbv; ++cb) {
-        float x[32], lo[32];
-        tc_ld32(t_out + lanes + (uint32_t)(cb * 32), x);
-        tc_ld32(t_inter + lanes + (uint32_t)(cb * 32), lo);
+        float x[32];
+        tmem_load_sum32(t_out + lanes + (uint32_t)(cb * 32), t_inter + lanes + (uint32_t)(cb * 32), x);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = real ? __fmul_rn(x[j] + lo[j], scale) : 0.0f;
+        for (int j = 0; j < 32; ++j) x[j] = real ? __fmul_rn(x[j], scale) : 0.0f;
         store_rows32<WIDE>(tile, lane, x, cb * 32, cols, out_row);
       }
       }
