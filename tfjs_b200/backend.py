@@ -29,6 +29,7 @@ first use, tfjs-backend-webgl/src/backend_webgl.ts uploadToGPU).  Set
 TFJS_CUDA_NO_LAZY_FUSION=1 to launch every kernel eagerly.
 """
 import ctypes
+import itertools
 import os
 import time as _time
 from ctypes import byref, c_float, c_int32, c_uint64, c_void_p
@@ -39,6 +40,7 @@ from . import _cabi
 from ._cabi import CudaError
 
 NP_DTYPES = {"float32": np.float32, "int32": np.int32, "bool": np.uint8}
+_ITEMSIZE = {name: np.dtype(t).itemsize for name, t in NP_DTYPES.items()}
 _FOREIGN_TYPES = {"<f4": ("float32", 4), "<i4": ("int32", 4), "|b1": ("bool", 1)}
 HOST_RESIDENT_BYTES = 4096  # keep a host copy of tensors up to this size
 
@@ -46,11 +48,10 @@ HOST_RESIDENT_BYTES = 4096  # keep a host copy of tensors up to this size
 class DataId(object):
     """Opaque key object; identity is the key (a WeakMap key in tfjs)."""
     __slots__ = ("id", "__weakref__")
-    _next = 0
+    _next = itertools.count(1)
 
     def __init__(self):
-        DataId._next += 1
-        self.id = DataId._next
+        self.id = next(DataId._next)
 
     def __repr__(self):
         return "DataId(%d)" % self.id
@@ -62,7 +63,7 @@ class TensorInfo(object):
 
     def __init__(self, dataId, shape, dtype):
         self.dataId = dataId
-        self.shape = [int(s) for s in shape]
+        self.shape = list(map(int, shape))
         self.dtype = dtype
 
     @property
@@ -81,24 +82,25 @@ class GPUData(object):
     `buffer` is the address, `bufSize` its bytes, `tensorRef` a tensor that keeps it alive.
     Libraries that read __cuda_array_interface__ take it without a copy.  When the last
     reference is gone the tensor is disposed, behind the work queued on `stream` by then."""
-    __slots__ = ("backend", "tensorRef", "buffer", "bufSize", "shape", "dtype", "stream")
+    __slots__ = ("backend", "tensorRef", "buffer", "bufSize", "stream")
     _TYPESTR = {"float32": "<f4", "int32": "<i4", "bool": "|b1"}
 
     def __init__(self, backend, tensorRef, buffer, bufSize, stream):
         self.backend, self.tensorRef, self.stream = backend, tensorRef, stream
         self.buffer, self.bufSize = buffer, bufSize
-        self.shape, self.dtype = list(tensorRef.shape), tensorRef.dtype
 
     @property
     def __cuda_array_interface__(self):
-        return {"shape": tuple(self.shape), "typestr": self._TYPESTR[self.dtype],
+        t = self.tensorRef
+        return {"shape": tuple(t.shape), "typestr": self._TYPESTR[t.dtype],
                 "data": (self.buffer, False), "strides": None, "version": 2}
 
     def dispose(self):
         ref, self.tensorRef = self.tensorRef, None
-        if ref is not None and self.backend.ctx:
+        backend = self.backend
+        if ref is not None and backend.ctx:
             if self.stream is not None:
-                self.backend.wait_stream(self.stream)
+                backend.check(backend.lib.tfjs_cuda_wait_stream(backend.ctx, self.stream))
             ref.dispose()
 
     def __del__(self):
@@ -513,6 +515,8 @@ class CudaBackend(object):
             raise CudaError(rc, "tfjs_cuda_create(device %d) failed with status "
                             "%d: no usable sm_100a GPU" % (device_ordinal, rc))
         self.ctx = ctx
+        self._out_id = c_int32()            # where calls leave a new id
+        self._out_id_ref = byref(self._out_id)
         self.device_ordinal = device_ordinal
         self.data = {}        # DataId -> _Record
         self._pinned = []
@@ -537,9 +541,8 @@ class CudaBackend(object):
             raise CudaError(rc, msg.decode() if msg else "status %d" % rc)
 
     def _alloc(self, nbytes):
-        out = c_int32()
-        self.check(self.lib.tfjs_cuda_alloc(self.ctx, int(nbytes), byref(out)))
-        return out.value
+        self.check(self.lib.tfjs_cuda_alloc(self.ctx, nbytes, self._out_id_ref))
+        return self._out_id.value
 
     def floatPrecision(self):
         return 32
@@ -579,7 +582,7 @@ class CudaBackend(object):
     def make_output(self, shape, dtype):
         """Allocate an uninitialised device tensor for a kernel result
         (makeTensorInfo, backend_cpu.ts:83-95)."""
-        nbytes = size_from_shape(shape) * np.dtype(NP_DTYPES[dtype]).itemsize
+        nbytes = size_from_shape(shape) * _ITEMSIZE[dtype]
         dataId = DataId()
         self.data[dataId] = _Record(self._alloc(nbytes), nbytes, dtype, 1, None)
         return TensorInfo(dataId, shape, dtype)
@@ -612,11 +615,11 @@ class CudaBackend(object):
         if shape is not None and size_from_shape(shape) != n:
             raise ValueError("createTensorFromGPUData: %d values for shape %s" % (n, list(shape)))
         if stream is not None:
-            self.wait_stream(stream)
-        dev = c_int32()
-        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes, byref(dev)))
+            self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, stream))
+        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes,
+                                                  self._out_id_ref))
         dataId = DataId()
-        rec = _Record(dev.value, nbytes, found, 1, None)
+        rec = _Record(self._out_id.value, nbytes, found, 1, None)
         rec.foreign, rec.stream = values, stream
         self.data[dataId] = rec
         return TensorInfo(dataId, have if shape is None else shape, found)
@@ -629,7 +632,7 @@ class CudaBackend(object):
         ptr = c_void_p()
         self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
         if stream is not None:
-            self.signal_stream(stream)
+            self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, stream))
         rec = self.data[tensor.dataId]
         rec.host = None        # whoever holds the memory may write to it
         return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream)
@@ -646,6 +649,9 @@ class CudaBackend(object):
     def _adjust(self, rec, dref, dheld):
         """Change a record's reference counts, tracking whether only pending launches
         keep it alive (such records are not reported by numDataIds)."""
+        if rec.held == 0 and dheld == 0:
+            rec.ref += dref
+            return
         was = rec.held > 0 and rec.ref <= rec.held
         rec.ref += dref
         rec.held += dheld
@@ -870,7 +876,7 @@ class CudaBackend(object):
             self._hidden -= 1
         del self.data[dataId]
         if rec.stream is not None:     # its owner's next work waits for what reads it here
-            self.signal_stream(rec.stream)
+            self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream))
         if rec.dev:
             self.check(self.lib.tfjs_cuda_free(self.ctx, rec.dev))
         if rec.pending is not None:

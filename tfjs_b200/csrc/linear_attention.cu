@@ -13,7 +13,8 @@ constexpr int kRowGroups = 32;  // threads that share a column's rows
 // A block holds dim_k x 32 of the state: thread (r, c) rows r, r + 32, ... of four columns.
 // Steps are dependent and end in a sum over the block, so this is the form for single
 // tokens, where reading and writing the state is all there is.
-template <int NR>
+// WIDE: dim_v and the addresses allow 16-byte accesses.
+template <int NR, bool WIDE>
 __global__ void __launch_bounds__(256)
 linear_recurrent_kernel(const LinearArgs a, int tiles) {
   __shared__ __align__(16) float part[8][kTileV];
@@ -26,12 +27,21 @@ linear_recurrent_kernel(const LinearArgs a, int tiles) {
   const uint64_t s0 = (uint64_t)unit * a.dk * a.dv;
   float s[NR][4];
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
+  for (int i = 0; i < NR; ++i) {
+    const int row = i * kRowGroups + r;
+    const float* p = a.state + s0 + (uint64_t)row * a.dv + c0;
+    const bool in = a.state && row < a.dk;
+    if (WIDE) {
+      const float4 v = in && c0 < a.dv ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      s[i][0] = v.x;
+      s[i][1] = v.y;
+      s[i][2] = v.z;
+      s[i][3] = v.w;
+    } else {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int row = i * kRowGroups + r;
-      s[i][x] = a.state && row < a.dk && c0 + x < a.dv ? __ldg(a.state + s0 + (uint64_t)row * a.dv + c0 + x) : 0.f;
+      for (int x = 0; x < 4; ++x) s[i][x] = in && c0 + x < a.dv ? __ldg(p + x) : 0.f;
     }
+  }
   for (int t = 0; t < n; ++t) {
     const uint64_t tok = (uint64_t)unit * a.seq + t;
     float v[4], o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -70,12 +80,18 @@ linear_recurrent_kernel(const LinearArgs a, int tiles) {
     if (tile * kTileV + lane < a.dv)
       a.out[(((uint64_t)b * a.seq + t) * a.heads + h) * a.dv + tile * kTileV + lane] = 0.f;
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
+  for (int i = 0; i < NR; ++i) {
+    const int row = i * kRowGroups + r;
+    float* p = a.out_state + s0 + (uint64_t)row * a.dv + c0;
+    if (row >= a.dk) continue;
+    if (WIDE) {
+      if (c0 < a.dv) *reinterpret_cast<float4*>(p) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+    } else {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int row = i * kRowGroups + r;
-      if (row < a.dk && c0 + x < a.dv) a.out_state[s0 + (uint64_t)row * a.dv + c0 + x] = s[i][x];
+      for (int x = 0; x < 4; ++x)
+        if (c0 + x < a.dv) p[x] = s[i][x];
     }
+  }
 }
 
 }  // namespace
@@ -138,12 +154,11 @@ extern "C" int tfjs_cuda_linear_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_li
   }
   const int tiles = (p->dim_v + kTileV - 1) / kTileV;
   const unsigned grid = (unsigned)(units * tiles);
-  if (p->dim_k <= 64)
-    linear_recurrent_kernel<2><<<grid, 256, 0, ctx->stream>>>(a, tiles);
-  else if (p->dim_k <= 128)
-    linear_recurrent_kernel<4><<<grid, 256, 0, ctx->stream>>>(a, tiles);
-  else
-    linear_recurrent_kernel<8><<<grid, 256, 0, ctx->stream>>>(a, tiles);
+  const bool wide = p->dim_v % 4 == 0 && (((uintptr_t)a.state | (uintptr_t)a.out_state) & 15) == 0;
+  auto kernel = p->dim_k <= 64    ? (wide ? linear_recurrent_kernel<2, true> : linear_recurrent_kernel<2, false>)
+                : p->dim_k <= 128 ? (wide ? linear_recurrent_kernel<4, true> : linear_recurrent_kernel<4, false>)
+                                  : (wide ? linear_recurrent_kernel<8, true> : linear_recurrent_kernel<8, false>);
+  kernel<<<grid, 256, 0, ctx->stream>>>(a, tiles);
   LAUNCH_CHECK(ctx, "linear_recurrent_kernel");
   ctx_mark_written(ctx, out_id);
   ctx_mark_written(ctx, out_state_id);

@@ -5,6 +5,23 @@
 
 namespace {
 
+// One row of head_dim values of both pools, copied by a warp; V values a lane at a time.
+template <int V>
+__device__ __forceinline__ void copy_row(float* k_cache, float* v_cache, uint64_t src, uint64_t dst, int dim, int lane) {
+  for (int d = lane * V; d < dim; d += 32 * V) {
+    if (V == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(k_cache + src + d);
+      const float4 y = *reinterpret_cast<const float4*>(v_cache + src + d);
+      *reinterpret_cast<float4*>(k_cache + dst + d) = x;
+      *reinterpret_cast<float4*>(v_cache + dst + d) = y;
+    } else {
+      const float x = k_cache[src + d], y = v_cache[src + d];
+      k_cache[dst + d] = x;
+      v_cache[dst + d] = y;
+    }
+  }
+}
+
 // ---- append ------------------------------------------------------------------------------
 // k and v are [batch, kv_heads, tokens, head_dim]; the tokens of one row and head are
 // contiguous at the source, and in runs of a page's places at the destination.  V values at a
@@ -47,8 +64,6 @@ paged_append_kernel(const PagedLayout g, const float* __restrict__ k, const floa
 }
 
 // ---- evict -------------------------------------------------------------------------------
-constexpr int kSelThreads = 1024;
-
 struct EvictArgs {
   const float* weights;     // [batch, kv_heads, capacity]
   const int* positions;     // or null
@@ -62,6 +77,8 @@ struct EvictArgs {
   int* tails;               // [units][list]: where from, ascending
   int list;                 // min(budget, capacity)
   int budget, recent;
+  float *k_cache, *v_cache;
+  int move;                 // the rows are moved by the block that chose them
 };
 
 // Weights as unsigned numbers of the same order: NaN above all, -0 equal to +0.
@@ -89,29 +106,31 @@ struct SlotView {
 };
 
 // Exclusive sum over the block of one value a thread, and the block's total.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t* total) {
+template <int NT>
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* warp_sums,
+                                                         unsigned long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t s = v;
+  unsigned long long s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t u = __shfl_up_sync(0xffffffffu, s, o);
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += u;
   }
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
   if (warp == 0) {
-    const uint32_t mine = warp_sums[lane];
-    uint32_t t = mine;
+    const unsigned long long mine = lane < NT / 32 ? warp_sums[lane] : 0;
+    unsigned long long t = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t u = __shfl_up_sync(0xffffffffu, t, o);
+      const unsigned long long u = __shfl_up_sync(0xffffffffu, t, o);
       if (lane >= o) t += u;
     }
-    warp_sums[lane] = t - mine;
+    if (lane < NT / 32) warp_sums[lane] = t - mine;
     if (lane == 31) warp_sums[32] = t;
   }
   __syncthreads();
-  const uint32_t r = warp_sums[warp] + s - v;
+  const unsigned long long r = warp_sums[warp] + s - v;
   *total = warp_sums[32];
   __syncthreads();   // warp_sums is reused by the next call
   return r;
@@ -119,11 +138,16 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
 
 // One block decides for one row and head which slots stay: the m-th largest key by a radix
 // select of 8 bits a pass (counting, no sorting), then one pass in slot order that ranks the
-// slots equal to it, the free places below m and the kept slots from m on.
-__global__ void __launch_bounds__(kSelThreads)
+// slots equal to it, the free places below m and the kept slots from m on: every thread has a
+// stretch of slots, so that each of these takes one sum over the block.  HELD: the keys are formed
+// once and kept in shared memory, which a row of up to 48 k slots allows.  NT: threads; 1024 for long
+// rows, 256 for short ones, of which an SM then holds several.  V: values a lane moves at a time.
+template <bool HELD, int V, int NT>
+__global__ void __launch_bounds__(NT)
 paged_evict_select_kernel(const PagedLayout g, const EvictArgs a) {
+  extern __shared__ uint32_t keys[];
   __shared__ uint32_t hist[256];
-  __shared__ uint32_t warp_sums[33];
+  __shared__ unsigned long long warp_sums[33];
   __shared__ uint32_t pick[2];
   const int unit = blockIdx.x;
   const int b = unit / g.kv_heads;
@@ -141,13 +165,13 @@ paged_evict_select_kernel(const PagedLayout g, const EvictArgs a) {
   int* op = a.out_positions + base;
   int* ok = a.out_kept + (uint64_t)unit * a.budget;
   if (unit == b * g.kv_heads && tid == 0) a.out_lengths[b] = m;
-  for (int j = m + tid; j < g.capacity; j += kSelThreads) {
+  for (int j = m + tid; j < g.capacity; j += NT) {
     ow[j] = 0.0f;
     op[j] = -1;
   }
-  for (int j = m + tid; j < a.budget; j += kSelThreads) ok[j] = -1;
+  for (int j = m + tid; j < a.budget; j += NT) ok[j] = -1;
   if (n <= m) {   // nothing to lose
-    for (int j = tid; j < m; j += kSelThreads) {
+    for (int j = tid; j < m; j += NT) {
       ow[j] = __ldg(s.w + j);
       op[j] = (int)s.position(j);
       ok[j] = j;
@@ -155,14 +179,19 @@ paged_evict_select_kernel(const PagedLayout g, const EvictArgs a) {
     if (tid == 0) a.moves[unit] = 0;
     return;
   }
+  if (HELD) {
+#pragma unroll 4
+    for (int j = tid; j < n; j += NT) keys[j] = s.key(j);   // (read by the same thread or behind a barrier)
+  }
+  auto key_of = [&](int j) { return HELD ? keys[j] : s.key(j); };
   // the key that the m-th largest has, and how many of the slots that have it stay
   uint32_t prefix = 0, mask = 0;
   uint32_t want = (uint32_t)m;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    for (int i = tid; i < 256; i += NT) hist[i] = 0;
     __syncthreads();
-    for (int j = tid; j < n; j += kSelThreads) {
-      const uint32_t key = s.key(j);
+    for (int j = tid; j < n; j += NT) {
+      const uint32_t key = key_of(j);
       if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
     }
     __syncthreads();
@@ -197,38 +226,52 @@ paged_evict_select_kernel(const PagedLayout g, const EvictArgs a) {
     want = pick[1];
     mask |= 255u << shift;
   }
-  // in slot order: slots equal to the threshold stay while `want` lasts
-  uint32_t equal_seen = 0, holes = 0, tails = 0;
+  // in slot order: slots equal to the threshold stay while `want` lasts.  (Stretches of an odd
+  // number of slots, so that the threads of a warp read different banks.)
+  const int stretch = ((n + NT - 1) / NT) | 1;
+  const int j0 = min(tid * stretch, n), j1 = min(j0 + stretch, n);
+  uint32_t equal = 0;
+  for (int j = j0; j < j1; ++j) equal += key_of(j) == prefix;
+  unsigned long long all;
+  const uint32_t equal_before = (uint32_t)block_scan<NT>(equal, warp_sums, &all);
+  auto each = [&](auto hole, auto tail) {
+    uint32_t rank = equal_before;
+    for (int j = j0; j < j1; ++j) {
+      const uint32_t key = key_of(j);
+      const bool keep = key > prefix || (key == prefix && rank++ < want);
+      if (j < m && !keep) hole(j);
+      if (j >= m && keep) tail(j);
+    }
+  };
+  uint32_t my_holes = 0, my_tails = 0;
+  each([&](int) { ++my_holes; }, [&](int) { ++my_tails; });
+  const unsigned long long before = block_scan<NT>((unsigned long long)my_tails << 32 | my_holes, warp_sums, &all);
+  const uint32_t holes = (uint32_t)all;
   int* hole_list = a.holes + (uint64_t)unit * a.list;
   int* tail_list = a.tails + (uint64_t)unit * a.list;
-  for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    const uint32_t key = j < n ? s.key(j) : 0u;
-    const bool equal = j < n && key == prefix;
-    uint32_t all;
-    const uint32_t rank = equal_seen + block_scan(equal, warp_sums, &all);
-    equal_seen += all;
-    const bool keep = j < n && (key > prefix || (equal && rank < want));
-    const bool hole = j < m && !keep, tail = j >= m && keep;
-    const uint32_t r = block_scan((hole ? 1u : 0u) | (tail ? 0x10000u : 0u), warp_sums, &all);
-    if (hole) hole_list[holes + (r & 0xffffu)] = j;
-    if (tail) tail_list[tails + (r >> 16)] = j;
-    if (keep && j < m) {
-      ow[j] = __ldg(s.w + j);
-      op[j] = (int)s.position(j);
-      ok[j] = j;
-    }
-    holes += all & 0xffffu;
-    tails += all >> 16;
+  uint32_t hole_at = (uint32_t)before, tail_at = (uint32_t)(before >> 32);
+  each([&](int j) { hole_list[hole_at++] = j; }, [&](int j) { tail_list[tail_at++] = j; });
+  for (int j = tid; j < m; j += NT) {
+    ow[j] = __ldg(s.w + j);
+    op[j] = (int)s.position(j);
+    ok[j] = j;
   }
-  __syncthreads();   // the lists of this block, written above, are read by other threads below
-  for (uint32_t r = tid; r < holes; r += kSelThreads) {
+  __syncthreads();   // the lists of this block are read, and the free places written again, by other threads
+  for (uint32_t r = tid; r < holes; r += NT) {
     const int to = hole_list[r], from = tail_list[r];
     ow[to] = __ldg(s.w + from);
     op[to] = (int)s.position(from);
     ok[to] = from;
   }
   if (tid == 0) a.moves[unit] = (int)holes;
+  if (a.move) {
+    const int h = unit - b * g.kv_heads;
+    for (uint32_t r = tid >> 5; r < holes; r += NT / 32) {
+      const uint32_t from = paged_row(g, b, h, tail_list[r]), to = paged_row(g, b, h, hole_list[r]);
+      if (from != kNoRow && to != kNoRow)
+        copy_row<V>(a.k_cache, a.v_cache, (uint64_t)from * g.head_dim, (uint64_t)to * g.head_dim, g.head_dim, tid & 31);
+    }
+  }
 }
 
 // The rows of the kept slots: sources are slots from m on, destinations slots below m, so no
@@ -248,19 +291,7 @@ paged_evict_move_kernel(const PagedLayout g, const int* __restrict__ moves,
     const uint32_t from = paged_row(g, b, h, __ldg(tails + (uint64_t)unit * list + r));
     const uint32_t to = paged_row(g, b, h, __ldg(holes + (uint64_t)unit * list + r));
     if (from == kNoRow || to == kNoRow) continue;
-    for (int d = lane * V; d < g.head_dim; d += 32 * V) {
-      const uint64_t src = (uint64_t)from * g.head_dim + d, dst = (uint64_t)to * g.head_dim + d;
-      if (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(k_cache + src);
-        const float4 y = *reinterpret_cast<const float4*>(v_cache + src);
-        *reinterpret_cast<float4*>(k_cache + dst) = x;
-        *reinterpret_cast<float4*>(v_cache + dst) = y;
-      } else {
-        const float x = k_cache[src], y = v_cache[src];
-        k_cache[dst] = x;
-        v_cache[dst] = y;
-      }
-    }
+    copy_row<V>(k_cache, v_cache, (uint64_t)from * g.head_dim, (uint64_t)to * g.head_dim, g.head_dim, lane);
   }
 }
 
@@ -364,14 +395,26 @@ int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params
   a.moves = (int*)mem;
   a.holes = a.moves + units;
   a.tails = a.holes + units * a.list;
-  paged_evict_select_kernel<<<(unsigned)units, kSelThreads, 0, ctx->stream>>>(g, a);
-  LAUNCH_CHECK(ctx, "paged_evict_select_kernel");
-  // at most min(budget, capacity - budget) slots of a row move
+  const bool wide = p->head_dim % 4 == 0 && (((uintptr_t)kp | (uintptr_t)vp) & 15) == 0;
+  // at most min(budget, capacity - budget) slots of a row move; a few the choosing block moves
+  // itself, which saves a launch
   const int most = g.capacity - p->budget < a.list ? g.capacity - p->budget : a.list;
-  if (most > 0) {
+  a.k_cache = kp;
+  a.v_cache = vp;
+  a.move = most <= 64;
+  const uint64_t held = (uint64_t)g.capacity * 4;
+  const bool small = g.capacity <= 4096, keep_keys = held <= 192 * 1024;
+  void (*kernel)(PagedLayout, EvictArgs) =
+      small ? (wide ? paged_evict_select_kernel<true, 4, 256> : paged_evict_select_kernel<true, 1, 256>)
+      : keep_keys ? (wide ? paged_evict_select_kernel<true, 4, 1024> : paged_evict_select_kernel<true, 1, 1024>)
+                  : (wide ? paged_evict_select_kernel<false, 4, 1024> : paged_evict_select_kernel<false, 1, 1024>);
+  if (held > 48 * 1024 && keep_keys)
+    CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)held));
+  kernel<<<(unsigned)units, small ? 256 : 1024, keep_keys ? held : 0, ctx->stream>>>(g, a);
+  LAUNCH_CHECK(ctx, "paged_evict_select_kernel");
+  if (!a.move) {
     uint64_t per = ((uint64_t)most + 31) / 32;
     if (per * units > (uint64_t)ctx->sm_count * 32) per = ((uint64_t)ctx->sm_count * 32 + units - 1) / units;
-    const bool wide = p->head_dim % 4 == 0 && (((uintptr_t)kp | (uintptr_t)vp) & 15) == 0;
     const unsigned grid = (unsigned)(units * per);
     if (wide)
       paged_evict_move_kernel<4><<<grid, 256, 0, ctx->stream>>>(g, a.moves, a.holes, a.tails, a.list, kp, vp, (int)per);

@@ -21,7 +21,7 @@ class KernelConfig(object):
 
 
 def _key(kernel_name, backend_name):
-    return "%s_%s" % (backend_name, kernel_name)
+    return f"{backend_name}_{kernel_name}"
 
 
 def register_kernel(config):

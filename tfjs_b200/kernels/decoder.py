@@ -70,7 +70,7 @@ def _outputs(backend, shapes, call):
     try:
         for shape, dtype in shapes:
             outs.append(backend.make_output(shape, dtype))
-        backend.check(call([dev(backend, o) for o in outs]))
+        backend.check(call([backend.data[o.dataId].dev for o in outs]))
     except Exception:
         for o in outs:
             backend.disposeData(o.dataId)
