@@ -154,3 +154,19 @@ def test_the_references_agree_with_each_other():
     one = np.ones((1, 1, 1, 2), np.float32)
     o, s, _, _ = dc.linear(one, one, one, np.zeros(1, np.float32))
     assert np.array_equal(o.ravel(), [2.0, 2.0]) and np.array_equal(s.ravel(), [1.0] * 4)
+
+
+def test_parameter_structs_match_the_header_and_the_typescript_packers():
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    header = open(os.path.join(root, "include", "tfjs_cuda.h")).read()
+    ts = open(os.path.join(root, "tfjs_b200", "ts", "src", "binding.ts")).read()
+    for cls, name, size in ((_cabi.PagedParams, "tfjs_cuda_paged_params", 48),
+                            (_cabi.LinearAttentionParams, "tfjs_cuda_linear_attention_params", 28)):
+        assert ctypes.sizeof(cls) == size and "new ArrayBuffer(%d)" % size in ts
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, header, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        fields = [f for line in re.findall(r"(?:int32_t|float) ([^;]*);", body) for f in re.split(r",\s*", line)]
+        assert fields == [f for f, _ in cls._fields_]
+        assert "v.setFloat32(%d, scale ?? 1, true)" % cls.scale.offset in ts

@@ -268,6 +268,53 @@ napi_value FusedAttention(napi_env env, napi_callback_info info) {
   if (rc != TFJS_CUDA_OK && rc != TFJS_CUDA_UNSUPPORTED) napi_throw_error(env, nullptr, tfjs_cuda_last_error(a.ctx(0)));
   return r;
 }
+// ctx, params, kCacheId, vCacheId, kId, vId, pageTableId, lengthsId, countsId (0: none), outLengthsId
+napi_value PagedCacheAppend(napi_env env, napi_callback_info info) {
+  Args a(env, info);
+  auto* p = static_cast<tfjs_cuda_paged_params*>(a.buffer(1));
+  return check(env, a.ctx(0), tfjs_cuda_paged_cache_append(a.ctx(0), p, a.i32(2), a.i32(3), a.i32(4), a.i32(5),
+                                                           a.i32(6), a.i32(7), a.i32(8), a.i32(9)));
+}
+// ctx, params, qId, kCacheId, vCacheId, pageTableId, lengthsId, maskId (0: none), weightsId (0: none), outId,
+// outWeightsId
+napi_value PagedAttention(napi_env env, napi_callback_info info) {
+  Args a(env, info);
+  auto* p = static_cast<tfjs_cuda_paged_params*>(a.buffer(1));
+  return check(env, a.ctx(0), tfjs_cuda_paged_attention(a.ctx(0), p, a.i32(2), a.i32(3), a.i32(4), a.i32(5), a.i32(6),
+                                                        a.i32(7), a.i32(8), a.i32(9), a.i32(10)));
+}
+// ctx, params, kCacheId, vCacheId, weightsId, pageTableId, lengthsId, positionsId (0: none), totalId (0: none),
+// outWeightsId, outPositionsId, outLengthsId, outKeptId
+napi_value PagedCacheEvict(napi_env env, napi_callback_info info) {
+  Args a(env, info);
+  auto* p = static_cast<tfjs_cuda_paged_params*>(a.buffer(1));
+  return check(env, a.ctx(0), tfjs_cuda_paged_cache_evict(a.ctx(0), p, a.i32(2), a.i32(3), a.i32(4), a.i32(5), a.i32(6),
+                                                          a.i32(7), a.i32(8), a.i32(9), a.i32(10), a.i32(11), a.i32(12)));
+}
+// ctx, params, qId, kId, vId, logDecayId, stateId (0: none), lengthsId (0: none), outId, outStateId
+napi_value LinearAttention(napi_env env, napi_callback_info info) {
+  Args a(env, info);
+  auto* p = static_cast<tfjs_cuda_linear_attention_params*>(a.buffer(1));
+  return check(env, a.ctx(0), tfjs_cuda_linear_attention(a.ctx(0), p, a.i32(2), a.i32(3), a.i32(4), a.i32(5), a.i32(6),
+                                                         a.i32(7), a.i32(8), a.i32(9)));
+}
+// Addresses and streams travel as BigInt.
+napi_value FromDevice(napi_env env, napi_callback_info info) {
+  Args a(env, info); int32_t id = 0; uint64_t ptr = 0; bool lossless = true;
+  napi_get_value_bigint_uint64(env, a.v[1], &ptr, &lossless);
+  check(env, a.ctx(0), tfjs_cuda_from_device(a.ctx(0), reinterpret_cast<void*>(ptr), a.u64(2), &id));
+  return num(env, id);
+}
+napi_value WaitStream(napi_env env, napi_callback_info info) {
+  Args a(env, info); uint64_t s = 0; bool lossless = true;
+  napi_get_value_bigint_uint64(env, a.v[1], &s, &lossless);
+  return check(env, a.ctx(0), tfjs_cuda_wait_stream(a.ctx(0), reinterpret_cast<void*>(s)));
+}
+napi_value SignalStream(napi_env env, napi_callback_info info) {
+  Args a(env, info); uint64_t s = 0; bool lossless = true;
+  napi_get_value_bigint_uint64(env, a.v[1], &s, &lossless);
+  return check(env, a.ctx(0), tfjs_cuda_signal_stream(a.ctx(0), reinterpret_cast<void*>(s)));
+}
 napi_value LayerNorm(napi_env env, napi_callback_info info) {
   Args a(env, info);  // ctx, xId, residualId (0: none), gammaId, betaId, rows, cols, epsilon, outId
   return check(env, a.ctx(0), tfjs_cuda_layer_norm(a.ctx(0), a.i32(1), a.i32(2), a.i32(3), a.i32(4), a.u64(5),
@@ -431,6 +478,9 @@ napi_value Init(napi_env env, napi_value exports) {
       {"addActivation", AddActivation},
       {"fusedDepthwiseConv2d", FusedDepthwiseConv2D}, {"fusedMatMul", FusedMatMul}, {"fusedMatMulHeads", FusedMatMulHeads}, {"fusedMatMulGroup", FusedMatMulGroup},
       {"pool2d", Pool2D}, {"binary", Binary}, {"unary", Unary}, {"softmax", Softmax}, {"layerNorm", LayerNorm}, {"softmaxScaledMasked", SoftmaxScaledMasked}, {"fusedAttention", FusedAttention},
+      {"pagedCacheAppend", PagedCacheAppend}, {"pagedAttention", PagedAttention},
+      {"pagedCacheEvict", PagedCacheEvict}, {"linearAttention", LinearAttention},
+      {"fromDevice", FromDevice}, {"waitStream", WaitStream}, {"signalStream", SignalStream},
       {"reduce", Reduce}, {"argMax", ArgMax}, {"transpose", Transpose}, {"gather", Gather},
       {"cast", Cast}, {"copyStrided", CopyStrided}, {"fill", Fill}, {"batchNorm", BatchNorm},
       {"dequantize", Dequantize}, {"dequantizeStatic", DequantizeStatic},

@@ -19,6 +19,14 @@ interface Record {
   host?: TypedArray;   // kept for small host-written tensors
   pending?: Pending;   // a deferred launch produces this tensor (pending.ts)
   held: number;        // how many of refCount belong to pending launches that read it
+  foreign?: ForeignData;  // the owner of device memory that is not the backend's
+}
+
+/** Device memory of another library (a WebGPUData-like value: an address instead of a GPUBuffer), and
+ * the cudaStream_t its owner works on, if the two are to be ordered. */
+export interface ForeignData {
+  buffer: bigint;
+  stream?: bigint;
 }
 
 const HOST_RESIDENT_BYTES = 4096;
@@ -103,6 +111,7 @@ export class CudaBackend extends KernelBackend {
     const dataId = {};
     for (const d of pending.deps()) this.adjust(this.data.get(d), 1, 1);
     this.data.set(dataId, {id: 0, nbytes, dtype, refCount: 1, pending, held: 0});
+    this.pendingIds.add(dataId);
     if (pending instanceof PendingMatMul) this.noteMatMul(dataId, pending);
     return {dataId, shape, dtype};
   }
@@ -221,6 +230,52 @@ export class CudaBackend extends KernelBackend {
   /** Device buffer id of a tensor (0 for an absent optional input). */
   deviceId(t?: TensorInfo): number { return t == null ? 0 : this.deviceIdOf(t.dataId); }
 
+  /** Launches what is pending on a tensor's present contents. */
+  private launchReaders(dataId: object, r: Record): void {
+    if (r.held === 0) return;
+    for (const other of this.pendingRecords()) {
+      if (other.pending != null && other.pending.deps().includes(dataId)) this.resolve(other);
+    }
+  }
+  private pendingIds = new Set<object>();
+  private pendingRecords(): Record[] {
+    for (const d of this.pendingIds) {
+      if (!this.data.has(d) || this.data.get(d).pending == null) this.pendingIds.delete(d);
+    }
+    return [...this.pendingIds].map(d => this.data.get(d) as Record);
+  }
+
+  /** Device buffer id of a tensor that a kernel is about to write in place: launches that are
+   * pending on its present contents happen first, and a host copy is dropped. */
+  deviceIdForUpdate(t: TensorInfo): number {
+    const r = this.data.get(t.dataId);
+    this.launchReaders(t.dataId, r);
+    const id = this.deviceIdOf(t.dataId);
+    r.host = undefined;
+    return id;
+  }
+
+  // -------------------------------------------------------- other libraries' memory --
+  /** A tensor over another library's device memory, without a copy (tf.tensor({buffer, zeroCopy: true})).
+   * With a stream, this backend's work waits for what is queued there now, and what is queued there after
+   * the tensor is disposed waits for this backend's work. */
+  fromForeign(values: ForeignData, shape: number[], dtype: DataType): TensorInfo {
+    const nbytes = util.sizeFromShape(shape) * bytesPerElement(dtype);
+    if (values.stream != null) binding.waitStream(this.ctx, values.stream);
+    const id = binding.fromDevice(this.ctx, values.buffer, nbytes);
+    const dataId = {};
+    this.data.set(dataId, {id, nbytes, dtype, refCount: 1, held: 0, foreign: values});
+    return {dataId, shape, dtype};
+  }
+
+  /** The device address of a tensor (tensor.dataToGPU()); whoever holds it may write to it. */
+  toForeign(t: TensorInfo, stream?: bigint): ForeignData {
+    const buffer = binding.devicePtr(this.ctx, this.deviceId(t));
+    if (stream != null) binding.signalStream(this.ctx, stream);
+    this.data.get(t.dataId).host = undefined;
+    return {buffer, stream};
+  }
+
   hostValues(t: TensorInfo): TypedArray|undefined { return this.data.get(t.dataId).host; }
 
   // ------------------------------------------------------------------------ data --
@@ -249,6 +304,8 @@ export class CudaBackend extends KernelBackend {
   override disposeData(dataId: object, force = false): boolean {
     if (!this.data.has(dataId)) return false;
     const r = this.data.get(dataId);
+    // its owner may reuse the memory from here on: pending readers launch now
+    if (r.foreign != null && r.refCount - r.held === 1) this.launchReaders(dataId, r);
     this.adjust(r, -1, 0);
     if (r.refCount > 0 && (!force || r.held > 0)) return false;
     this.drop(dataId, r);
@@ -258,6 +315,8 @@ export class CudaBackend extends KernelBackend {
   private drop(dataId: object, r: Record): void {
     if (r.held > 0 && r.refCount <= r.held) this.hidden--;
     this.data.delete(dataId);
+    this.pendingIds.delete(dataId);
+    if (r.foreign?.stream != null) binding.signalStream(this.ctx, r.foreign.stream);
     if (r.id !== 0) binding.free(this.ctx, r.id);
     if (r.pending != null) {
       const p = r.pending;

@@ -64,6 +64,21 @@ export interface CudaBinding {
   fusedAttention(ctx: Ctx, q: number, k: number, v: number, mask: number, hasScale: number,
                  scale: number, batch: number, heads: number, seq: number, headDim: number,
                  unitsPerMask: number, out: number): boolean;
+  /** The paged key-value cache (params: packPagedParams; ids of absent tensors are 0). */
+  pagedCacheAppend(ctx: Ctx, params: ArrayBuffer, kCache: number, vCache: number, k: number, v: number,
+                   pageTable: number, lengths: number, counts: number, outLengths: number): void;
+  pagedAttention(ctx: Ctx, params: ArrayBuffer, q: number, kCache: number, vCache: number,
+                 pageTable: number, lengths: number, mask: number, weights: number, out: number,
+                 outWeights: number): void;
+  pagedCacheEvict(ctx: Ctx, params: ArrayBuffer, kCache: number, vCache: number, weights: number,
+                  pageTable: number, lengths: number, positions: number, total: number,
+                  outWeights: number, outPositions: number, outLengths: number, outKept: number): void;
+  linearAttention(ctx: Ctx, params: ArrayBuffer, q: number, k: number, v: number, logDecay: number,
+                  state: number, lengths: number, out: number, outState: number): void;
+  /** A tensor over device memory of the caller's; order against a cudaStream_t of the caller's. */
+  fromDevice(ctx: Ctx, address: bigint, nbytes: number): number;
+  waitStream(ctx: Ctx, stream: bigint): void;
+  signalStream(ctx: Ctx, stream: bigint): void;
   layerNorm(ctx: Ctx, x: number, residual: number, gamma: number, beta: number, rows: number,
             cols: number, epsilon: number, out: number): void;
   reduce(ctx: Ctx, op: number, x: number, outer: number, reduce: number, inner: number,
@@ -208,6 +223,31 @@ export function packMatMulParams(
     v.setFloat32(56, gelu[2], true);
     v.setInt32(60, gelu[3] ? 1 : 0, true);
   }
+  return buf;
+}
+
+/** tfjs_cuda_paged_params: 11 int32 fields and a float. */
+export function packPagedParams(p: {
+  batch: number, heads?: number, kvHeads: number, headDim: number, numPages: number,
+  pageSize: number, maxPages: number, tokens?: number, budget?: number, recent?: number
+}, scale?: number|null): ArrayBuffer {
+  const buf = new ArrayBuffer(48);
+  const v = new DataView(buf);
+  [p.batch, p.heads ?? 0, p.kvHeads, p.headDim, p.numPages, p.pageSize, p.maxPages, p.tokens ?? 0,
+   p.budget ?? 0, p.recent ?? 0, scale != null ? 1 : 0]
+      .forEach((x, i) => v.setInt32(4 * i, x, true));
+  v.setFloat32(44, scale ?? 1, true);
+  return buf;
+}
+
+/** tfjs_cuda_linear_attention_params: 6 int32 fields and a float. */
+export function packLinearAttentionParams(
+    batch: number, heads: number, seq: number, dimK: number, dimV: number,
+    scale?: number|null): ArrayBuffer {
+  const buf = new ArrayBuffer(28);
+  const v = new DataView(buf);
+  [batch, heads, seq, dimK, dimV, scale != null ? 1 : 0].forEach((x, i) => v.setInt32(4 * i, x, true));
+  v.setFloat32(24, scale ?? 1, true);
   return buf;
 }
 
