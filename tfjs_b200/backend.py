@@ -30,6 +30,7 @@ TFJS_CUDA_NO_LAZY_FUSION=1 to launch every kernel eagerly.
 """
 import ctypes
 import itertools
+import math
 import os
 import time as _time
 from ctypes import byref, c_float, c_int32, c_uint64, c_void_p
@@ -498,10 +499,7 @@ class PendingRead(object):
 
 
 def size_from_shape(shape):
-    n = 1
-    for s in shape:
-        n *= int(s)
-    return n
+    return math.prod(map(int, shape))
 
 
 class CudaBackend(object):
@@ -628,12 +626,12 @@ class CudaBackend(object):
         """GPUData over `tensor`'s device memory (the KernelBackend method behind
         tensor.dataToGPU()), without a copy; launches a pending producer first.  With `stream`,
         what is queued there from now on runs after this backend's work."""
-        dev = self.device_id(tensor.dataId)
+        rec = self.data[tensor.dataId]
         ptr = c_void_p()
-        self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
+        self.check(self.lib.tfjs_cuda_device_ptr(
+            self.ctx, rec.dev or self.device_id(tensor.dataId), byref(ptr)))
         if stream is not None:
             self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, stream))
-        rec = self.data[tensor.dataId]
         rec.host = None        # whoever holds the memory may write to it
         return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream)
 
@@ -865,7 +863,10 @@ class CudaBackend(object):
         if rec.foreign is not None and rec.ref - rec.held == 1:
             # its owner may reuse the memory from here on: pending readers launch now
             self._launch_readers(dataId, rec)
-        self._adjust(rec, -1, 0)
+        if rec.held == 0:
+            rec.ref -= 1
+        else:
+            self._adjust(rec, -1, 0)
         if rec.ref > 0 and (not force or rec.held > 0):
             return False
         self._drop(dataId, rec)

@@ -59,9 +59,11 @@ class Tensor(object):
         result keeps the memory alive on its own; this handle may be disposed.  `stream`:
         what is queued on that stream from now on runs after the kernels launched so far."""
         self._check()
-        backend = self._engine.backend
+        engine = self._engine
+        backend = engine.backend
         backend.incRef(self.dataId)
-        ref = self._engine.make_tensor_from_info(self.info())
+        engine.num_tensors += 1
+        ref = Tensor(engine, self.info())
         try:
             return backend.readToGPU(ref, stream)
         except Exception:
@@ -149,8 +151,9 @@ class Engine(object):
             self.ready()
         interface = getattr(values, "__cuda_array_interface__", None)
         if interface is not None:
-            return self.make_tensor_from_info(
-                self.backend.createTensorFromGPUData(values, shape, dtype, stream, interface))
+            info = self.backend.createTensorFromGPUData(values, shape, dtype, stream, interface)
+            self.num_tensors += 1
+            return Tensor(self, info)
         arr = np.asarray(values)
         if dtype is None:
             if arr.dtype == np.bool_:
@@ -213,7 +216,8 @@ class Engine(object):
             # record in which it was launched
             rec["deferred"] = any(self.backend.pending_of(t.dataId) is not None for t in o)
             prof.append(rec)
-        outs = out if isinstance(out, (list, tuple)) else [out]
+        many = isinstance(out, (list, tuple))
+        outs = out if many else [out]
         if self.is_test:
             # engine.ts:557-588: a kernel may only add one data id per output
             # whose data id is new.
@@ -223,9 +227,8 @@ class Engine(object):
             if leaked > 0:
                 raise RuntimeError("Backend '%s' has an internal memory leak (%d data ids) "
                                    "after running '%s'" % (self.backend_name, leaked, kernel_name))
-        tensors = [self.make_tensor_from_info(o) for o in outs]
-        return tensors if isinstance(out, (list, tuple)) else tensors[0]
-
+        self.num_tensors += len(outs)
+        return [Tensor(self, o) for o in outs] if many else Tensor(self, out)
 
     def _take_slots(self):
         slot = self._prof_next_slot

@@ -10,7 +10,10 @@ BACKEND = "cuda"
 
 def dev(backend, info):
     """Device buffer id of a TensorInfo (0 when the optional input is absent)."""
-    return backend.device_id(info.dataId) if info is not None else 0
+    if info is None:
+        return 0
+    # (0 until it is uploaded or its pending producer has been launched)
+    return backend.data[info.dataId].dev or backend.device_id(info.dataId)
 
 
 def per_channel_len(info, channels):

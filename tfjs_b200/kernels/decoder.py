@@ -7,8 +7,6 @@ value, as everywhere else.
 """
 from ctypes import byref
 
-import numpy as np
-
 from .. import _cabi
 from ..kernel_registry import KernelConfig
 from .common import BACKEND, dev
@@ -45,10 +43,10 @@ def _paged(name, inp):
     _want(name, "lengths", lengths, [None], "int32")
     batch = lengths.shape[0]
     _want(name, "pageTable", table, [batch, None], "int32")
-    p = _cabi.PagedParams()
-    p.batch, p.max_pages = batch, table.shape[1]
-    p.num_pages, p.kv_heads, p.page_size, p.head_dim = kc.shape
-    return p, p.max_pages * p.page_size
+    num_pages, kv_heads, page_size, head_dim = kc.shape
+    max_pages = table.shape[1]
+    return _cabi.PagedParams(batch, 0, kv_heads, head_dim, num_pages, page_size, max_pages), \
+        max_pages * page_size
 
 
 def _not_a_pool(name, inp, names):
@@ -59,8 +57,8 @@ def _not_a_pool(name, inp, names):
 
 
 def _scale(p, scale):
-    p.has_scale = int(scale is not None)
-    p.scale = float(np.float32(scale if scale is not None else 1.0))
+    if scale is not None:
+        p.has_scale, p.scale = 1, scale      # (a c_float: rounded to float32 on the way)
 
 
 def _outputs(backend, shapes, call):
@@ -152,20 +150,20 @@ def _linear_attention(args):
     q, k, v, decay = inp["q"], inp["k"], inp["v"], inp["logDecay"]
     state, lengths = inp.get("state"), inp.get("lengths")
     _want(name, "q", q, [None] * 4, "float32")
-    p = _cabi.LinearAttentionParams()
-    p.batch, p.heads, p.seq, p.dim_k = q.shape
+    batch, heads, seq, dim_k = q.shape
     _want(name, "k", k, q.shape, "float32")
-    _want(name, "v", v, [p.batch, p.heads, p.seq, None], "float32")
-    p.dim_v = v.shape[3]
-    _want(name, "logDecay", decay, [p.heads], "float32")
-    states = [p.batch, p.heads, p.dim_k, p.dim_v]
+    _want(name, "v", v, [batch, heads, seq, None], "float32")
+    dim_v = v.shape[3]
+    _want(name, "logDecay", decay, [heads], "float32")
+    states = [batch, heads, dim_k, dim_v]
     if state is not None:
         _want(name, "state", state, states, "float32")
     if lengths is not None:
-        _want(name, "lengths", lengths, [p.batch], "int32")
+        _want(name, "lengths", lengths, [batch], "int32")
+    p = _cabi.LinearAttentionParams(batch, heads, seq, dim_k, dim_v)
     _scale(p, args["attrs"].get("scale"))
     reads = [dev(backend, t) for t in (q, k, v, decay, state, lengths)]
-    return _outputs(backend, [([p.batch, p.seq, p.heads, p.dim_v], "float32"), (states, "float32")],
+    return _outputs(backend, [([batch, seq, heads, dim_v], "float32"), (states, "float32")],
                     lambda out: backend.lib.tfjs_cuda_linear_attention(
                         backend.ctx, byref(p), *reads, *out))
 
