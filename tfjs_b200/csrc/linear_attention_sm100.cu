@@ -26,9 +26,8 @@
 namespace {
 
 constexpr int kC = 128;            // tokens of a chunk = rows of an MMA
-constexpr int kProducers = 8;      // warps 0-7: load, split, store operands; 8-11: one per quarter of
-                                   // the tensor-memory lanes
-constexpr int kThreads = (kProducers + 4) * 32;
+constexpr int kProducers = 8;      // warps 0-7: load, split, store operands; those from 8 on read tensor
+                                   // memory, each in the quarter of its lanes that it may access
 constexpr int kMaxStages = 4;
 constexpr int kSmemCap = 232448;
 
@@ -59,8 +58,8 @@ __device__ __forceinline__ Item item_of(const ChunkArgs& g, int i) {
   return t;
 }
 
-// Four values of a row of `dim` from column d on (p points there), zeros outside and where !in.
-// Volatile, so that a stage's loads are issued together and early: left to itself the compiler
+// Four values, zeros where !in; load_cols4: of a row of `dim` that is not on 16 bytes, from column d
+// on (p points there).  Volatile, so that a stage's loads are issued together and early: left to itself the compiler
 // moves each one down to its use.  Predicated, since a branch a load costs as much as the rest.
 __device__ __forceinline__ float4 load16(const float* p, bool in) {
   float4 r;
@@ -78,11 +77,14 @@ __device__ __forceinline__ float load1(const float* p, bool in) {
       : "=f"(r) : "l"(p), "r"((int)in));
   return r;
 }
-template <bool WIDE>
-__device__ __forceinline__ float4 load_cols(const float* p, int d, int dim, bool in) {
-  if (WIDE) return load16(p, in && d < dim);
+__device__ __forceinline__ float4 load_cols4(const float* p, int d, int dim, bool in) {
   return make_float4(load1(p, in && d < dim), load1(p + 1, in && d + 1 < dim), load1(p + 2, in && d + 2 < dim),
                      load1(p + 3, in && d + 3 < dim));
+}
+// Bits 0 .. of the places 0, 32, 64, ... (at most `most` of them) that lie below n.
+__device__ __forceinline__ uint32_t places(int n, int most) {
+  const int c = n <= 0 ? 0 : (n + 31) >> 5;
+  return (1u << (c < most ? c : most)) - 1u;
 }
 
 // x rounded to TF32's 11 bits, to nearest
@@ -192,9 +194,11 @@ constexpr uint32_t kAMN = 1u << 15, kBMN = 1u << 16;
 __device__ __forceinline__ uint32_t n_field(int n) { return (uint32_t)(n >> 3) << 17; }
 
 // ---- A^T of every chunk: M = dim_v tile, N = dim_k, K = tokens ------------------------------
+constexpr int kStateThreads = (kProducers + 4 + 1) * 32;
+
 // Warp 12's first thread issues the MMAs.  NK: at most that many blocks of 32 columns of K.
 template <bool WIDE, int NK>
-__global__ void __launch_bounds__(kThreads + 32, 1)
+__global__ void __launch_bounds__(kStateThreads, 1)
 linear_chunk_states_kernel(const ChunkArgs g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -263,12 +267,19 @@ linear_chunk_states_kernel(const ChunkArgs g) {
       const uint64_t row = (uint64_t)s.t.unit * g.a.seq + (uint64_t)s.t.c * kC + (in ? j : 0);
       const float* pv = g.a.v + row * g.a.dv + s.t.dv0 + c4 * 4;
       const float* pk = g.a.k + row * g.a.dk + c4 * 4;
+      if (WIDE) {
+        const uint32_t mv = in ? places(g.a.dv - s.t.dv0 - c4 * 4, 4) : 0u, mk = in ? places(g.a.dk - c4 * 4, NK) : 0u;
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
-        x[y] = load_cols<WIDE>(pv + y * 32, s.t.dv0 + y * 32 + c4 * 4, g.a.dv, in && y < nbv);
+        for (int y = 0; y < 4; ++y) x[y] = load16(pv + y * 32, mv >> y & 1u);
 #pragma unroll
-      for (int y = 0; y < NK; ++y)
-        x[4 + y] = load_cols<WIDE>(pk + y * 32, y * 32 + c4 * 4, g.a.dk, in && y < nbk);
+        for (int y = 0; y < NK; ++y) x[4 + y] = load16(pk + y * 32, mk >> y & 1u);
+      } else {
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          x[y] = load_cols4(pv + y * 32, s.t.dv0 + y * 32 + c4 * 4, g.a.dv, in && y < nbv);
+#pragma unroll
+        for (int y = 0; y < NK; ++y) x[4 + y] = load_cols4(pk + y * 32, y * 32 + c4 * 4, g.a.dk, in && y < nbk);
+      }
     };
     uint32_t slot = 0, phase = 1;
     auto store = [&](const Stage& s, float4 (&x)[S]) -> bool {
@@ -447,13 +458,16 @@ linear_chunk_scan_kernel(const ChunkArgs g, int blocks_per_unit) {
 // Tensor memory, in columns (hi hi sums left, sums of the small products right):
 //   [0, 128) scores, later the probabilities' hi parts     [256, 384) scores, later their lo parts
 //   [128, 256) Q S, later decayed                          [384, 512) Q S, later P V
+// Eight producer warps, eight that read tensor memory.
+constexpr int kOutThreads = 512;
+
 template <bool WIDE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kOutThreads, 1)
 linear_chunk_outputs_kernel(const ChunkArgs g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t tiles = base + (uint32_t)(g.stages * g.stage_bytes);
-  const uint32_t bars = tiles + 4 * 4096u;
+  const uint32_t bars = tiles + 8 * 4096u;
   auto full = [&](int s) { return bars + 8u * (uint32_t)s; };
   auto empty = [&](int s) { return bars + 8u * (uint32_t)(kMaxStages + s); };
   const uint32_t s_full = bars + 8u * (2 * kMaxStages), o_full = s_full + 8u;
@@ -515,26 +529,42 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       const uint64_t row0 = (uint64_t)s.t.unit * g.a.seq + (uint64_t)s.t.c * kC;
       const bool is_v = s.ks >= nk;
       const int d = s.ks * 32 + c4 * 4;
-      const uint64_t at = (row0 + r0) * g.a.dk + d;
-      const float *pq = g.a.q + at, *pk = g.a.k + at;
-      const float* ps = g.states + (((uint64_t)s.t.unit * g.chunks + s.t.c) * g.a.dv + s.t.dv0 + r0) * g.a.dk + d;
-      const uint32_t by = 32u * (uint32_t)g.a.dk;
       const int j0 = (s.ks - nk) * 64 + r0;                // V: this thread's tokens are j0 and j0 + 32
-      const float* pv = g.a.v + (row0 + j0) * g.a.dv + s.t.dv0 + c4 * 4;
-      const uint32_t by_v = 32u * (uint32_t)g.a.dv;
-#pragma unroll
-      for (int y = 0; y < 12; ++y) {
-        const int tg = y >> 2, cb = y & 3;                 // V: places 0 to 7
-        const float* p = y < 4 ? pq + y * by : y < 8 ? pk + (y - 4) * by : ps + (y - 8) * by;
-        bool in = y < 8 ? cb * 32 + r0 < s.t.n : cb < nbv && s.t.dv0 + cb * 32 + r0 < g.a.dv;
-        int col = d, dim = g.a.dk;
+      const uint64_t at = (row0 + r0) * g.a.dk + d;
+      const float* p0 = g.a.q + at;
+      const float* p1 = g.a.k + at;
+      const float* p2 = g.states + (((uint64_t)s.t.unit * g.chunks + s.t.c) * g.a.dv + s.t.dv0 + r0) * g.a.dk + d;
+      uint32_t by = 32u * (uint32_t)g.a.dk;
+      if (is_v) {
+        p0 = g.a.v + (row0 + j0) * g.a.dv + s.t.dv0 + c4 * 4;
+        p1 = p0 + 32u * (uint32_t)g.a.dv;
+        by = 32u;
+      }
+      if (WIDE) {
+        uint32_t m0 = 0u, m1 = 0u, m2 = 0u;
         if (is_v) {
-          p = pv + (tg == 1 ? by_v : 0u) + cb * 32;
-          in = y < 8 && cb < nbv && j0 + tg * 32 < s.t.n;
-          col = s.t.dv0 + cb * 32 + c4 * 4;
-          dim = g.a.dv;
+          const uint32_t cols = places(g.a.dv - s.t.dv0 - c4 * 4, 4);
+          m0 = j0 < s.t.n ? cols : 0u;
+          m1 = j0 + 32 < s.t.n ? cols : 0u;
+        } else if (d < g.a.dk) {
+          m0 = m1 = places(s.t.n - r0, 4);
+          m2 = places(g.a.dv - s.t.dv0 - r0, 4);
         }
-        x[y] = load_cols<WIDE>(p, col, dim, in);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          x[y] = load16(p0 + y * by, m0 >> y & 1u);
+          x[4 + y] = load16(p1 + y * by, m1 >> y & 1u);
+          x[8 + y] = load16(p2 + y * by, m2 >> y & 1u);
+        }
+      } else {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int col = is_v ? s.t.dv0 + y * 32 + c4 * 4 : d, dim = is_v ? g.a.dv : g.a.dk;
+          const bool row_in = y * 32 + r0 < s.t.n;
+          x[y] = load_cols4(p0 + y * by, col, dim, is_v ? y < nbv && j0 < s.t.n : row_in);
+          x[4 + y] = load_cols4(p1 + y * by, col, dim, is_v ? y < nbv && j0 + 32 < s.t.n : row_in);
+          x[8 + y] = load_cols4(p2 + y * by, col, dim, !is_v && y < nbv && s.t.dv0 + y * 32 + r0 < g.a.dv);
+        }
       }
     };
     uint32_t slot = 0, phase = 1;
@@ -587,7 +617,7 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       if (!store(b, xb)) break;
     }
   } else {
-    // The first of these warps also issues the MMAs, of which its first thread: the four have nothing
+    // The first of these warps also issues the MMAs, of which its first thread: they have nothing
     // else to do while the scores are formed.
     const bool issuer = warp == kProducers;
     const uint32_t idesc_s = kIdesc | n_field(128 + g.dvp);
@@ -677,10 +707,10 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       __syncwarp();
       return true;
     };
-    auto four_warps = []() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-    const int q = warp & 3;
+    auto all_warps = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    const int q = warp & 3, half = (warp - kProducers) >> 2;   // two warps a quarter: every second block
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    const uint32_t tile = tiles + (uint32_t)q * 4096u;
+    const uint32_t tile = tiles + (uint32_t)(warp - kProducers) * 4096u;
     const int tok = q * 32 + lane;                         // this thread's row
     uint32_t done = 0;
     int powers_of = -1;
@@ -697,14 +727,15 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
         float z[32];
 #pragma unroll
         for (int x = 0; x < 32; ++x) z[x] = 0.f;
-        for (int cb = 0; cb < nbv; ++cb) store_rows32<WIDE>(tile, lane, z, cb * 32, cols, out_row);
+        for (int cb = half; cb < nbv; cb += 2) store_rows32<WIDE>(tile, lane, z, cb * 32, cols, out_row);
         continue;
       }
-      if (t.h != powers_of) {                              // (the same for all four warps)
-        four_warps();
+      if (t.h != powers_of) {                              // (the same for all eight warps)
+        all_warps();
         const float ld = __ldg(g.a.log_decay + t.h);
-        for (int e = (int)threadIdx.x - kProducers * 32; e <= kC; e += 128) power[e] = decay_power(ld, e);
-        four_warps();
+        const int e = (int)threadIdx.x - kProducers * 32;
+        if (e <= kC) power[e] = decay_power(ld, e);
+        all_warps();
         powers_of = t.h;
       }
       // (a warp that gave up takes part in the barriers alone)
@@ -716,7 +747,7 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       tc_fence_after();
       if (alive) {
 #pragma unroll 1
-      for (int j0 = 0; j0 < kC; j0 += 32) {
+      for (int j0 = half * 32; j0 < kC; j0 += 64) {
         float x[32], lo[32];
         if (j0 <= q * 32) {
           tmem_load_sum32(t_s + lanes + (uint32_t)j0, t_lo + lanes + (uint32_t)j0, x);
@@ -736,7 +767,7 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       }
       const float w = power[tok + 1];
 #pragma unroll 1
-      for (int cb = 0; cb < nbv; ++cb) {
+      for (int cb = half; cb < nbv; cb += 2) {
         float x[32];
         tmem_load_sum32(t_inter + lanes + (uint32_t)(cb * 32), t_out + lanes + (uint32_t)(cb * 32), x);
 #pragma unroll
@@ -746,7 +777,7 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       }
       tc_fence_before();
-      four_warps();                                        // the probabilities of all rows are there
+      all_warps();                                        // the probabilities of all rows are there
       tc_fence_after();
       if (issuer && alive) alive = issue_values(t.n);
       if (alive && !warp_wait(o_full, done & 1)) {
@@ -758,7 +789,7 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       const bool real = tok < t.n;
       const float scale = g.a.has_scale ? g.a.scale : 1.0f;
 #pragma unroll 1
-      for (int cb = 0; cb < nbv; ++cb) {
+      for (int cb = half; cb < nbv; cb += 2) {
         float x[32];
         tmem_load_sum32(t_out + lanes + (uint32_t)(cb * 32), t_inter + lanes + (uint32_t)(cb * 32), x);
 #pragma unroll
@@ -767,7 +798,7 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
       }
       }
       tc_fence_before();
-      four_warps();                                        // all sums are read: the next products may come
+      all_warps();                                        // all sums are read: the next products may come
       tc_fence_after();
       ++done;
     }
@@ -792,10 +823,10 @@ int launch_chunks(tfjs_cuda_ctx* ctx, ChunkArgs& g) {
   const unsigned grid = (unsigned)(g.items < ctx->sm_count ? g.items : ctx->sm_count);
   if (g.dkp <= 128) {
     CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
-    linear_chunk_states_kernel<WIDE, 4><<<grid, kThreads + 32, s_smem, ctx->stream>>>(s);
+    linear_chunk_states_kernel<WIDE, 4><<<grid, kStateThreads, s_smem, ctx->stream>>>(s);
   } else {
     CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
-    linear_chunk_states_kernel<WIDE, 8><<<grid, kThreads + 32, s_smem, ctx->stream>>>(s);
+    linear_chunk_states_kernel<WIDE, 8><<<grid, kStateThreads, s_smem, ctx->stream>>>(s);
   }
   LAUNCH_CHECK(ctx, "linear_chunk_states_kernel");
   const unsigned units = (unsigned)(g.a.batch * g.a.heads);
@@ -807,12 +838,12 @@ int launch_chunks(tfjs_cuda_ctx* ctx, ChunkArgs& g) {
   LAUNCH_CHECK(ctx, "linear_chunk_scan_kernel");
   const int qk = 32768 + 2 * (128 + g.dvp) * 128, v = 2 * 64 * g.dvp * 4;
   g.stage_bytes = qk > v ? qk : v;
-  const int o_fixed = 1024 + 4 * 4096 + 256 + (kC + 1) * 4;
+  const int o_fixed = 1024 + 8 * 4096 + 256 + (kC + 1) * 4;
   g.stages = (kSmemCap - o_fixed) / g.stage_bytes;
   if (g.stages > kMaxStages) g.stages = kMaxStages;
   const int o_smem = o_fixed + g.stages * g.stage_bytes;
   CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_outputs_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, o_smem));
-  linear_chunk_outputs_kernel<WIDE><<<grid, kThreads, o_smem, ctx->stream>>>(g);
+  linear_chunk_outputs_kernel<WIDE><<<grid, kOutThreads, o_smem, ctx->stream>>>(g);
   LAUNCH_CHECK(ctx, "linear_chunk_outputs_kernel");
   return TFJS_CUDA_OK;
 }
