@@ -54,6 +54,31 @@ def test_there_and_back_on_a_stream(cuda_engine):
     assert backend.numDataIds() == before
 
 
+def test_what_reads_foreign_memory_launches_at_once(cuda_engine):
+    """Elementwise kernels are usually deferred; over memory that its owner may rewrite they are not."""
+    from tfjs_b200 import ops as tf
+    stream = torch.cuda.current_stream().cuda_stream
+    x = torch.ones(10000, device="cuda")
+    t = tf.tensor(x, stream=stream)
+    y = tf.add(t, t)
+    cuda_engine.backend.signal_stream(stream)
+    x.fill_(7.0)
+    z = tf.mul(y, y)
+    assert np.all(z.arraySync() == 4.0)
+    for k in (t, y, z):
+        k.dispose()
+    # the tensor is forgotten even where the stream cannot be signalled: inside a captured step
+    before = cuda_engine.backend.numDataIds()
+    t = tf.tensor(x, stream=stream)
+    cuda_engine.backend.capture_begin(1 << 20)
+    with pytest.raises(Exception):
+        t.dispose()
+    with pytest.raises(Exception):
+        cuda_engine.backend.capture_end()
+    assert cuda_engine.backend.numDataIds() == before
+    assert np.all(x.cpu().numpy() == 7.0)
+
+
 def test_a_host_resident_tensor_goes_to_the_gpu(cuda_engine):
     from tfjs_b200 import ops as tf
     t = tf.tensor(np.arange(6, dtype=np.float32).reshape(2, 3))

@@ -119,6 +119,32 @@ def test_bad_lengths_are_reported(tf, cuda_engine):
         t.dispose()
 
 
+def test_captured_prompts_replay(tf, cuda_engine):
+    """Two captured prompts of different sizes, replayed in turn with an eager one in between: each
+    has a workspace of its own."""
+    backend = cuda_engine.backend
+    made = []
+    for seed, n, d in ((8, 300, 64), (9, 150, 128)):
+        q, k, v, s = inputs(seed, 2, 2, n, d, d)
+        ld = decays(2)
+        ts = [tf.tensor(x) for x in (q, k, v, ld, s)]
+        for t in ts:
+            backend.device_id(t.dataId)
+        backend.sync()
+        backend.capture_begin(64 << 20)
+        outs = tf.linear_attention(*ts, scale=0.125)
+        made.append((backend.capture_end(), outs, ts, dc.linear(q, k, v, ld, s, 0.125)))
+    for i in range(6):
+        backend.graph_launch(made[i % 2][0])
+        if i == 3:
+            call(tf, *[np.zeros((1, 1, 700, 32), np.float32)] * 3, decays(1))
+    for graph, outs, ts, ref in made:
+        check([t.arraySync() for t in outs], ref)
+        backend.graph_destroy(graph)
+        for t in ts + outs:
+            t.dispose()
+
+
 def test_captured_tokens_replay(tf, cuda_engine):
     """A captured token whose new state is copied over the old one: a replay a token."""
     backend = cuda_engine.backend

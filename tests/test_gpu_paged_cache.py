@@ -70,6 +70,10 @@ SHAPES = [
     (4, 1, 256, 24, [70, 333]),
     (32, 2, 255, 16, [40]),
     (5, 5, 2, 2, [11, 3]),
+    (40, 1, 64, 16, [200, 3]),
+    (6, 2, 128, 16, [400, 30]),
+    (24, 2, 20, 4, [70, 260, 1]),
+    (4, 1, 96, 1, [77]),
 ]
 
 
@@ -101,6 +105,23 @@ def test_attention_of_a_long_row(tf):
     w = r.random((2, 2, cache.capacity)).astype(np.float32)
     ref, neww, off, woff = dc.attention(q, cache, lengths, 0.125, None, w)
     got, gotw = attend(tf, cache, q, 0.125, None, w)
+    check(got, ref, off)
+    check(gotw, neww, woff)
+
+
+@pytest.mark.parametrize("heads,kv", [(2, 1), (4, 1), (8, 1), (16, 2)])
+def test_many_ragged_rows(tf, heads, kv):
+    """More rows than a warp has lanes, empty ones among them: every block takes an equal share of
+    the tiles, which begins and ends inside rows."""
+    r = np.random.default_rng(heads)
+    lengths = [int(n) for n in r.integers(0, 700, 75)]
+    lengths[10] = lengths[74] = lengths[0] = 0
+    lengths[40] = 1500
+    cache = dc.Cache(heads, kv, 32, 16, lengths)
+    q = r.standard_normal((75, heads, 1, 32)).astype(np.float32)
+    w = r.random((75, kv, cache.capacity)).astype(np.float32)
+    ref, neww, off, woff = dc.attention(q, cache, lengths, 0.2, None, w)
+    got, gotw = attend(tf, cache, q, 0.2, None, w)
     check(got, ref, off)
     check(gotw, neww, woff)
 
@@ -201,6 +222,8 @@ def run_evict(tf, cache, w, budget, recent, positions=None, total=None):
     (2, 16, 64, [3000, 1023, 1024, 2049], 1024, 100, True),
     (1, 8, 16, [50], 4000, 10, False),
     (3, 24, 8, [500, 17], 250, 0, True),
+    (1, 4, 64, [60000, 20], 20000, 7000, True),      # keys do not fit shared memory
+    (2, 6, 16, [9000, 4097], 4096, 0, False),
 ])
 def test_evict(tf, kv, dim, page, lengths, budget, recent, order):
     r = np.random.default_rng(budget + dim)

@@ -100,9 +100,11 @@ class GPUData(object):
         ref, self.tensorRef = self.tensorRef, None
         backend = self.backend
         if ref is not None and backend.ctx:
-            if self.stream is not None:
-                backend.check(backend.lib.tfjs_cuda_wait_stream(backend.ctx, self.stream))
-            ref.dispose()
+            try:
+                if self.stream is not None:
+                    backend.check(backend.lib.tfjs_cuda_wait_stream(backend.ctx, self.stream))
+            finally:
+                ref.dispose()
 
     def __del__(self):
         try:
@@ -519,6 +521,7 @@ class CudaBackend(object):
         self.data = {}        # DataId -> _Record
         self._pinned = []
         self._hidden = 0      # records kept alive only by pending launches
+        self._foreign = 0     # records over memory that is not the backend's
         self.lazy_fusion = os.environ.get("TFJS_CUDA_NO_LAZY_FUSION", "0") in ("", "0")
         # a pending 3x3 depthwise convolution consumed by a 1x1 convolution runs inside that
         # convolution's launch (TFJS_CUDA_NO_DW_PROJECT=1 keeps the two launches)
@@ -619,6 +622,7 @@ class CudaBackend(object):
         dataId = DataId()
         rec = _Record(self._out_id.value, nbytes, found, 1, None)
         rec.foreign, rec.stream = values, stream
+        self._foreign += 1
         self.data[dataId] = rec
         return TensorInfo(dataId, have if shape is None else shape, found)
 
@@ -673,6 +677,9 @@ class CudaBackend(object):
                                     if any(self._still_pending_matmul(i) for i in ids)}
             ids = [i for i in self._matmuls_on.get(pending.a, []) if self._still_pending_matmul(i)]
             self._matmuls_on[pending.a] = ids + [dataId]
+        if self._foreign and any(self.data[d].foreign is not None for d in pending.deps()):
+            # its owner may rewrite the memory whenever it likes: what reads it launches now
+            self._resolve(rec)
         return TensorInfo(dataId, shape, dtype)
 
     def _still_pending_matmul(self, dataId):
@@ -860,9 +867,6 @@ class CudaBackend(object):
         rec = self.data.get(dataId)
         if rec is None:
             return False
-        if rec.foreign is not None and rec.ref - rec.held == 1:
-            # its owner may reuse the memory from here on: pending readers launch now
-            self._launch_readers(dataId, rec)
         if rec.held == 0:
             rec.ref -= 1
         else:
@@ -876,13 +880,15 @@ class CudaBackend(object):
         if rec.held > 0 and rec.ref <= rec.held:
             self._hidden -= 1
         del self.data[dataId]
-        if rec.stream is not None:     # its owner's next work waits for what reads it here
-            self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream))
         if rec.dev:
             self.check(self.lib.tfjs_cuda_free(self.ctx, rec.dev))
         if rec.pending is not None:
             pending, rec.pending = rec.pending, None
             self._release(pending)
+        if rec.foreign is not None:
+            self._foreign -= 1
+            if rec.stream is not None:     # its owner's next work waits for what read it here
+                self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream))
 
     def refCount(self, dataId):
         rec = self.data.get(dataId)

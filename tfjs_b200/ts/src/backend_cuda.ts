@@ -41,6 +41,7 @@ export class CudaBackend extends KernelBackend {
   readonly ctx: Ctx;
   private data: DataStorage<Record>;
   private hidden = 0;           // records kept alive only by pending launches
+  private foreign = 0;          // records over memory that is not the backend's
   private logDepth = 0;
   /** chain signature -> the library has a straight-line kernel for it */
   readonly ewCatalogue = new Map<string, boolean>();
@@ -110,9 +111,12 @@ export class CudaBackend extends KernelBackend {
     const nbytes = util.sizeFromShape(shape) * bytesPerElement(dtype);
     const dataId = {};
     for (const d of pending.deps()) this.adjust(this.data.get(d), 1, 1);
-    this.data.set(dataId, {id: 0, nbytes, dtype, refCount: 1, pending, held: 0});
+    const r: Record = {id: 0, nbytes, dtype, refCount: 1, pending, held: 0};
+    this.data.set(dataId, r);
     this.pendingIds.add(dataId);
     if (pending instanceof PendingMatMul) this.noteMatMul(dataId, pending);
+    // the owner of foreign memory may rewrite it whenever it likes: what reads it launches now
+    if (this.foreign > 0 && pending.deps().some(d => this.data.get(d).foreign != null)) this.resolve(r);
     return {dataId, shape, dtype};
   }
 
@@ -265,6 +269,7 @@ export class CudaBackend extends KernelBackend {
     const id = binding.fromDevice(this.ctx, values.buffer, nbytes);
     const dataId = {};
     this.data.set(dataId, {id, nbytes, dtype, refCount: 1, held: 0, foreign: values});
+    this.foreign++;
     return {dataId, shape, dtype};
   }
 
@@ -304,8 +309,6 @@ export class CudaBackend extends KernelBackend {
   override disposeData(dataId: object, force = false): boolean {
     if (!this.data.has(dataId)) return false;
     const r = this.data.get(dataId);
-    // its owner may reuse the memory from here on: pending readers launch now
-    if (r.foreign != null && r.refCount - r.held === 1) this.launchReaders(dataId, r);
     this.adjust(r, -1, 0);
     if (r.refCount > 0 && (!force || r.held > 0)) return false;
     this.drop(dataId, r);
@@ -316,8 +319,11 @@ export class CudaBackend extends KernelBackend {
     if (r.held > 0 && r.refCount <= r.held) this.hidden--;
     this.data.delete(dataId);
     this.pendingIds.delete(dataId);
-    if (r.foreign?.stream != null) binding.signalStream(this.ctx, r.foreign.stream);
     if (r.id !== 0) binding.free(this.ctx, r.id);
+    if (r.foreign != null) {
+      this.foreign--;
+      if (r.foreign.stream != null) binding.signalStream(this.ctx, r.foreign.stream);
+    }
     if (r.pending != null) {
       const p = r.pending;
       r.pending = undefined;
