@@ -988,6 +988,10 @@ paged_attention_join_kernel(const PagedLayout g, const PagedAttnArgs a, const fl
     __syncthreads();
     const int part0 = part0_s, parts = parts_s;
     const int heads = min(a.chunk, a.group - gc * a.chunk);
+    if (parts == 1 && out_weights == nullptr) {  // one block has written the result
+      __syncthreads();
+      continue;
+    }
     for (int gi = warp; gi < heads; gi += kJoinThreads / 32) {
       const float2* ml = a.part_ml + (uint64_t)part0 * a.chunk + gi;
       float mx = -INFINITY, sum = 0.f;
@@ -1185,9 +1189,12 @@ extern "C" int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_pag
   a.tile = plan.tile;
   a.slots = plan.slots;
   a.group_chunks = (a.group + a.chunk - 1) / a.chunk;
-  // Rows of up to four tiles: a block each, whose result needs no joining.
+  // Short rows: a block each, whose result needs no joining.  (12 rows and heads of 128 / 256 / 512
+  // slots: 6.5 / 9.9 / 16 us against 10 / 10 / 11 with equal shares and their joining; 128 of 256 / 512 /
+  // 1024: 14 / 21 / 36 against 16 / 22 / 28; 256 of them: 15 / 24 / 43 against 32 / 37 / 54, but there a
+  // single long row among short ones would be waited for.)
   const uint64_t blocks = kv_units * a.group_chunks;
-  a.whole = cap <= 4ull * a.tile;
+  a.whole = cap <= (blocks * 4 >= (uint64_t)ctx->sm_count * 3 ? 8ull : 4ull) * a.tile;
   a.shares = a.whole ? (int)blocks : plan.blocks;
 
   cudaSetDevice(ctx->device);
@@ -1204,8 +1211,11 @@ extern "C" int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_pag
   }
   if ((rc = form.launch(ctx, g, a, plan))) return rc;
   if (weights_id || !a.whole) {
-    // blocks for the heads to join, and one for every four slots a thread
-    uint64_t per = a.whole ? 1 : a.group;
+    // blocks for the heads to join (few, where the rows and heads are many), and one for every four
+    // slots a thread
+    uint64_t per = ((uint64_t)ctx->sm_count * 4 + kv_units - 1) / kv_units;
+    if (per > (uint64_t)a.group) per = a.group;
+    if (a.whole) per = 1;
     const bool four = weights_id && cap % 4 == 0 && (((uintptr_t)wp | (uintptr_t)owp) & 15) == 0;
     const uint64_t stretch = kJoinThreads * 4;
     if (weights_id && per < (cap + stretch - 1) / stretch) per = (cap + stretch - 1) / stretch;

@@ -140,8 +140,8 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
 // select of 8 bits a pass (counting, no sorting), then one pass in slot order that ranks the
 // slots equal to it, the free places below m and the kept slots from m on: every thread has a
 // stretch of slots, so that each of these takes one sum over the block.  HELD: the keys are formed
-// once and kept in shared memory, which a row of up to 48 k slots allows.  NT: threads; 1024 for long
-// rows, 256 for short ones, of which an SM then holds several.  V: values a lane moves at a time.
+// once and kept in shared memory, which a row of up to 48 k slots allows.  NT: threads.  V: values a
+// lane moves at a time.
 template <bool HELD, int V, int NT>
 __global__ void __launch_bounds__(NT)
 paged_evict_select_kernel(const PagedLayout g, const EvictArgs a) {
@@ -403,7 +403,10 @@ int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params
   a.v_cache = vp;
   a.move = most <= 64;
   const uint64_t held = (uint64_t)g.capacity * 4;
-  const bool small = g.capacity <= 4096, keep_keys = held <= 192 * 1024;
+  // 256 threads where there are more rows and heads than SMs, which then hold several blocks, and rows
+  // are short (256 of them with 1025 / 2049 / 4097 / 8193 slots: 10 / 14 / 23 / 41 us against 16 / 18 /
+  // 22 / 32 with 1024 threads; 8 of them: 10 / 13 / 18 / 38 against 8 / 9 / 12 / 16)
+  const bool small = g.capacity <= 4096 && units > (uint64_t)ctx->sm_count, keep_keys = held <= 192 * 1024;
   void (*kernel)(PagedLayout, EvictArgs) =
       small ? (wide ? paged_evict_select_kernel<true, 4, 256> : paged_evict_select_kernel<true, 1, 256>)
       : keep_keys ? (wide ? paged_evict_select_kernel<true, 4, 1024> : paged_evict_select_kernel<true, 1, 1024>)
