@@ -6,9 +6,9 @@
 
 namespace {
 
-// Up to here the recurrence, one dependent step a token: 16 / 32 / 64 tokens take 8 / 14 / 26 us for
-// 12 states of 64 x 64 and 115 / 213 / 409 us for 1024 of 128 x 128, where the chunked form takes
-// 17 / 17 / 18 and 295 / 298 / 310.
+// Up to here the recurrence, one dependent step a token: 8 / 16 / 32 tokens take 7 / 11 / 19 us for
+// 12 states of 64 x 64 and 69 / 123 / 229 us for 1024 of 128 x 128, where the chunked form takes
+// 17 and 295 for each of them.
 constexpr int kFewTokens = 32;
 constexpr int kTileV = 32;      // columns of the state that a block holds
 constexpr int kRowGroups = 32;  // threads that share a column's rows

@@ -10,7 +10,7 @@
 //
 // The rows of one page and head are contiguous, so tiles of keys and values travel as bulk
 // copies into a ring in shared memory, issued by a warp of their own and several tiles ahead of
-// the four warps that compute: the bytes in flight do not depend on registers.  Head sizes that
+// the warps that compute: the bytes in flight do not depend on registers.  Head sizes that
 // are no multiple of four values (rows not on 16 bytes) take a kernel with plain loads.
 //
 // Arithmetic, for up to 4 query heads a key-value head: fp32 multiply-adds.  For more, the
@@ -18,7 +18,8 @@
 // where the bytes take 83; 144 with MMAs, whose 16 rows half a group of 4 would leave empty:
 // 196 against 148 us with 4 heads of 128), so the products run as m16n8k8 TF32 MMAs with each operand split into
 // two TF32 parts and three products (fp32 accuracy; the single query row of a decode step has no
-// tile for the 128-row tcgen05 form).  Tensor cores cut sums off instead of rounding them, so
+// tile for the 128-row tcgen05 form); with up to 8 heads both parts of the queries, or of the
+// probabilities, are the 16 rows of one.  Tensor cores cut sums off instead of rounding them, so
 // sums over a tile start from zero and are added to fp32 registers.
 #include "paged.cuh"
 #include "ptx.cuh"
@@ -26,7 +27,7 @@
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWarps = 4;            // that compute
+constexpr int kWarps = 4;            // that compute with plain loads
 
 struct PagedAttnArgs {
   const float* q;         // [batch, heads, head_dim]
@@ -196,10 +197,14 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
-__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+template <int NW>
+__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory"); }
 
-constexpr int kBulkThreads = (kWarps + 1) * 32;
 constexpr int kMaxSlots = 8;
+// Warps that compute and blocks of an SM.  The MMA form of small heads is bound by the latency of its
+// instructions, so it has 16 warps on an SM.
+constexpr int compute_warps(int dm, int gt, bool mma) { return mma && gt == 8 && dm <= 64 ? 8 : 4; }
+constexpr int blocks_per_sm(int dm, int gt, bool mma) { return dm <= 64 && compute_warps(dm, gt, mma) == 4 ? 3 : 2; }
 
 // x = hi + lo, hi rounded to TF32's 11 bits
 __device__ __forceinline__ float tf32_hi(float x) {
@@ -216,15 +221,16 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], float a0, float a1, floa
 }
 
 // Slots of a warp's share of a tile, and shared memory beside the ring: queries, probabilities
-// (multiply-add form), two places for the joining of the warps, their maxima and sums, barriers.
+// (multiply-add form), places for the joining of the warps, their maxima and sums, barriers.
 template <int DM>
 constexpr int warp_slots() { return DM <= 128 ? 16 : 8; }
 template <int DM, int GT, bool MMA>
 constexpr int query_floats() { return MMA ? DM * 8 * (GT == 16 ? 4 : 2) : GT * DM; }
 template <int DM, int GT, bool MMA>
 constexpr int bulk_fixed_bytes() {
-  return query_floats<DM, GT, MMA>() * 4 + (MMA ? 0 : kWarps * warp_slots<DM>() * GT * 4) + 2 * GT * DM * 4 +
-         kWarps * GT * 8 + 2 * kMaxSlots * 8 + 128;
+  constexpr int NW = compute_warps(DM, GT, MMA);
+  return query_floats<DM, GT, MMA>() * 4 + (MMA ? 0 : NW * warp_slots<DM>() * GT * 4) + NW / 2 * GT * DM * 4 +
+         NW * GT * 8 + 2 * kMaxSlots * 8 + 128;
 }
 
 // One warp's computing state, multiply-add form.  Scores: four lanes a slot, each 16-byte pieces
@@ -243,7 +249,7 @@ struct FmaState {
 
   __device__ __forceinline__ static void load_queries(const PagedLayout& g, const PagedAttnArgs& a, const Piece& p,
                                                       float* q_s, int tid) {
-    for (int i = tid; i < GT * DM; i += kWarps * 32) {
+    for (int i = tid; i < GT * DM; i += compute_warps(DM, GT, false) * 32) {
       const int gi = i / DM, d = i - gi * DM;
       q_s[i] = gi < p.live && d < g.head_dim
                    ? __ldg(a.q + ((uint64_t)p.b * a.heads + p.head0 + gi) * g.head_dim + d) : 0.f;
@@ -413,7 +419,7 @@ struct MmaState {
   // [step of 8][lane][hi (row, K c), hi (row, K c + 4), then row + 8, then lo the same]
   __device__ __forceinline__ static void load_queries(const PagedLayout& g, const PagedAttnArgs& a, const Piece& p,
                                                       float* q_s, int tid) {
-    for (int i = tid; i < GT * DM; i += kWarps * 32) {
+    for (int i = tid; i < GT * DM; i += compute_warps(DM, GT, true) * 32) {
       const int gi = i / DM, d = i - gi * DM;
       const float x = gi < p.live && d < g.head_dim
                           ? __ldg(a.q + ((uint64_t)p.b * a.heads + p.head0 + gi) * g.head_dim + d) : 0.f;
@@ -470,18 +476,22 @@ struct MmaState {
         for (int t = 0; t < NT; ++t) {
           const float b0 = tf32_hi(kv[t][2 * y]), b1 = tf32_hi(kv[t][2 * y + 1]);
           const float c0 = kv[t][2 * y] - b0, c1 = kv[t][2 * y + 1] - b1;
-          const float h1 = R == 2 ? qh[2 * R - 2] : 0.f, h3 = R == 2 ? qh[2 * R - 1] : 0.f;
-          const float l1 = R == 2 ? ql[2 * R - 2] : 0.f, l3 = R == 2 ? ql[2 * R - 1] : 0.f;
-          mma_tf32(lo[t], qh[0], h1, qh[1], h3, c0, c1);
-          mma_tf32(lo[t], ql[0], l1, ql[1], l3, b0, b1);
-          mma_tf32(hi[t], qh[0], h1, qh[1], h3, b0, b1);
+          if constexpr (R == 1) {                         // rows + 8: the queries' lo parts
+            mma_tf32(lo[t], qh[0], ql[0], qh[1], ql[1], c0, c1);
+            mma_tf32(hi[t], qh[0], ql[0], qh[1], ql[1], b0, b1);
+          } else {
+            mma_tf32(lo[t], qh[0], qh[2], qh[1], qh[3], c0, c1);
+            mma_tf32(lo[t], ql[0], ql[2], ql[1], ql[3], b0, b1);
+            mma_tf32(hi[t], qh[0], qh[2], qh[1], qh[3], b0, b1);
+          }
         }
       }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int x = 0; x < 2 * R; ++x) s[t][x] = hi[t][x] + lo[t][x];
+      for (int x = 0; x < 2 * R; ++x)
+        s[t][x] = R == 1 ? hi[t][x] + (hi[t][2 + x] + (lo[t][x] + lo[t][2 + x])) : hi[t][x] + lo[t][x];
   }
   float down[R];
   __device__ __forceinline__ void softmax(const PagedLayout& g, const PagedAttnArgs& a, const Piece& pc, int t0,
@@ -558,20 +568,24 @@ struct MmaState {
         const float4 x0 = in && (all || (seen >> (t * 8 + 2 * c) & 1u)) ? *reinterpret_cast<const float4*>(p0) : zero;
         const float4 x1 = in && (all || (seen >> (t * 8 + 2 * c + 1) & 1u)) ? *reinterpret_cast<const float4*>(p0 + D) : zero;
         const float v0[4] = {x0.x, x0.y, x0.z, x0.w}, v1[4] = {x1.x, x1.y, x1.z, x1.w};
-        const float h1 = R == 2 ? ph[t][2 * R - 2] : 0.f, h3 = R == 2 ? ph[t][2 * R - 1] : 0.f;
-        const float l1 = R == 2 ? pl[t][2 * R - 2] : 0.f, l3 = R == 2 ? pl[t][2 * R - 1] : 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float b0 = tf32_hi(v0[e]), b1 = tf32_hi(v1[e]);
-          mma_tf32(o[e], ph[t][0], h1, ph[t][1], h3, v0[e] - b0, v1[e] - b1);
-          mma_tf32(o[e], pl[t][0], l1, pl[t][1], l3, b0, b1);
-          mma_tf32(o[e], ph[t][0], h1, ph[t][1], h3, b0, b1);
+          if constexpr (R == 1) {                         // rows + 8: the probabilities' lo parts
+            mma_tf32(o[e], ph[t][0], pl[t][0], ph[t][1], pl[t][1], v0[e] - b0, v1[e] - b1);
+            mma_tf32(o[e], ph[t][0], pl[t][0], ph[t][1], pl[t][1], b0, b1);
+          } else {
+            mma_tf32(o[e], ph[t][0], ph[t][2], ph[t][1], ph[t][3], v0[e] - b0, v1[e] - b1);
+            mma_tf32(o[e], pl[t][0], pl[t][2], pl[t][1], pl[t][3], b0, b1);
+            mma_tf32(o[e], ph[t][0], ph[t][2], ph[t][1], ph[t][3], b0, b1);
+          }
         }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int x = 0; x < 2 * R; ++x) acc[j][e][x] = fmaf(acc[j][e][x], down[x >> 1], o[e][x]);
+        for (int x = 0; x < 2 * R; ++x)
+          acc[j][e][x] = fmaf(acc[j][e][x], down[x >> 1], R == 1 ? o[e][x] + o[e][2 + x] : o[e][x]);
     }
   }
   __device__ __forceinline__ void finish(float2* ml, int lane) {
@@ -600,21 +614,20 @@ struct MmaState {
 
 template <int DM, int GT, bool MMA> struct Chosen { typedef FmaState<DM, GT> State; };
 template <int DM, int GT> struct Chosen<DM, GT, true> { typedef MmaState<DM, GT> State; };
-constexpr int blocks_per_sm(int dm) { return dm <= 64 ? 3 : 2; }
 
 template <int DM, int GT, bool MMA>
-__global__ void __launch_bounds__(kBulkThreads, blocks_per_sm(DM))
+__global__ void __launch_bounds__((compute_warps(DM, GT, MMA) + 1) * 32, blocks_per_sm(DM, GT, MMA))
 paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
   typedef typename Chosen<DM, GT, MMA>::State State;
-  constexpr int TW = warp_slots<DM>(), T = kWarps * TW;
+  constexpr int TW = warp_slots<DM>(), NW = compute_warps(DM, GT, MMA), T = NW * TW;
   extern __shared__ __align__(128) uint8_t smem[];
   const int D = g.head_dim;
   const uint32_t tile_bytes = (uint32_t)(T * D * 4);
   float* q_s = reinterpret_cast<float*>(smem + (uint32_t)a.slots * tile_bytes);
-  float* joined = q_s + query_floats<DM, GT, MMA>();      // [2][GT][DM]
-  float* p_all = joined + 2 * GT * DM;
-  float2* ml_s = reinterpret_cast<float2*>(p_all + (MMA ? 0 : kWarps * TW * GT));
-  const uint32_t bars = smem_u32(ml_s + kWarps * GT);
+  float* joined = q_s + query_floats<DM, GT, MMA>();      // [NW / 2][GT][DM]
+  float* p_all = joined + NW / 2 * GT * DM;
+  float2* ml_s = reinterpret_cast<float2*>(p_all + (MMA ? 0 : NW * TW * GT));
+  const uint32_t bars = smem_u32(ml_s + NW * GT);
   auto full = [&](int s) { return bars + 8u * (uint32_t)s; };
   auto empty = [&](int s) { return bars + 8u * (uint32_t)(kMaxSlots + s); };
   const uint32_t ring = smem_u32(smem);
@@ -622,7 +635,7 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
   if (tid == 0) {
     for (int s = 0; s < a.slots; ++s) {
       mbar_init(full(s), 1);
-      mbar_init(empty(s), kWarps);
+      mbar_init(empty(s), NW);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -639,7 +652,7 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
     }
   };
 
-  if (warp == kWarps) {
+  if (warp == NW) {
     // ------------------------------------------------------------------ producer --
     int used = 0;
     bool alive = true;
@@ -692,7 +705,7 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
   while (walk.next(g, a, pc)) {
     State::load_queries(g, a, pc, q_s, tid);
     st.reset();
-    compute_barrier();
+    compute_barrier<NW>();
     // lane j looks after slot t0 + j: its page, and what the mask adds to it (fetched a tile ahead)
     auto look = [&](int t, int& page, float& add) {
       const int mine = pc.begin + t * T + warp * TW + lane;
@@ -732,42 +745,46 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
       if (lane == 0) mbar_arrive(empty(slot));
       step();
     }
-    // the four warps' results: 2 and 3 give theirs to 0 and 1, then 1 gives its to 0
+    // the warps' results: the upper half of them gives its to the lower half, until one has all
     st.finish(ml_s + warp * GT, lane);
-    compute_barrier();
+    compute_barrier<NW>();
     auto top = [&](int gi) {
-      return fmaxf(fmaxf(ml_s[gi].x, ml_s[GT + gi].x), fmaxf(ml_s[2 * GT + gi].x, ml_s[3 * GT + gi].x));
+      float m = ml_s[gi].x;
+#pragma unroll
+      for (int w = 1; w < NW; ++w) m = fmaxf(m, ml_s[w * GT + gi].x);
+      return m;
     };
-    for (int round = 2; round >= 1; --round) {
+    for (int round = NW / 2; round >= 1; round >>= 1) {
+      const bool first = round == NW / 2;
       if (warp >= round && warp < 2 * round) {
         float* to = joined + (warp - round) * GT * DM;
         st.each(lane, [&](int gi, int d, float& x, float& y) {
-          const float f = round == 2 ? exp_from(ml_s[warp * GT + gi].x, top(gi)) : 1.0f;
+          const float f = first ? exp_from(ml_s[warp * GT + gi].x, top(gi)) : 1.0f;
           to[gi * DM + d] = x * f;
           to[gi * DM + d + 1] = y * f;
         });
       }
-      compute_barrier();
+      compute_barrier<NW>();
       if (warp < round) {
         const float* from = joined + warp * GT * DM;
         st.each(lane, [&](int gi, int d, float& x, float& y) {
-          const float f = round == 2 ? exp_from(ml_s[warp * GT + gi].x, top(gi)) : 1.0f;
+          const float f = first ? exp_from(ml_s[warp * GT + gi].x, top(gi)) : 1.0f;
           x = fmaf(x, f, from[gi * DM + d]);
           y = fmaf(y, f, from[gi * DM + d + 1]);
         });
       }
-      if (round == 2) compute_barrier();
+      if (round > 1) compute_barrier<NW>();
     }
     if (warp == 0)
       st.each(lane, [&](int gi, int d, float& x, float& y) {
         const float mx = top(gi);
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum = fmaf(ml_s[w * GT + gi].y, exp_from(ml_s[w * GT + gi].x, mx), sum);
+        for (int w = 0; w < NW; ++w) sum = fmaf(ml_s[w * GT + gi].y, exp_from(ml_s[w * GT + gi].x, mx), sum);
         write_result<GT>(g, a, pc, gi, d, x, mx, sum);
         write_result<GT>(g, a, pc, gi, d + 1, y, mx, sum);
       });
-    compute_barrier();                                    // queries, maxima and `joined` are free again
+    compute_barrier<NW>();                                    // queries, maxima and `joined` are free again
   }
 }
 
@@ -1072,11 +1089,11 @@ struct Plan {
 // (the keys and the values of one tile).
 template <int DM, int GT, bool MMA>
 Plan plan_bulk(const tfjs_cuda_ctx* ctx, int dim) {
-  constexpr int fixed = bulk_fixed_bytes<DM, GT, MMA>(), T = kWarps * warp_slots<DM>();
+  constexpr int fixed = bulk_fixed_bytes<DM, GT, MMA>(), T = compute_warps(DM, GT, MMA) * warp_slots<DM>();
   Plan p;
   p.chunk = GT;
   p.tile = T;
-  int per_sm = blocks_per_sm(DM);
+  int per_sm = blocks_per_sm(DM, GT, MMA);
   const int tile = T * dim * 4;
   do {
     const int room = 227 * 1024 / per_sm - 1024 - fixed;
@@ -1091,7 +1108,7 @@ template <int DM, int GT, bool MMA>
 int launch_bulk(tfjs_cuda_ctx* ctx, const PagedLayout& g, const PagedAttnArgs& a, const Plan& p) {
   CUDA_TRY(ctx, cudaFuncSetAttribute(paged_attention_bulk_kernel<DM, GT, MMA>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
-  paged_attention_bulk_kernel<DM, GT, MMA><<<a.shares, kBulkThreads, p.smem, ctx->stream>>>(g, a);
+  paged_attention_bulk_kernel<DM, GT, MMA><<<a.shares, (compute_warps(DM, GT, MMA) + 1) * 32, p.smem, ctx->stream>>>(g, a);
   LAUNCH_CHECK(ctx, MMA ? "paged_attention_bulk_kernel<mma>" : "paged_attention_bulk_kernel<fma>");
   return TFJS_CUDA_OK;
 }
