@@ -1235,7 +1235,13 @@ extern "C" int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_pag
     if (a.whole) per = 1;
     const bool four = weights_id && cap % 4 == 0 && (((uintptr_t)wp | (uintptr_t)owp) & 15) == 0;
     const uint64_t stretch = kJoinThreads * 4;
-    if (weights_id && per < (cap + stretch - 1) / stretch) per = (cap + stretch - 1) / stretch;
+    if (weights_id) {
+      // (all of them at once: finding the parts takes a block as long as a stretch of slots)
+      uint64_t want = (cap + stretch - 1) / stretch;
+      const uint64_t room = (uint64_t)ctx->sm_count * 8 / kv_units;
+      if (want > room) want = room;
+      if (per < want) per = want;
+    }
     if (per * kv_units > 0x7fffffffull) per = 0x7fffffffull / kv_units;
     const unsigned grid = (unsigned)(kv_units * per);
     const unsigned stat = a.group * sizeof(float2);
