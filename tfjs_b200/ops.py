@@ -333,7 +333,7 @@ def paged_cache_append(kCache, vCache, k, v, pageTable, lengths, counts=None):
     to the slots from lengths[b] on; counts [batch] int32 says how many tokens of each row
     are real (a padded batch), all by default.  Tokens beyond maxPages * pageSize slots are
     dropped, and places whose page is not in the pool skipped; the next blocking read reports
-    either.  A kernel of the 'cuda' backend with no counterpart among the reference's ops."""
+    either.  Rows may share pages that they only read, not those that are written.  A kernel of the 'cuda' backend with no counterpart among the reference's ops."""
     return _run("_PagedCacheAppend", {"kCache": kCache, "vCache": vCache, "k": k, "v": v,
                                       "pageTable": pageTable, "lengths": lengths,
                                       "counts": counts})
@@ -363,7 +363,8 @@ def paged_cache_evict(kCache, vCache, weights, pageTable, lengths, budget, recen
     the largest; among equals the lower slot stays).
 
     The pools are updated in place: kept slots behind the budget move into the places that
-    become free, so slots are no longer in the order of their tokens.  positions [batch,
+    become free, so slots are no longer in the order of their tokens.  A row that loses slots
+    must not share its pages with another.  positions [batch,
     kvHeads, maxPages * pageSize] int32 says which token each slot holds; entries below 0
     (and all of them when it is absent) stand for tokens appended in order: total[b] -
     (lengths[b] - slot), with total [batch] int32 the tokens a row has seen (default: its
