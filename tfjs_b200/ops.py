@@ -333,7 +333,8 @@ def paged_cache_append(kCache, vCache, k, v, pageTable, lengths, counts=None):
     to the slots from lengths[b] on; counts [batch] int32 says how many tokens of each row
     are real (a padded batch), all by default.  Tokens beyond maxPages * pageSize slots are
     dropped, and places whose page is not in the pool skipped; the next blocking read reports
-    either.  Rows may share pages that they only read, not those that are written.  A kernel of the 'cuda' backend with no counterpart among the reference's ops."""
+    either.  Rows may share pages that they only read, not those that are written.  A kernel
+    of the 'cuda' backend with no counterpart among the reference's ops."""
     return _run("_PagedCacheAppend", {"kCache": kCache, "vCache": vCache, "k": k, "v": v,
                                       "pageTable": pageTable, "lengths": lengths,
                                       "counts": counts})
