@@ -825,10 +825,10 @@ int launch_chunks(tfjs_cuda_ctx* ctx, ChunkArgs& g) {
   const int s_smem = s_fixed + s.stages * s.stage_bytes;
   const unsigned grid = (unsigned)(g.items < ctx->sm_count ? g.items : ctx->sm_count);
   if (g.dkp <= 128) {
-    CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
+    CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap));
     linear_chunk_states_kernel<WIDE, 4><<<grid, kStateThreads, s_smem, ctx->stream>>>(s);
   } else {
-    CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, s_smem));
+    CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_states_kernel<WIDE, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap));
     linear_chunk_states_kernel<WIDE, 8><<<grid, kStateThreads, s_smem, ctx->stream>>>(s);
   }
   LAUNCH_CHECK(ctx, "linear_chunk_states_kernel");
@@ -845,7 +845,7 @@ int launch_chunks(tfjs_cuda_ctx* ctx, ChunkArgs& g) {
   g.stages = (kSmemCap - o_fixed) / g.stage_bytes;
   if (g.stages > kMaxStages) g.stages = kMaxStages;
   const int o_smem = o_fixed + g.stages * g.stage_bytes;
-  CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_outputs_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, o_smem));
+  CUDA_TRY(ctx, cudaFuncSetAttribute(linear_chunk_outputs_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemCap));
   linear_chunk_outputs_kernel<WIDE><<<grid, kOutThreads, o_smem, ctx->stream>>>(g);
   LAUNCH_CHECK(ctx, "linear_chunk_outputs_kernel");
   return TFJS_CUDA_OK;

@@ -1080,6 +1080,8 @@ paged_attention_join_kernel(const PagedLayout g, const PagedAttnArgs a, const fl
 }
 
 // ---- host ------------------------------------------------------------------------------------
+constexpr int kBlockSmem = 226 * 1024;   // that a single block of an SM may ask for
+
 // How a call is cut into shares, and what its blocks need.
 struct Plan {
   int chunk, tile, blocks, slots, smem;
@@ -1096,7 +1098,7 @@ Plan plan_bulk(const tfjs_cuda_ctx* ctx, int dim) {
   int per_sm = blocks_per_sm(DM, GT, MMA);
   const int tile = T * dim * 4;
   do {
-    const int room = 227 * 1024 / per_sm - 1024 - fixed;
+    const int room = (kBlockSmem + 1024) / per_sm - 1024 - fixed;   // (a block has 1 KB beside what it asks for)
     p.slots = room > 0 ? room / tile : 0;
   } while (p.slots < 2 && --per_sm > 0);
   if (p.slots > kMaxSlots) p.slots = kMaxSlots;
@@ -1106,8 +1108,9 @@ Plan plan_bulk(const tfjs_cuda_ctx* ctx, int dim) {
 }
 template <int DM, int GT, bool MMA>
 int launch_bulk(tfjs_cuda_ctx* ctx, const PagedLayout& g, const PagedAttnArgs& a, const Plan& p) {
+  // (the most that any call of it takes, so that two contexts of a process cannot lower it for each other)
   CUDA_TRY(ctx, cudaFuncSetAttribute(paged_attention_bulk_kernel<DM, GT, MMA>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, kBlockSmem));
   paged_attention_bulk_kernel<DM, GT, MMA><<<a.shares, (compute_warps(DM, GT, MMA) + 1) * 32, p.smem, ctx->stream>>>(g, a);
   LAUNCH_CHECK(ctx, MMA ? "paged_attention_bulk_kernel<mma>" : "paged_attention_bulk_kernel<fma>");
   return TFJS_CUDA_OK;

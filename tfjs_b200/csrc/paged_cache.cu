@@ -437,13 +437,16 @@ int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params
   // 256 threads where there are more rows and heads than SMs, which then hold several blocks, and rows
   // are short (256 of them with 1025 / 2049 / 4097 / 8193 slots: 10 / 14 / 23 / 41 us against 16 / 18 /
   // 22 / 32 with 1024 threads; 8 of them: 10 / 13 / 18 / 38 against 8 / 9 / 12 / 16)
-  const bool small = g.capacity <= 4096 && units > (uint64_t)ctx->sm_count, keep_keys = held <= 192 * 1024;
+  constexpr int kMostHeld = 192 * 1024;
+  const bool small = g.capacity <= 4096 && units > (uint64_t)ctx->sm_count, keep_keys = held <= (uint64_t)kMostHeld;
   void (*kernel)(PagedLayout, EvictArgs) =
       small ? (wide ? paged_evict_select_kernel<true, 4, 256> : paged_evict_select_kernel<true, 1, 256>)
       : keep_keys ? (wide ? paged_evict_select_kernel<true, 4, 1024> : paged_evict_select_kernel<true, 1, 1024>)
                   : (wide ? paged_evict_select_kernel<false, 4, 1024> : paged_evict_select_kernel<false, 1, 1024>);
-  if (held > 48 * 1024 && keep_keys)
-    CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)held));
+  // (Without asking for more, a launch has 48 KB for the keys and the kernel's own arrays together.  The
+  // same amount whatever the row needs, so that two contexts of a process cannot lower it for each other.)
+  if (held > 32 * 1024 && keep_keys)
+    CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld));
   kernel<<<(unsigned)units, small ? 256 : 1024, keep_keys ? held : 0, ctx->stream>>>(g, a);
   LAUNCH_CHECK(ctx, "paged_evict_select_kernel");
   if (!a.move) {
