@@ -115,7 +115,9 @@ int tfjs_cuda_read_begin(tfjs_cuda_ctx* ctx, int32_t id, void* host, uint64_t nb
 int tfjs_cuda_read_wait(tfjs_cuda_ctx* ctx, int32_t ticket);
 int tfjs_cuda_sync(tfjs_cuda_ctx* ctx);
 int tfjs_cuda_size_of(tfjs_cuda_ctx* ctx, int32_t id, uint64_t* out_nbytes);
-/* Raw device address of a tensor, for interop (profilers, other libraries). */
+/* Raw device address of a tensor, for interop (profilers, other libraries).  An upload that is
+ * still on its way is waited for on the device: work on a stream that tfjs_cuda_signal_stream is
+ * called for afterwards finds it there. */
 int tfjs_cuda_device_ptr(tfjs_cuda_ctx* ctx, int32_t id, void** out_ptr);
 /* A tensor over device memory that belongs to the caller (another library's buffer), without
  * a copy: the device half of creating a tensor from GPU data.  `ptr` must be device memory of

@@ -672,6 +672,10 @@ int tfjs_cuda_device_ptr(tfjs_cuda_ctx* ctx, int32_t id, void** out_ptr) {
   if (!ctx || !out_ptr) return TFJS_CUDA_INVALID_ARG;
   Buffer* b = ctx_buf(ctx, id);
   if (!b) return ctx_fail(ctx, TFJS_CUDA_UNKNOWN_ID, "device_ptr: unknown tensor id %d", id);
+  if (b->ready) {   // still on its way: the compute stream waits, and whoever is signalled behind it
+    const int rc = ctx_get(ctx, id, 0, "device_ptr", &b);
+    if (rc) return rc;
+  }
   *out_ptr = b->ptr;
   return TFJS_CUDA_OK;
 }
