@@ -36,3 +36,29 @@ def test_an_upload_that_is_handed_out_at_once(cuda_engine):
         assert summed(ws["w"]) == src.astype(np.float64).sum()
         ws["w"].dispose()
     assert backend.numDataIds() == before
+
+
+def test_from_one_stream_through_a_tensor_to_another(cuda_engine):
+    """A tensor over memory that stream A fills, handed on to stream B, which was signalled just before:
+    B waits for A."""
+    from tfjs_b200 import ops as tf
+    backend = cuda_engine.backend
+    before = backend.numDataIds()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    n = 1 << 25
+    x = torch.zeros(n, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(4):
+        for s in (a, b):                     # either has been the one signalled last
+            backend.signal_stream(s.cuda_stream)
+        with torch.cuda.stream(a):
+            for _ in range(50):
+                x += 1.0
+        t = tf.tensor(x, stream=a.cuda_stream)
+        with torch.cuda.stream(b):
+            g = torch.as_tensor(t.dataToGPU(b.cuda_stream), device="cuda")
+            assert g.double().sum().item() == 50.0 * (i + 1) * n
+        del g
+        t.dispose()
+        a.wait_stream(b)
+    assert backend.numDataIds() == before

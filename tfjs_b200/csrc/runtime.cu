@@ -734,7 +734,14 @@ static int order_streams(tfjs_cuda_ctx* ctx, cudaStream_t before, cudaStream_t a
 int tfjs_cuda_wait_stream(tfjs_cuda_ctx* ctx, void* stream) {
   if (!ctx) return TFJS_CUDA_INVALID_ARG;
   NOT_WHILE_CAPTURING(ctx, "waiting for a caller's stream");
-  return order_streams(ctx, (cudaStream_t)stream, ctx->stream, (cudaStream_t)stream);
+  const int rc = order_streams(ctx, (cudaStream_t)stream, ctx->stream, (cudaStream_t)stream);
+  if (rc) return rc;
+  // That work is in front of this context's stream now, so whoever is signalled waits for it too; the
+  // stream it came from alone has it already.
+  unsigned long long id = 0;
+  if (cudaStreamGetId((cudaStream_t)stream, &id) != cudaSuccess || id != ctx->signalled_stream) ctx->work++;
+  cudaGetLastError();
+  return TFJS_CUDA_OK;
 }
 
 int tfjs_cuda_signal_stream(tfjs_cuda_ctx* ctx, void* stream) {
