@@ -1,0 +1,106 @@
+"""What the host side of the backend asks of the library when device memory changes hands, on a
+stand-in for the library that records the calls."""
+import pytest
+
+from tfjs_b200 import _cabi
+from tfjs_b200.backend import CudaBackend
+
+
+class Library(object):
+    """Every call succeeds; `calls` holds their names, ids and addresses are made up, and `fail` gives
+    the status of calls that are to fail."""
+
+    def __init__(self):
+        self.calls, self.fail, self.ids, self.freed = [], {}, 0, []
+
+    def __getattr__(self, name):
+        if not name.startswith("tfjs_cuda_"):
+            raise AttributeError(name)
+        name = name[len("tfjs_cuda_"):]
+
+        def call(*args):
+            self.calls.append(name)
+            if name == "last_error":
+                return b"made to fail"
+            if name in self.fail:
+                return self.fail[name]
+            if name in ("alloc", "upload", "from_device"):
+                self.ids += 1
+                args[-1]._obj.value = self.ids
+            elif name == "device_ptr":
+                args[-1]._obj.value = 4096 * args[1]
+            elif name == "create":
+                args[-1]._obj.value = 1
+            elif name == "capture_end":
+                args[-1]._obj.value = 1
+            elif name == "free":
+                self.freed.append(args[1])
+            return 0
+        return call
+
+    def taken(self):
+        calls, self.calls = self.calls, []
+        return calls
+
+
+class Deferred(object):
+    """A deferred kernel over `reads`."""
+
+    def __init__(self, *reads, fails=False):
+        self.reads, self.fails, self.desc = reads, fails, None
+
+    def deps(self):
+        return list(self.reads)
+
+    def launch(self, backend, dev, post_act):
+        backend.lib.tfjs_cuda_a_kernel(backend.ctx)
+        if self.fails:
+            raise RuntimeError("a launch that fails")
+
+
+class Memory(object):
+    """Another library's."""
+
+    def __init__(self, shape=(2000,), read_only=False, **more):
+        self.__cuda_array_interface__ = dict({"shape": shape, "typestr": "<f4", "strides": None,
+                                              "data": (1 << 20, read_only), "version": 3}, **more)
+
+
+@pytest.fixture
+def backend(monkeypatch):
+    lib = Library()
+    monkeypatch.setattr(_cabi, "load", lambda: lib)
+    b = CudaBackend(0)
+    lib.taken()
+    yield b
+    b.ctx = None
+
+
+def test_handing_out_takes_a_reference(backend):
+    """The caller's handle is the caller's: of a TensorInfo and of an engine's tensor."""
+    from tfjs_b200.engine import Engine
+    t = backend.make_output([2000], "float32")
+    g = backend.readToGPU(t, 7)
+    assert g.buffer == 4096 * backend.data[t.dataId].dev and g.bufSize == 8000
+    g.dispose()
+    g.dispose()
+    assert backend.refCount(t.dataId) == 1 and backend.lib.freed == []
+    g = backend.readToGPU(t)
+    backend.disposeData(t.dataId)
+    assert backend.lib.freed == []
+    g.dispose()
+    assert len(backend.lib.freed) == 1 and backend.numDataIds() == 0
+    engine = Engine()
+    engine.backend = backend
+    x = engine.make_tensor_from_info(backend.make_output([2000], "float32"))
+    g = backend.readToGPU(x)
+    h = x.dataToGPU(7)
+    del g, h
+    assert not x.isDisposed and backend.refCount(x.dataId) == 1
+    backend.lib.fail["device_ptr"] = 2
+    for f in (backend.readToGPU, lambda y: y.dataToGPU()):
+        with pytest.raises(_cabi.CudaError):
+            f(x)
+    assert backend.refCount(x.dataId) == 1
+    x.dispose()
+    assert backend.numDataIds() == 0 and engine.num_tensors == 0

@@ -82,7 +82,7 @@ class GPUData(object):
     """A tensor's device memory (tfjs-core's GPUData, the result of tensor.dataToGPU()):
     `buffer` is the address, `bufSize` its bytes, `tensorRef` a tensor that keeps it alive.
     Libraries that read __cuda_array_interface__ take it without a copy.  When the last
-    reference is gone the tensor is disposed, behind the work queued on `stream` by then."""
+    reference is gone that tensor is disposed, behind the work queued on `stream` by then."""
     __slots__ = ("backend", "tensorRef", "buffer", "bufSize", "stream")
     _TYPESTR = {"float32": "<f4", "int32": "<i4", "bool": "|b1"}
 
@@ -104,7 +104,10 @@ class GPUData(object):
                 if self.stream is not None:
                     backend.check(backend.lib.tfjs_cuda_wait_stream(backend.ctx, self.stream))
             finally:
-                ref.dispose()
+                if isinstance(ref, TensorInfo):
+                    backend.disposeData(ref.dataId)
+                else:
+                    ref.dispose()
 
     def __del__(self):
         try:
@@ -629,7 +632,18 @@ class CudaBackend(object):
     def readToGPU(self, tensor, stream=None):
         """GPUData over `tensor`'s device memory (the KernelBackend method behind
         tensor.dataToGPU()), without a copy; launches a pending producer first.  With `stream`,
-        what is queued there from now on runs after this backend's work."""
+        what is queued there from now on runs after this backend's work.  The result has a
+        reference of its own: `tensor` remains the caller's."""
+        ref = TensorInfo(tensor.dataId, tensor.shape, tensor.dtype)
+        self.incRef(ref.dataId)
+        try:
+            return self.gpu_data(ref, stream)
+        except Exception:
+            self.disposeData(ref.dataId)
+            raise
+
+    def gpu_data(self, tensor, stream):
+        """readToGPU for a reference that the result takes over."""
         rec = self.data[tensor.dataId]
         ptr = c_void_p()
         self.check(self.lib.tfjs_cuda_device_ptr(

@@ -65,7 +65,7 @@ class Tensor(object):
         engine.num_tensors += 1
         ref = Tensor(engine, self.info())
         try:
-            return backend.readToGPU(ref, stream)
+            return backend.gpu_data(ref, stream)
         except Exception:
             ref.dispose()
             raise
