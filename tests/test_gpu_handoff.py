@@ -62,3 +62,32 @@ def test_from_one_stream_through_a_tensor_to_another(cuda_engine):
         t.dispose()
         a.wait_stream(b)
     assert backend.numDataIds() == before
+
+
+def test_what_is_pending_on_a_handed_out_tensor_saw_it_before(cuda_engine):
+    """An operation that was called before its operand's memory was handed out, or while somebody has
+    it, gives what it gives when launched at once."""
+    from tfjs_b200 import ops as tf
+    backend = cuda_engine.backend
+    before = backend.numDataIds()
+    stream = torch.cuda.current_stream().cuda_stream
+    t = tf.tensor(np.full(10000, 3.0, np.float32))
+    y = tf.add(t, t)                                    # deferred
+    assert not backend.lazy_fusion or backend.pending_of(y.dataId) is not None
+    g = torch.as_tensor(t.dataToGPU(stream), device="cuda")
+    g.zero_()
+    torch.cuda.synchronize()
+    assert np.all(y.arraySync() == 6.0)
+    z = tf.add(t, t)                                    # while g is there
+    backend.signal_stream(stream)
+    g.fill_(5.0)
+    torch.cuda.synchronize()
+    assert np.all(z.arraySync() == 0.0)
+    backend.wait_stream(stream)
+    del g
+    u = tf.add(t, t)                                    # nobody else has it any more
+    assert not backend.lazy_fusion or backend.pending_of(u.dataId) is not None
+    assert np.all(u.arraySync() == 10.0)
+    for k in (t, y, z, u):
+        k.dispose()
+    assert backend.numDataIds() == before

@@ -104,3 +104,20 @@ def test_handing_out_takes_a_reference(backend):
     assert backend.refCount(x.dataId) == 1
     x.dispose()
     assert backend.numDataIds() == 0 and engine.num_tensors == 0
+
+
+def test_readers_launch_before_an_address_is_handed_out(backend):
+    t = backend.make_output([2000], "float32")
+    y = backend.defer([2000], "float32", Deferred(t.dataId))
+    backend.lib.taken()
+    g = backend.readToGPU(t, 7)
+    assert backend.lib.taken() == ["alloc", "a_kernel", "device_ptr", "signal_stream"]
+    assert backend.pending_of(y.dataId) is None
+    # while somebody holds it, what reads it launches at once
+    z = backend.defer([2000], "float32", Deferred(t.dataId))
+    assert backend.lib.taken() == ["alloc", "a_kernel"] and backend.pending_of(z.dataId) is None
+    g2 = backend.readToGPU(t, 7)
+    g.dispose()
+    assert backend.pending_of(backend.defer([2000], "float32", Deferred(t.dataId)).dataId) is None
+    g2.dispose()
+    assert backend.pending_of(backend.defer([2000], "float32", Deferred(y.dataId)).dataId) is not None

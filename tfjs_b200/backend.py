@@ -104,6 +104,7 @@ class GPUData(object):
                 if self.stream is not None:
                     backend.check(backend.lib.tfjs_cuda_wait_stream(backend.ctx, self.stream))
             finally:
+                backend.gpu_data_released(ref.dataId)
                 if isinstance(ref, TensorInfo):
                     backend.disposeData(ref.dataId)
                 else:
@@ -117,7 +118,8 @@ class GPUData(object):
 
 
 class _Record(object):
-    __slots__ = ("dev", "nbytes", "dtype", "ref", "host", "pending", "held", "foreign", "stream")
+    __slots__ = ("dev", "nbytes", "dtype", "ref", "host", "pending", "held", "foreign", "stream",
+                 "shared")
 
     def __init__(self, dev, nbytes, dtype, ref, host):
         self.dev = dev        # device buffer id, 0 = not uploaded / not launched yet
@@ -129,6 +131,7 @@ class _Record(object):
         self.held = 0         # how many of `ref` belong to pending launches
         self.foreign = None   # the owner of device memory that is not the backend's
         self.stream = None    # the stream its owner works on, if it is to be ordered
+        self.shared = 0       # how many GPUData hold the memory
 
 
 class PendingConv(object):
@@ -524,7 +527,7 @@ class CudaBackend(object):
         self.data = {}        # DataId -> _Record
         self._pinned = []
         self._hidden = 0      # records kept alive only by pending launches
-        self._foreign = 0     # records over memory that is not the backend's
+        self._exposed = 0     # records whose memory others may write: foreign or shared
         self.lazy_fusion = os.environ.get("TFJS_CUDA_NO_LAZY_FUSION", "0") in ("", "0")
         # a pending 3x3 depthwise convolution consumed by a 1x1 convolution runs inside that
         # convolution's launch (TFJS_CUDA_NO_DW_PROJECT=1 keeps the two launches)
@@ -625,7 +628,7 @@ class CudaBackend(object):
         dataId = DataId()
         rec = _Record(self._out_id.value, nbytes, found, 1, None)
         rec.foreign, rec.stream = values, stream
-        self._foreign += 1
+        self._exposed += 1
         self.data[dataId] = rec
         return TensorInfo(dataId, have if shape is None else shape, found)
 
@@ -644,14 +647,26 @@ class CudaBackend(object):
 
     def gpu_data(self, tensor, stream):
         """readToGPU for a reference that the result takes over."""
+        # Whoever holds the memory may write to it: what is pending on its present contents launches
+        # first, and there is no host copy from now on.
+        dev = self.device_id_for_update(tensor.dataId)
         rec = self.data[tensor.dataId]
         ptr = c_void_p()
-        self.check(self.lib.tfjs_cuda_device_ptr(
-            self.ctx, rec.dev or self.device_id(tensor.dataId), byref(ptr)))
+        self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
         if stream is not None:
             self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, stream))
-        rec.host = None        # whoever holds the memory may write to it
+        if rec.shared == 0 and rec.foreign is None:
+            self._exposed += 1
+        rec.shared += 1
         return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream)
+
+    def gpu_data_released(self, dataId):
+        """A GPUData over this tensor has gone."""
+        rec = self.data.get(dataId)
+        if rec is not None and rec.shared:
+            rec.shared -= 1
+            if rec.shared == 0 and rec.foreign is None:
+                self._exposed -= 1
 
     def wait_stream(self, stream):
         """This backend's work from now on runs after what is queued on `stream`."""
@@ -691,10 +706,14 @@ class CudaBackend(object):
                                     if any(self._still_pending_matmul(i) for i in ids)}
             ids = [i for i in self._matmuls_on.get(pending.a, []) if self._still_pending_matmul(i)]
             self._matmuls_on[pending.a] = ids + [dataId]
-        if self._foreign and any(self.data[d].foreign is not None for d in pending.deps()):
-            # its owner may rewrite the memory whenever it likes: what reads it launches now
+        if self._exposed and any(self._is_exposed(self.data[d]) for d in pending.deps()):
+            # somebody else may rewrite the memory at any time: what reads it launches now
             self._resolve(rec)
         return TensorInfo(dataId, shape, dtype)
+
+    @staticmethod
+    def _is_exposed(rec):
+        return rec.foreign is not None or rec.shared > 0
 
     def _still_pending_matmul(self, dataId):
         rec = self.data.get(dataId)
@@ -899,8 +918,9 @@ class CudaBackend(object):
         if rec.pending is not None:
             pending, rec.pending = rec.pending, None
             self._release(pending)
+        if self._is_exposed(rec):
+            self._exposed -= 1
         if rec.foreign is not None:
-            self._foreign -= 1
             if rec.stream is not None:     # its owner's next work waits for what read it here
                 self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream))
 

@@ -20,6 +20,7 @@ interface Record {
   pending?: Pending;   // a deferred launch produces this tensor (pending.ts)
   held: number;        // how many of refCount belong to pending launches that read it
   foreign?: ForeignData;  // the owner of device memory that is not the backend's
+  shared?: boolean;    // its address was handed out
 }
 
 /** Device memory of another library (a WebGPUData-like value: an address instead of a GPUBuffer), and
@@ -41,7 +42,7 @@ export class CudaBackend extends KernelBackend {
   readonly ctx: Ctx;
   private data: DataStorage<Record>;
   private hidden = 0;           // records kept alive only by pending launches
-  private foreign = 0;          // records over memory that is not the backend's
+  private exposed = 0;          // records whose memory others may write: foreign or shared
   private logDepth = 0;
   /** chain signature -> the library has a straight-line kernel for it */
   readonly ewCatalogue = new Map<string, boolean>();
@@ -115,10 +116,12 @@ export class CudaBackend extends KernelBackend {
     this.data.set(dataId, r);
     this.pendingIds.add(dataId);
     if (pending instanceof PendingMatMul) this.noteMatMul(dataId, pending);
-    // the owner of foreign memory may rewrite it whenever it likes: what reads it launches now
-    if (this.foreign > 0 && pending.deps().some(d => this.data.get(d).foreign != null)) this.resolve(r);
+    // somebody else may rewrite the memory at any time: what reads it launches now
+    if (this.exposed > 0 && pending.deps().some(d => this.isExposed(this.data.get(d)))) this.resolve(r);
     return {dataId, shape, dtype};
   }
+
+  private isExposed(r: Record): boolean { return r.foreign != null || r.shared === true; }
 
   pendingOf(t: TensorInfo): Pending|undefined { return this.data.get(t.dataId).pending; }
   pendingOfId(dataId: object): Pending|undefined { return this.data.get(dataId)?.pending; }
@@ -269,15 +272,18 @@ export class CudaBackend extends KernelBackend {
     const id = binding.fromDevice(this.ctx, values.buffer, nbytes);
     const dataId = {};
     this.data.set(dataId, {id, nbytes, dtype, refCount: 1, held: 0, foreign: values});
-    this.foreign++;
+    this.exposed++;
     return {dataId, shape, dtype};
   }
 
-  /** The device address of a tensor (tensor.dataToGPU()); whoever holds it may write to it. */
+  /** The device address of a tensor (tensor.dataToGPU()); whoever holds it may write to it, so what is
+   * pending on its present contents launches first, and what reads it later launches when called. */
   toForeign(t: TensorInfo, stream?: bigint): ForeignData {
-    const buffer = binding.devicePtr(this.ctx, this.deviceId(t));
+    const buffer = binding.devicePtr(this.ctx, this.deviceIdForUpdate(t));
     if (stream != null) binding.signalStream(this.ctx, stream);
-    this.data.get(t.dataId).host = undefined;
+    const r = this.data.get(t.dataId);
+    if (!r.shared && r.foreign == null) this.exposed++;
+    r.shared = true;
     return {buffer, stream};
   }
 
@@ -320,10 +326,8 @@ export class CudaBackend extends KernelBackend {
     this.data.delete(dataId);
     this.pendingIds.delete(dataId);
     if (r.id !== 0) binding.free(this.ctx, r.id);
-    if (r.foreign != null) {
-      this.foreign--;
-      if (r.foreign.stream != null) binding.signalStream(this.ctx, r.foreign.stream);
-    }
+    if (this.isExposed(r)) this.exposed--;
+    if (r.foreign?.stream != null) binding.signalStream(this.ctx, r.foreign.stream);
     if (r.pending != null) {
       const p = r.pending;
       r.pending = undefined;
