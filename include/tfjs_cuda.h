@@ -117,12 +117,17 @@ int tfjs_cuda_sync(tfjs_cuda_ctx* ctx);
 int tfjs_cuda_size_of(tfjs_cuda_ctx* ctx, int32_t id, uint64_t* out_nbytes);
 /* Raw device address of a tensor, for interop (profilers, other libraries).  An upload that is
  * still on its way is waited for on the device: work on a stream that tfjs_cuda_signal_stream is
- * called for afterwards finds it there. */
+ * called for afterwards finds it there.  Who has the address may write there, ordered by the stream calls
+ * below, until it says with one tfjs_cuda_device_ptr_end for each device_ptr that it is done (or frees
+ * the tensor): until then products pack the tensor anew each time, and a captured step that reads
+ * an earlier packed copy is stale. */
 int tfjs_cuda_device_ptr(tfjs_cuda_ctx* ctx, int32_t id, void** out_ptr);
+int tfjs_cuda_device_ptr_end(tfjs_cuda_ctx* ctx, int32_t id);
 /* A tensor over device memory that belongs to the caller (another library's buffer), without
  * a copy: the device half of creating a tensor from GPU data.  `ptr` must be device memory of
  * the context's GPU, 16-byte aligned, and stay valid until the id has been freed and the work
- * that reads it has run (tfjs_cuda_signal_stream orders its next user behind that work).
+ * that reads it has run (tfjs_cuda_signal_stream orders its next user behind that work).  Its owner
+ * may rewrite it between calls; each call reads what is there.
  * tfjs_cuda_free forgets the id and leaves the memory alone; tfjs_cuda_memory does not count
  * its bytes. */
 int tfjs_cuda_from_device(tfjs_cuda_ctx* ctx, void* ptr, uint64_t nbytes, int32_t* out_id);

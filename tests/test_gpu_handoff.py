@@ -91,3 +91,91 @@ def test_what_is_pending_on_a_handed_out_tensor_saw_it_before(cuda_engine):
     for k in (t, y, z, u):
         k.dispose()
     assert backend.numDataIds() == before
+
+
+def _conv(tf, x, f):
+    return tf.conv2d(x, f, 1, "same")
+
+
+@pytest.mark.parametrize("size,channels", [(1, 64), (3, 32), (3, 6)])
+def test_a_foreign_filter_is_read_anew(cuda_engine, size, channels):
+    """A filter whose owner rewrites it: each convolution uses what is there, not a copy that an
+    earlier one made; a captured one as well."""
+    from tfjs_b200 import ops as tf
+    backend = cuda_engine.backend
+    backend.set_math_mode("tf32")
+    r = np.random.default_rng(size + channels)
+    x = tf.tensor(r.standard_normal((2, 14, 14, channels)).astype(np.float32))
+    values = [r.standard_normal((size, size, channels, 64)).astype(np.float32) for _ in range(3)]
+    own = [tf.tensor(v) for v in values]
+    refs = [_conv(tf, x, f) for f in own]
+    want = [t.arraySync() for t in refs]
+    mem = torch.from_numpy(values[0]).cuda()
+    torch.cuda.synchronize()
+    f = tf.tensor(mem)
+    outs = []
+    for i in range(2):
+        mem.copy_(torch.from_numpy(values[i]))
+        torch.cuda.synchronize()
+        outs.append(_conv(tf, x, f))
+        assert np.array_equal(outs[-1].arraySync(), want[i])
+    backend.capture_begin(16 << 20)
+    out = _conv(tf, x, f)
+    backend.device_id(out.dataId)
+    graph = backend.capture_end()
+    for i in (2, 0):
+        mem.copy_(torch.from_numpy(values[i]))
+        torch.cuda.synchronize()
+        backend.graph_launch(graph)
+        assert np.array_equal(out.arraySync(), want[i])
+    backend.graph_destroy(graph)
+    for t in [x, f, out] + own + refs + outs:
+        t.dispose()
+
+
+@pytest.mark.parametrize("product", ["matmul", "conv"])
+def test_a_handed_out_weight_is_read_anew(cuda_engine, product):
+    """A weight that its holder rewrites: products see it, a captured step with the old copy is
+    refused, and once nobody holds it any more one copy serves again."""
+    from tfjs_b200 import _cabi, ops as tf
+    backend = cuda_engine.backend
+    backend.set_math_mode("tf32")
+    r = np.random.default_rng(5)
+    if product == "matmul":
+        a = tf.tensor(r.standard_normal((96, 64)).astype(np.float32))
+        w = tf.tensor(r.standard_normal((64, 128)).astype(np.float32))
+        f = lambda: tf.mat_mul(a, w)                                       # noqa: E731
+    else:
+        a = tf.tensor(r.standard_normal((2, 9, 9, 32)).astype(np.float32))
+        w = tf.tensor(r.standard_normal((3, 3, 32, 64)).astype(np.float32))
+        f = lambda: _conv(tf, a, w)                                        # noqa: E731
+
+    def value():
+        t = f()
+        v = t.arraySync()
+        t.dispose()
+        return v
+    first = value()
+    backend.capture_begin(16 << 20)
+    out = f()
+    backend.device_id(out.dataId)
+    graph = backend.capture_end()
+    g = torch.as_tensor(w.dataToGPU(torch.cuda.current_stream().cuda_stream), device="cuda")
+    with pytest.raises(_cabi.CudaError) as e:
+        backend.graph_launch(graph)
+    assert e.value.code == _cabi.UNSUPPORTED
+    for factor in (2.0, 0.25):                        # powers of two: the products scale exactly
+        g.mul_(factor)
+        torch.cuda.synchronize()
+        first = first * np.float32(factor)
+        assert np.array_equal(value(), first)
+    del g
+    assert np.array_equal(value(), first)
+    backend.launch_log(True)
+    assert np.array_equal(value(), first)
+    log = backend.launch_log_take()
+    backend.launch_log(False)
+    assert log and "pack_weight" not in log
+    backend.graph_destroy(graph)
+    for t in (a, w, out):
+        t.dispose()

@@ -121,3 +121,20 @@ def test_readers_launch_before_an_address_is_handed_out(backend):
     assert backend.pending_of(backend.defer([2000], "float32", Deferred(t.dataId)).dataId) is None
     g2.dispose()
     assert backend.pending_of(backend.defer([2000], "float32", Deferred(y.dataId)).dataId) is not None
+
+
+def test_the_library_is_told_when_nobody_holds_a_tensor_any_more(backend):
+    t = backend.make_output([2000], "float32")
+    g, g2 = backend.readToGPU(t, 7), backend.readToGPU(t)
+    backend.lib.taken()
+    g.dispose()
+    assert backend.lib.taken() == ["wait_stream", "device_ptr_end"]
+    backend.disposeData(t.dataId)
+    g2.dispose()
+    assert backend.lib.taken() == ["free"]
+    t = backend.make_output([2000], "float32")
+    backend.lib.fail["signal_stream"] = 2
+    backend.lib.taken()
+    with pytest.raises(_cabi.CudaError):
+        backend.readToGPU(t, 7)
+    assert backend.lib.taken() == ["device_ptr", "signal_stream", "last_error", "device_ptr_end"]

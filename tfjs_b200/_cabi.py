@@ -96,6 +96,7 @@ SIGNATURES = {
     "tfjs_cuda_sync": (c_int, [_CTX]),
     "tfjs_cuda_size_of": (c_int, [_CTX, c_int32, POINTER(c_uint64)]),
     "tfjs_cuda_device_ptr": (c_int, [_CTX, c_int32, POINTER(c_void_p)]),
+    "tfjs_cuda_device_ptr_end": (c_int, [_CTX, c_int32]),
     "tfjs_cuda_from_device": (c_int, [_CTX, c_void_p, c_uint64, POINTER(c_int32)]),
     "tfjs_cuda_wait_stream": (c_int, [_CTX, c_void_p]),
     "tfjs_cuda_signal_stream": (c_int, [_CTX, c_void_p]),

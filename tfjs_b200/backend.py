@@ -654,7 +654,11 @@ class CudaBackend(object):
         ptr = c_void_p()
         self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
         if stream is not None:
-            self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, stream))
+            try:
+                self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, stream))
+            except CudaError:
+                self.lib.tfjs_cuda_device_ptr_end(self.ctx, dev)
+                raise
         if rec.shared == 0 and rec.foreign is None:
             self._exposed += 1
         rec.shared += 1
@@ -665,6 +669,8 @@ class CudaBackend(object):
         rec = self.data.get(dataId)
         if rec is not None and rec.shared:
             rec.shared -= 1
+            if rec.ref > 1:    # (else the buffer goes as well)
+                self.check(self.lib.tfjs_cuda_device_ptr_end(self.ctx, rec.dev))
             if rec.shared == 0 and rec.foreign is None:
                 self._exposed -= 1
 

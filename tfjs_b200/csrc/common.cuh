@@ -21,6 +21,10 @@ struct Buffer {
   bool uploaded = false;        // block came from tfjs_cuda_upload: recycled for uploads
   bool in_arena = false;        // lives in the arena of a captured graph
   bool foreign = false;         // the caller's memory (tfjs_cuda_from_device): never freed here
+  int held_outside = 0;         // tfjs_cuda_device_ptr calls that tfjs_cuda_device_ptr_end has not ended
+  // Somebody else may write it at any time, and no call says so: a copy of its contents serves one
+  // kernel and not the next.
+  bool exposed() const { return foreign || held_outside > 0; }
 };
 
 // A captured step (tfjs_cuda_capture_begin .. _end): the instantiated graph and the

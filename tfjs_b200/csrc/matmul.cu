@@ -73,13 +73,31 @@ __global__ void im2col_kernel(const float* __restrict__ x, float* __restrict__ c
   }
 }
 
-// Returns the packed copy of weight `id`, building it if needed.
+int pack_into(tfjs_cuda_ctx* ctx, const Buffer* src, float* dst, uint64_t total, int N, int taps, int cin,
+              int cin_pad, int in_is_nk) {
+  if (!total) return TFJS_CUDA_OK;
+  pack_weight_kernel<<<grid_for(total, kThreads, ctx->sm_count), kThreads, 0, ctx->stream>>>(
+      (const float*)src->ptr, dst, total, N, taps, cin, cin_pad, in_is_nk);
+  ctx->launches++;
+  if (ctx->log_launches) ctx->launch_log.push_back("pack_weight_kernel");
+  return ctx_check(ctx, cudaGetLastError(), "pack_weight_kernel");
+}
+
+// Returns the packed copy of weight `id`, building it if needed.  Of memory that somebody else may
+// write the copy is made anew for each call, in the same place, so that a captured step that makes
+// it reads what is there at each replay.
 int get_packed(tfjs_cuda_ctx* ctx, int32_t id, Buffer* src, int batch, int N, int taps,
                int cin, int cin_pad, int in_is_nk, const float** out) {
   const int layout = (taps << 20) ^ (cin_pad << 4) ^ (in_is_nk << 1) ^ (batch << 28) ^ 1;
+  const uint64_t total = (uint64_t)batch * N * taps * cin_pad;
   auto it = ctx->packed.find(id);
-  if (it != ctx->packed.end() && it->second.version == src->version &&
-      it->second.layout == layout && it->second.rows == N) {
+  if (it != ctx->packed.end() && it->second.layout == layout && it->second.rows == N &&
+      (src->exposed() || it->second.version == src->version)) {
+    if (src->exposed()) {
+      const int rc = pack_into(ctx, src, it->second.ptr, total, N, taps, cin, cin_pad, in_is_nk);
+      if (rc) return rc;
+      it->second.version = src->version;
+    }
     if (ctx->capturing) ctx->capture_packed.push_back(id);
     *out = it->second.ptr;
     return TFJS_CUDA_OK;
@@ -87,23 +105,16 @@ int get_packed(tfjs_cuda_ctx* ctx, int32_t id, Buffer* src, int batch, int N, in
   NOT_WHILE_CAPTURING(ctx, "packing a weight tensor");
   ctx_drop_packed(ctx, id);
   PackedWeight pw;
-  const uint64_t total = (uint64_t)batch * N * taps * cin_pad;
   pw.bytes = total * 4;
   CUDA_TRY(ctx, cudaMallocAsync((void**)&pw.ptr, pw.bytes ? pw.bytes : 16, ctx->stream));
   pw.version = src->version;
   pw.rows = N;
   pw.k_pad = taps * cin_pad;
   pw.layout = layout;
-  if (total) {
-    pack_weight_kernel<<<grid_for(total, kThreads, ctx->sm_count), kThreads, 0, ctx->stream>>>(
-        (const float*)src->ptr, pw.ptr, total, N, taps, cin, cin_pad, in_is_nk);
-    ctx->launches++;
-    if (ctx->log_launches) ctx->launch_log.push_back("pack_weight_kernel");
-    int rc = ctx_check(ctx, cudaGetLastError(), "pack_weight_kernel");
-    if (rc) {
-      cudaFreeAsync(pw.ptr, ctx->stream);
-      return rc;
-    }
+  const int rc = pack_into(ctx, src, pw.ptr, total, N, taps, cin, cin_pad, in_is_nk);
+  if (rc) {
+    cudaFreeAsync(pw.ptr, ctx->stream);
+    return rc;
   }
   ctx->packed[id] = pw;
   *out = pw.ptr;

@@ -343,6 +343,7 @@ int tfjs_cuda_free(tfjs_cuda_ctx* ctx, int32_t id) {
   if (ctx->capturing && (b->ready || ctx->packed.count(id)))
     NOT_WHILE_CAPTURING(ctx, "freeing a weight or a tensor whose upload is pending");
   ctx_drop_packed(ctx, id);
+  b->held_outside = 0;
   if (b->ready) {  // never used since its upload: still order the free behind the copy
     cudaStreamWaitEvent(ctx->stream, b->ready, 0);
     ctx->event_pool.push_back(b->ready);
@@ -676,7 +677,23 @@ int tfjs_cuda_device_ptr(tfjs_cuda_ctx* ctx, int32_t id, void** out_ptr) {
     const int rc = ctx_get(ctx, id, 0, "device_ptr", &b);
     if (rc) return rc;
   }
+  if (ctx->capturing)
+    for (int32_t w : ctx->capture_packed)
+      if (w == id) NOT_WHILE_CAPTURING(ctx, "handing out a weight that the step reads a copy of");
+  // captured steps that read a packed copy of it would not see what the holder writes
+  ctx_packed_contents_changed(ctx, id);
+  b->held_outside++;
   *out_ptr = b->ptr;
+  return TFJS_CUDA_OK;
+}
+
+int tfjs_cuda_device_ptr_end(tfjs_cuda_ctx* ctx, int32_t id) {
+  if (!ctx) return TFJS_CUDA_INVALID_ARG;
+  Buffer* b = ctx_buf(ctx, id);
+  if (!b) return ctx_fail(ctx, TFJS_CUDA_UNKNOWN_ID, "device_ptr_end: unknown tensor id %d", id);
+  if (b->held_outside == 0)
+    return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "device_ptr_end: nobody holds tensor id %d", id);
+  if (--b->held_outside == 0) b->version++;   // the next packed copy is made of what is there now
   return TFJS_CUDA_OK;
 }
 
@@ -707,7 +724,7 @@ int tfjs_cuda_from_device(tfjs_cuda_ctx* ctx, void* ptr, uint64_t nbytes, int32_
   b.ptr = ptr;
   b.bytes = nbytes;
   b.live = true;
-  b.from_host = false;   // its owner may rewrite it at any time: never packed once and kept
+  b.from_host = false;   // not a weight: products read it as it lies
   b.foreign = true;
   b.version++;
   ctx->n_live++;

@@ -396,6 +396,10 @@ napi_value DevicePtr(napi_env env, napi_callback_info info) {
   check(env, a.ctx(0), tfjs_cuda_device_ptr(a.ctx(0), a.i32(1), &p));
   napi_value r; napi_create_bigint_uint64(env, (uint64_t)(uintptr_t)p, &r); return r;
 }
+napi_value DevicePtrEnd(napi_env env, napi_callback_info info) {
+  Args a(env, info);
+  return check(env, a.ctx(0), tfjs_cuda_device_ptr_end(a.ctx(0), a.i32(1)));
+}
 napi_value Trim(napi_env env, napi_callback_info info) {
   Args a(env, info); return check(env, a.ctx(0), tfjs_cuda_trim(a.ctx(0)));
 }
@@ -485,7 +489,7 @@ napi_value Init(napi_env env, napi_value exports) {
       {"cast", Cast}, {"copyStrided", CopyStrided}, {"fill", Fill}, {"batchNorm", BatchNorm},
       {"dequantize", Dequantize}, {"dequantizeStatic", DequantizeStatic},
       {"batchNormRows", BatchNormRows}, {"deviceCount", DeviceCount}, {"upload", Upload},
-      {"readAsync", ReadAsync}, {"sizeOf", SizeOf}, {"devicePtr", DevicePtr}, {"trim", Trim},
+      {"readAsync", ReadAsync}, {"sizeOf", SizeOf}, {"devicePtr", DevicePtr}, {"devicePtrEnd", DevicePtrEnd}, {"trim", Trim},
       {"hostAlloc", HostAlloc}, {"hostFree", HostFree}, {"eventRecord", EventRecord},
       {"eventElapsed", EventElapsed}, {"launchCount", LaunchCount}, {"launchLog", LaunchLog},
       {"launchLogTake", LaunchLogTake}, {"flushL2", FlushL2}, {"weightsBegin", WeightsBegin},

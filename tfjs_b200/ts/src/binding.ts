@@ -108,6 +108,7 @@ export interface CudaBinding {
   readAsync(ctx: Ctx, id: number, out: ArrayBufferView, nbytes: number): void;
   sizeOf(ctx: Ctx, id: number): number;
   devicePtr(ctx: Ctx, id: number): bigint;
+  devicePtrEnd(ctx: Ctx, id: number): void;
   trim(ctx: Ctx): void;
   hostAlloc(ctx: Ctx, nbytes: number): ArrayBuffer;
   hostFree(ctx: Ctx, buffer: ArrayBuffer): void;
