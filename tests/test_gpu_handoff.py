@@ -179,3 +179,45 @@ def test_a_handed_out_weight_is_read_anew(cuda_engine, product):
     backend.graph_destroy(graph)
     for t in (a, w, out):
         t.dispose()
+
+
+def test_a_holder_that_goes_away_during_a_capture(cuda_engine):
+    """Neither side's capture is disturbed, and the memory is used again only behind the holder's work."""
+    from tfjs_b200 import ops as tf
+    backend = cuda_engine.backend
+    before = backend.numDataIds()
+    side = torch.cuda.Stream()
+    n = 1 << 22
+    x = tf.tensor(np.arange(n, dtype=np.float32))
+    y = tf.tensor(np.full(5000, 2.0, np.float32))
+    g = torch.as_tensor(x.dataToGPU(side.cuda_stream), device="cuda")
+    x.dispose()
+    with torch.cuda.stream(side):
+        total = torch.zeros((), device="cuda", dtype=torch.float64)
+        for _ in range(20):
+            total += g.double().sum()
+    backend.capture_begin(1 << 20)
+    del g
+    z = tf.mul(y, y)
+    backend.device_id(z.dataId)
+    graph = backend.capture_end()
+    w = tf.tensor(np.zeros(n, np.float32))             # of the same size: may take that block
+    backend.graph_launch(graph)
+    assert np.all(z.arraySync() == 4.0)
+    with torch.cuda.stream(side):
+        assert total.item() == 20 * (float(n) * (n - 1) / 2)
+    # the holder captures a graph of its own on that stream
+    g = torch.as_tensor(w.dataToGPU(side.cuda_stream), device="cuda")
+    w.dispose()
+    torch.cuda.synchronize()
+    theirs = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(theirs, stream=side):
+        total += 1.0
+        del g
+    assert backend.numDataIds() == before + 3          # y, z, and what w held
+    backend.sync()
+    assert backend.numDataIds() == before + 2
+    backend.graph_destroy(graph)
+    for t in (y, z):
+        t.dispose()
+    assert backend.numDataIds() == before

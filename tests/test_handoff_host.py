@@ -138,3 +138,43 @@ def test_the_library_is_told_when_nobody_holds_a_tensor_any_more(backend):
     with pytest.raises(_cabi.CudaError):
         backend.readToGPU(t, 7)
     assert backend.lib.taken() == ["device_ptr", "signal_stream", "last_error", "device_ptr_end"]
+
+
+def test_memory_is_kept_until_its_holders_stream_can_be_waited_for(backend):
+    """Not freed in front of the holder's work: not during a capture, which the wait would discard, and
+    not while the holder's own stream is being captured."""
+    t, u = backend.make_output([2000], "float32"), backend.make_output([2000], "float32")
+    held = [backend.readToGPU(x, 7) for x in (t, u)]
+    for x in (t, u):
+        backend.disposeData(x.dataId)
+    backend.capture_begin(1 << 20)
+    backend.lib.taken()
+    held.pop().dispose()
+    assert backend.lib.taken() == [] and backend.lib.freed == []
+    backend.capture_end()
+    assert backend.lib.taken() == ["capture_end", "wait_stream", "free"]
+    backend.lib.fail["wait_stream"] = _cabi.UNSUPPORTED
+    held.pop().dispose()
+    assert len(backend.lib.freed) == 1
+    del backend.lib.fail["wait_stream"]
+    backend.lib.taken()
+    backend.sync()
+    assert backend.lib.taken() == ["wait_stream", "free", "sync"] and backend.numDataIds() == 0
+    # a capture that ends badly, and one that never began
+    v = backend.make_output([2000], "float32")
+    g = backend.readToGPU(v, 7)
+    backend.disposeData(v.dataId)
+    backend.capture_begin(1 << 20)
+    g.dispose()
+    backend.lib.fail["capture_end"] = 2
+    with pytest.raises(_cabi.CudaError):
+        backend.capture_end()
+    assert backend.numDataIds() == 0
+    backend.lib.fail["capture_begin"] = 2
+    with pytest.raises(_cabi.CudaError):
+        backend.capture_begin(1 << 20)
+    w = backend.make_output([2000], "float32")
+    g = backend.readToGPU(w, 7)
+    backend.disposeData(w.dataId)
+    g.dispose()
+    assert backend.numDataIds() == 0

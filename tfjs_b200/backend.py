@@ -97,18 +97,11 @@ class GPUData(object):
                 "data": (self.buffer, False), "strides": None, "version": 2}
 
     def dispose(self):
+        """Releases the tensor, behind the work on `stream`; where that stream cannot be waited
+        for now (a step of either side is being captured), as soon as it can."""
         ref, self.tensorRef = self.tensorRef, None
-        backend = self.backend
-        if ref is not None and backend.ctx:
-            try:
-                if self.stream is not None:
-                    backend.check(backend.lib.tfjs_cuda_wait_stream(backend.ctx, self.stream))
-            finally:
-                backend.gpu_data_released(ref.dataId)
-                if isinstance(ref, TensorInfo):
-                    backend.disposeData(ref.dataId)
-                else:
-                    ref.dispose()
+        if ref is not None and self.backend.ctx:
+            self.backend.release_gpu_data(ref, self.stream)
 
     def __del__(self):
         try:
@@ -527,6 +520,8 @@ class CudaBackend(object):
         self.data = {}        # DataId -> _Record
         self._pinned = []
         self._hidden = 0      # records kept alive only by pending launches
+        self._capturing = False
+        self._unreleased = [] # (tensor, stream) of GPUData that are gone while it could not be waited for
         self._exposed = 0     # records whose memory others may write: foreign or shared
         self.lazy_fusion = os.environ.get("TFJS_CUDA_NO_LAZY_FUSION", "0") in ("", "0")
         # a pending 3x3 depthwise convolution consumed by a 1x1 convolution runs inside that
@@ -647,6 +642,8 @@ class CudaBackend(object):
 
     def gpu_data(self, tensor, stream):
         """readToGPU for a reference that the result takes over."""
+        if self._unreleased:
+            self._release_gpu_data()
         # Whoever holds the memory may write to it: what is pending on its present contents launches
         # first, and there is no host copy from now on.
         dev = self.device_id_for_update(tensor.dataId)
@@ -664,18 +661,42 @@ class CudaBackend(object):
         rec.shared += 1
         return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream)
 
-    def gpu_data_released(self, dataId):
-        """A GPUData over this tensor has gone."""
-        rec = self.data.get(dataId)
-        if rec is not None and rec.shared:
-            rec.shared -= 1
-            if rec.ref > 1:    # (else the buffer goes as well)
-                self.check(self.lib.tfjs_cuda_device_ptr_end(self.ctx, rec.dev))
-            if rec.shared == 0 and rec.foreign is None:
-                self._exposed -= 1
+    def release_gpu_data(self, ref, stream):
+        """Disposes the tensor that a GPUData held, behind the work on its holder's stream.  Its memory
+        must not be used again before that, so a wait that is refused is tried again later."""
+        self._unreleased.append((ref, stream))
+        self._release_gpu_data()
+
+    def _release_gpu_data(self):
+        if self._capturing:       # (the library would refuse the wait and discard the capture)
+            return
+        todo, self._unreleased = self._unreleased, []
+        while todo:
+            ref, stream = todo.pop(0)
+            if stream is not None and \
+                    self.lib.tfjs_cuda_wait_stream(self.ctx, stream) != _cabi.OK:
+                self._unreleased.append((ref, stream))
+                continue
+            try:
+                rec = self.data.get(ref.dataId)
+                if rec is not None and rec.shared:
+                    rec.shared -= 1
+                    if rec.ref > 1:    # (else the buffer goes as well)
+                        self.check(self.lib.tfjs_cuda_device_ptr_end(self.ctx, rec.dev))
+                    if rec.shared == 0 and rec.foreign is None:
+                        self._exposed -= 1
+                if isinstance(ref, TensorInfo):
+                    self.disposeData(ref.dataId)
+                else:
+                    ref.dispose()
+            except Exception:
+                self._unreleased.extend(todo)
+                raise
 
     def wait_stream(self, stream):
         """This backend's work from now on runs after what is queued on `stream`."""
+        if self._unreleased:
+            self._release_gpu_data()
         self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, int(stream)))
 
     def signal_stream(self, stream):
@@ -1001,6 +1022,8 @@ class CudaBackend(object):
         return True
 
     def sync(self):
+        if self._unreleased:
+            self._release_gpu_data()
         self.check(self.lib.tfjs_cuda_sync(self.ctx))
 
     def set_math_mode(self, mode):
@@ -1021,12 +1044,18 @@ class CudaBackend(object):
 
     def capture_begin(self, arena_bytes):
         self.check(self.lib.tfjs_cuda_capture_begin(self.ctx, int(arena_bytes)))
+        self._capturing = True
 
     def capture_end(self, abandon=False):
         """Graph id of the captured step; raises CudaError (UNSUPPORTED) when the capture
         had to be discarded."""
         graph = c_int32()
-        self.check(self.lib.tfjs_cuda_capture_end(self.ctx, 1 if abandon else 0, byref(graph)))
+        try:
+            self.check(self.lib.tfjs_cuda_capture_end(self.ctx, 1 if abandon else 0, byref(graph)))
+        finally:
+            self._capturing = False
+            if self._unreleased:
+                self._release_gpu_data()
         return graph.value
 
     def graph_launch(self, graph):
