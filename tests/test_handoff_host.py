@@ -178,3 +178,19 @@ def test_memory_is_kept_until_its_holders_stream_can_be_waited_for(backend):
     backend.disposeData(w.dataId)
     g.dispose()
     assert backend.numDataIds() == 0
+
+
+def test_foreign_memory_is_referenced_until_its_owners_stream_can_be_signalled(backend):
+    import sys
+    memory = Memory()
+    count = sys.getrefcount(memory)
+    t = backend.createTensorFromGPUData(memory, stream=7)
+    backend.lib.fail["signal_stream"] = _cabi.UNSUPPORTED       # (its owner captures a graph there)
+    backend.disposeData(t.dataId)
+    assert backend.numDataIds() == 0 and sys.getrefcount(memory) > count
+    backend.sync()
+    assert sys.getrefcount(memory) > count
+    del backend.lib.fail["signal_stream"]
+    backend.lib.taken()
+    backend.sync()
+    assert backend.lib.taken() == ["signal_stream", "sync"] and sys.getrefcount(memory) == count

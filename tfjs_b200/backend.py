@@ -521,7 +521,8 @@ class CudaBackend(object):
         self._pinned = []
         self._hidden = 0      # records kept alive only by pending launches
         self._capturing = False
-        self._unreleased = [] # (tensor, stream) of GPUData that are gone while it could not be waited for
+        self._unreleased = []   # (tensor, stream) of GPUData that went while it could not be waited for
+        self._unsignalled = []  # (foreign memory, stream) of tensors that are gone, likewise
         self._exposed = 0     # records whose memory others may write: foreign or shared
         self.lazy_fusion = os.environ.get("TFJS_CUDA_NO_LAZY_FUSION", "0") in ("", "0")
         # a pending 3x3 depthwise convolution consumed by a 1x1 convolution runs inside that
@@ -642,7 +643,7 @@ class CudaBackend(object):
 
     def gpu_data(self, tensor, stream):
         """readToGPU for a reference that the result takes over."""
-        if self._unreleased:
+        if self._unreleased or self._unsignalled:
             self._release_gpu_data()
         # Whoever holds the memory may write to it: what is pending on its present contents launches
         # first, and there is no host copy from now on.
@@ -670,6 +671,9 @@ class CudaBackend(object):
     def _release_gpu_data(self):
         if self._capturing:       # (the library would refuse the wait and discard the capture)
             return
+        self._unsignalled = [
+            (memory, stream) for memory, stream in self._unsignalled
+            if self.lib.tfjs_cuda_signal_stream(self.ctx, stream) != _cabi.OK]
         todo, self._unreleased = self._unreleased, []
         while todo:
             ref, stream = todo.pop(0)
@@ -695,7 +699,7 @@ class CudaBackend(object):
 
     def wait_stream(self, stream):
         """This backend's work from now on runs after what is queued on `stream`."""
-        if self._unreleased:
+        if self._unreleased or self._unsignalled:
             self._release_gpu_data()
         self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, int(stream)))
 
@@ -947,9 +951,13 @@ class CudaBackend(object):
             self._release(pending)
         if self._is_exposed(rec):
             self._exposed -= 1
-        if rec.foreign is not None:
-            if rec.stream is not None:     # its owner's next work waits for what read it here
-                self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream))
+        if rec.stream is not None:     # its owner's next work waits for what read it here
+            rc = self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream)
+            if rc == _cabi.UNSUPPORTED and not self._capturing:
+                # its owner is capturing on that stream: the memory stays referenced until it is not
+                self._unsignalled.append((rec.foreign, rec.stream))
+            else:                      # (a capture began behind all work that read it)
+                self.check(rc)
 
     def refCount(self, dataId):
         rec = self.data.get(dataId)
@@ -1022,7 +1030,7 @@ class CudaBackend(object):
         return True
 
     def sync(self):
-        if self._unreleased:
+        if self._unreleased or self._unsignalled:
             self._release_gpu_data()
         self.check(self.lib.tfjs_cuda_sync(self.ctx))
 
@@ -1054,7 +1062,7 @@ class CudaBackend(object):
             self.check(self.lib.tfjs_cuda_capture_end(self.ctx, 1 if abandon else 0, byref(graph)))
         finally:
             self._capturing = False
-            if self._unreleased:
+            if self._unreleased or self._unsignalled:
                 self._release_gpu_data()
         return graph.value
 
@@ -1104,6 +1112,7 @@ class CudaBackend(object):
             self.lib.tfjs_cuda_destroy(self.ctx)
             self.ctx = None
             self.data = {}
+            self._unreleased, self._unsignalled = [], []
 
     def __del__(self):
         try:
