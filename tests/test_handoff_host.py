@@ -194,3 +194,30 @@ def test_foreign_memory_is_referenced_until_its_owners_stream_can_be_signalled(b
     backend.lib.taken()
     backend.sync()
     assert backend.lib.taken() == ["signal_stream", "sync"] and sys.getrefcount(memory) == count
+
+
+def test_read_only_memory_and_the_interfaces_own_stream(backend):
+    from tfjs_b200.kernels import decoder
+    waited = []
+    plain = backend.lib.tfjs_cuda_wait_stream
+    backend.lib.tfjs_cuda_wait_stream = lambda ctx, stream: waited.append(stream) or plain(ctx, stream)
+    pool = [9, 2, 16, 64]
+    kc = backend.createTensorFromGPUData(Memory(pool, read_only=True, stream=5))
+    assert waited == [5]
+    vc = backend.createTensorFromGPUData(Memory(pool, stream=None))
+    backend.createTensorFromGPUData(Memory(pool, stream=1), stream=9)
+    assert waited == [5, 9]
+    make = lambda shape, dtype="float32": backend.make_output(shape, dtype)     # noqa: E731
+    inp = {"kCache": kc, "vCache": vc, "pageTable": make([3, 4], "int32"), "lengths": make([3], "int32"),
+           "k": make([3, 2, 1, 64]), "v": make([3, 2, 1, 64]), "weights": make([3, 2, 64])}
+    backend.lib.taken()
+    for kernel, attrs in ((decoder._paged_cache_append, {}), (decoder._paged_cache_evict, {"budget": 8})):
+        for names in (("kCache", "vCache"), ("vCache", "kCache")):
+            pools = dict(zip(names, (kc, vc)))
+            with pytest.raises(ValueError, match="read-only"):
+                kernel({"backend": backend, "inputs": dict(inp, **pools), "attrs": attrs})
+    assert not [c for c in backend.lib.taken() if c.startswith("paged")]
+    inp["q"] = make([3, 4, 1, 64])
+    decoder._paged_attention({"backend": backend, "inputs": dict(inp, weights=None), "attrs": {}})
+    g, h = backend.readToGPU(kc), backend.readToGPU(vc)
+    assert g.__cuda_array_interface__["data"][1] is True and h.__cuda_array_interface__["data"][1] is False

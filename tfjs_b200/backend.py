@@ -83,18 +83,18 @@ class GPUData(object):
     `buffer` is the address, `bufSize` its bytes, `tensorRef` a tensor that keeps it alive.
     Libraries that read __cuda_array_interface__ take it without a copy.  When the last
     reference is gone that tensor is disposed, behind the work queued on `stream` by then."""
-    __slots__ = ("backend", "tensorRef", "buffer", "bufSize", "stream")
+    __slots__ = ("backend", "tensorRef", "buffer", "bufSize", "stream", "read_only")
     _TYPESTR = {"float32": "<f4", "int32": "<i4", "bool": "|b1"}
 
-    def __init__(self, backend, tensorRef, buffer, bufSize, stream):
+    def __init__(self, backend, tensorRef, buffer, bufSize, stream, read_only):
         self.backend, self.tensorRef, self.stream = backend, tensorRef, stream
-        self.buffer, self.bufSize = buffer, bufSize
+        self.buffer, self.bufSize, self.read_only = buffer, bufSize, read_only
 
     @property
     def __cuda_array_interface__(self):
         t = self.tensorRef
         return {"shape": tuple(t.shape), "typestr": self._TYPESTR[t.dtype],
-                "data": (self.buffer, False), "strides": None, "version": 2}
+                "data": (self.buffer, self.read_only), "strides": None, "version": 2}
 
     def dispose(self):
         """Releases the tensor, behind the work on `stream`; where that stream cannot be waited
@@ -112,7 +112,7 @@ class GPUData(object):
 
 class _Record(object):
     __slots__ = ("dev", "nbytes", "dtype", "ref", "host", "pending", "held", "foreign", "stream",
-                 "shared")
+                 "shared", "read_only")
 
     def __init__(self, dev, nbytes, dtype, ref, host):
         self.dev = dev        # device buffer id, 0 = not uploaded / not launched yet
@@ -125,6 +125,7 @@ class _Record(object):
         self.foreign = None   # the owner of device memory that is not the backend's
         self.stream = None    # the stream its owner works on, if it is to be ordered
         self.shared = 0       # how many GPUData hold the memory
+        self.read_only = False  # foreign memory that its owner does not let others write
 
 
 class PendingConv(object):
@@ -599,7 +600,9 @@ class CudaBackend(object):
         float32, int32 or bool memory of this GPU.  `stream` (a cudaStream_t as a number, 0 = the
         default stream): this backend's work waits for what is queued there now, and what is
         queued there after the tensor is disposed waits for this backend's work.  Without it
-        the caller orders the two."""
+        the caller orders the two; what is queued on a stream that the interface itself names is
+        waited for.  Memory that the interface says is read-only is refused where a kernel would
+        write to it."""
         info = interface if interface is not None else values.__cuda_array_interface__
         found, step = _FOREIGN_TYPES.get(info["typestr"], (None, 0))
         if found is None or (dtype is not None and dtype != found):
@@ -617,13 +620,16 @@ class CudaBackend(object):
                 step *= d
         if shape is not None and size_from_shape(shape) != n:
             raise ValueError("createTensorFromGPUData: %d values for shape %s" % (n, list(shape)))
-        if stream is not None:
-            self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, stream))
+        # (the interface's numbers for the legacy and the per-thread default stream, 1 and 2, are the
+        # handles that CUDA has for them)
+        before = stream if stream is not None else info.get("stream")
+        if before is not None:
+            self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, before))
         self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes,
                                                   self._out_id_ref))
         dataId = DataId()
         rec = _Record(self._out_id.value, nbytes, found, 1, None)
-        rec.foreign, rec.stream = values, stream
+        rec.foreign, rec.stream, rec.read_only = values, stream, bool(info["data"][1])
         self._exposed += 1
         self.data[dataId] = rec
         return TensorInfo(dataId, have if shape is None else shape, found)
@@ -645,10 +651,10 @@ class CudaBackend(object):
         """readToGPU for a reference that the result takes over."""
         if self._unreleased or self._unsignalled:
             self._release_gpu_data()
+        rec = self.data[tensor.dataId]
         # Whoever holds the memory may write to it: what is pending on its present contents launches
         # first, and there is no host copy from now on.
-        dev = self.device_id_for_update(tensor.dataId)
-        rec = self.data[tensor.dataId]
+        dev = self.device_id(tensor.dataId) if rec.read_only else self.device_id_for_update(tensor.dataId)
         ptr = c_void_p()
         self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
         if stream is not None:
@@ -660,7 +666,7 @@ class CudaBackend(object):
         if rec.shared == 0 and rec.foreign is None:
             self._exposed += 1
         rec.shared += 1
-        return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream)
+        return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream, rec.read_only)
 
     def release_gpu_data(self, ref, stream):
         """Disposes the tensor that a GPUData held, behind the work on its holder's stream.  Its memory
@@ -870,6 +876,8 @@ class CudaBackend(object):
         """Device buffer id of a tensor that a kernel is about to write in place: launches
         that are pending on its present contents happen first, and a host copy is dropped."""
         rec = self.data[dataId]
+        if rec.read_only:
+            raise ValueError("the memory of this tensor is read-only")
         self._launch_readers(dataId, rec)
         dev = self.device_id(dataId)
         rec.host = None
