@@ -221,3 +221,19 @@ def test_a_holder_that_goes_away_during_a_capture(cuda_engine):
     for t in (y, z):
         t.dispose()
     assert backend.numDataIds() == before
+
+
+def test_a_copy_over_a_small_tensor(cuda_engine):
+    """backend.copy, which hands a captured step's results to its next replay: a small tensor written
+    from the host reads as the copy left it, and what is pending on the old contents saw those."""
+    from tfjs_b200 import ops as tf
+    backend = cuda_engine.backend
+    t, s = tf.tensor(np.array([1, 2, 3], np.int32)), tf.tensor(np.array([7, 8, 9], np.int32))
+    backend.copy(s.dataId, t.dataId)
+    assert list(t.arraySync()) == [7, 8, 9] and list(s.arraySync()) == [7, 8, 9]
+    x, y = tf.tensor(np.full(5000, 1.0, np.float32)), tf.tensor(np.full(5000, 4.0, np.float32))
+    z = tf.add(x, x)
+    backend.copy(y.dataId, x.dataId)
+    assert np.all(z.arraySync() == 2.0) and np.all(x.arraySync() == 4.0)
+    for k in (t, s, x, y, z):
+        k.dispose()

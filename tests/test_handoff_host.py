@@ -3,7 +3,7 @@ stand-in for the library that records the calls."""
 import pytest
 
 from tfjs_b200 import _cabi
-from tfjs_b200.backend import CudaBackend
+from tfjs_b200.backend import CudaBackend, TensorInfo
 
 
 class Library(object):
@@ -221,3 +221,17 @@ def test_read_only_memory_and_the_interfaces_own_stream(backend):
     decoder._paged_attention({"backend": backend, "inputs": dict(inp, weights=None), "attrs": {}})
     g, h = backend.readToGPU(kc), backend.readToGPU(vc)
     assert g.__cuda_array_interface__["data"][1] is True and h.__cuda_array_interface__["data"][1] is False
+
+
+def test_a_copy_writes_its_destination(backend):
+    import numpy as np
+    src, dst = backend.make_output([2], "float32"), TensorInfo(backend.write(np.zeros(2), [2], "float32"), [2], "float32")
+    y = backend.defer([2], "float32", Deferred(dst.dataId))
+    backend.lib.taken()
+    backend.copy(src.dataId, dst.dataId)
+    assert backend.lib.taken() == ["alloc", "a_kernel", "alloc", "write", "copy"]
+    assert backend.pending_of(y.dataId) is None and backend.host_values(dst.dataId) is None
+    backend.copy(src.dataId, src.dataId)
+    locked = backend.createTensorFromGPUData(Memory((2,), read_only=True))
+    with pytest.raises(ValueError, match="read-only"):
+        backend.copy(src.dataId, locked.dataId)

@@ -1055,8 +1055,9 @@ class CudaBackend(object):
     def copy(self, src_dataId, dst_dataId):
         """Device-to-device copy of a whole tensor, in stream order."""
         nbytes = self.data[src_dataId].nbytes
-        self.check(self.lib.tfjs_cuda_copy(self.ctx, self.device_id(src_dataId),
-                                           self.device_id(dst_dataId), nbytes))
+        src = self.device_id(src_dataId)
+        dst = self.device_id_for_update(dst_dataId) if src_dataId is not dst_dataId else src
+        self.check(self.lib.tfjs_cuda_copy(self.ctx, src, dst, nbytes))
 
     def capture_begin(self, arena_bytes):
         self.check(self.lib.tfjs_cuda_capture_begin(self.ctx, int(arena_bytes)))
