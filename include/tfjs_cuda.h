@@ -471,6 +471,8 @@ int tfjs_cuda_fused_attention(tfjs_cuda_ctx* ctx, int32_t q_id, int32_t k_id, in
  * A page number outside [0, num_pages) that a call needs and a length outside [0, capacity]
  * are skipped on the device (the slots of such a page count as absent, the length is clamped)
  * and reported by the next blocking call (read, read_wait, sync) as TFJS_CUDA_INVALID_ARG.
+ * A tensor that a call writes must lie apart from every other tensor of the call (tensors over memory of
+ * the caller's need not); a call where it does not is refused.
  * No counterpart in the reference's kernel set. */
 typedef struct tfjs_cuda_paged_params {
   int32_t batch, heads, kv_heads, head_dim; /* heads: attention only, a multiple of kv_heads */

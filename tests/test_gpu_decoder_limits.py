@@ -22,3 +22,39 @@ def test_evict_around_the_shared_memory_steps(tf, slots, dim):
     got = run_evict(tf, cache, w, 60, 20)
     for a, b in zip(got, ref):
         assert a.dtype == b.dtype and np.array_equal(a, b, equal_nan=a.dtype == np.float32)
+
+
+def test_memory_that_a_call_writes_is_its_own(tf, cuda_engine):
+    """Tensors over one piece of memory have ids of their own: two pools in one place, new rows inside a
+    pool, or overlapping pools are refused, and neighbours are not."""
+    import torch
+    from tfjs_b200 import _cabi
+    x = torch.zeros(4 * 2 * 8 * 16 * 2, device="cuda")
+    n = 4 * 2 * 8 * 16
+    torch.cuda.synchronize()
+
+    def view(at, *shape):
+        return tf.tensor(x[at:at + int(np.prod(shape))].view(*shape))
+    kc, vc = view(0, 4, 2, 8, 16), view(n, 4, 2, 8, 16)
+    same, over = view(0, 4, 2, 8, 16), view(n // 2, 4, 2, 8, 16)
+    table, lengths = tf.tensor(np.array([[0, 1]], np.int32)), tf.tensor(np.array([3], np.int32))
+    k = tf.tensor(np.ones((1, 2, 1, 16), np.float32))
+    inside = view(n - 32, 1, 2, 1, 16)
+    w = tf.tensor(np.zeros((1, 2, 16), np.float32))
+    w_inside = view(n, 1, 2, 16)
+    q = tf.tensor(np.ones((1, 2, 1, 16), np.float32))
+    for bad in (lambda: tf.paged_cache_append(kc, same, k, k, table, lengths),
+                lambda: tf.paged_cache_append(kc, over, k, k, table, lengths),
+                lambda: tf.paged_cache_append(kc, vc, inside, k, table, lengths),
+                lambda: tf.paged_cache_append(kc, vc, k, inside, table, lengths),
+                lambda: tf.paged_cache_evict(kc, over, w, table, lengths, 2),
+                lambda: tf.paged_cache_evict(kc, vc, w_inside, table, lengths, 2)):
+        with pytest.raises(_cabi.CudaError) as e:
+            bad()
+        assert e.value.code == 1
+    outs = [tf.paged_cache_append(kc, vc, k, k, table, lengths)]
+    outs.append(tf.paged_attention(q, kc, vc, table, outs[0]))
+    outs.append(tf.paged_attention(q, kc, same, table, outs[0]))     # (nothing is written to the pools)
+    for t in outs + [kc, vc, same, over, table, lengths, k, inside, w, w_inside, q]:
+        t.dispose()
+    assert float(x.sum()) == 2 * 2 * 16

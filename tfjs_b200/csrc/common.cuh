@@ -157,6 +157,18 @@ struct TempBuffer {
     return rc;
   }
 };
+// Device memory that a call uses.  Tensors over memory of the caller's can lie in one another, so that
+// ids alone do not tell whether what a call writes is apart from what else it uses.
+struct Span {
+  const void* ptr;
+  uint64_t bytes;
+  bool meets(const Span& o) const {
+    return bytes && o.bytes && (uintptr_t)ptr < (uintptr_t)o.ptr + o.bytes && (uintptr_t)o.ptr < (uintptr_t)ptr + bytes;
+  }
+};
+// Refuses a call (INVALID_ARG) when a tensor that it writes (the first `n_written` of `spans`) overlaps
+// another one that it writes or reads; absent tensors have no bytes.
+int ctx_apart(tfjs_cuda_ctx* ctx, const char* who, const Span* spans, int n, int n_written);
 void ctx_mark_written(tfjs_cuda_ctx* ctx, int32_t id);
 void ctx_drop_packed(tfjs_cuda_ctx* ctx, int32_t id);
 // Marks captured steps that read the packed copy of weight `id` as stale (no memory call).

@@ -132,6 +132,10 @@ extern "C" int tfjs_cuda_linear_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_li
       return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is also an input", who);
   if (out_id == out_state_id)
     return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is given twice", who);
+  const Span spans[] = {{out->ptr, tokens * p->dim_v * 4}, {os->ptr, st}, {q->ptr, tokens * p->dim_k * 4},
+                        {k->ptr, tokens * p->dim_k * 4}, {v->ptr, tokens * p->dim_v * 4}, {d->ptr, (uint64_t)p->heads * 4},
+                        {s ? s->ptr : nullptr, s ? st : 0}, {n ? n->ptr : nullptr, n ? (uint64_t)p->batch * 4 : 0}};
+  if ((rc = ctx_apart(ctx, who, spans, 8, 2))) return rc;
   LinearArgs a;
   a.q = (const float*)q->ptr;
   a.k = (const float*)k->ptr;

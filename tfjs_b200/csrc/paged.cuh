@@ -14,6 +14,7 @@ struct PagedLayout {
   int page_shift;       // log2(page_size), or -1
   int capacity;         // max_pages * page_size
   int* flag;            // the context's error word
+  uint64_t pool_bytes;  // of each pool
 };
 
 // Slots of row b, clamped to [0, capacity]; a length outside that is reported.
@@ -63,6 +64,7 @@ int paged_layout(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params* p, const char
   if ((rc = ctx_get(ctx, v_cache_id, pool, who, vc))) return rc;
   if ((rc = ctx_get(ctx, table_id, (uint64_t)p->batch * p->max_pages * 4, who, &table))) return rc;
   if ((rc = ctx_get(ctx, lengths_id, (uint64_t)p->batch * 4, who, &lengths))) return rc;
+  g->pool_bytes = pool;
   g->table = (const int*)table->ptr;
   g->lengths = (const int*)lengths->ptr;
   g->kv_heads = p->kv_heads;

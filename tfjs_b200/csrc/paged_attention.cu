@@ -1184,6 +1184,12 @@ extern "C" int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_pag
       return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is also an input", who);
   if (out_id == out_weights_id)
     return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is given twice", who);
+  const uint64_t values = units * p->head_dim * 4, sums = kv_units * cap * 4, rows = (uint64_t)p->batch * 4;
+  const Span spans[] = {{out->ptr, values}, {ow ? ow->ptr : nullptr, ow ? sums : 0}, {q->ptr, values},
+                        {kc->ptr, g.pool_bytes}, {vc->ptr, g.pool_bytes}, {g.table, rows * p->max_pages},
+                        {g.lengths, rows}, {mask ? mask->ptr : nullptr, mask ? rows * cap : 0},
+                        {w ? w->ptr : nullptr, w ? sums : 0}};
+  if ((rc = ctx_apart(ctx, who, spans, 9, 2))) return rc;
 
   PagedAttnArgs a;
   a.q = (const float*)q->ptr;

@@ -351,6 +351,11 @@ int tfjs_cuda_paged_cache_append(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_param
   if (out_lengths_id == lengths_id || k_id == k_cache_id || k_id == v_cache_id ||
       v_id == k_cache_id || v_id == v_cache_id)
     return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is also an input", who);
+  const uint64_t rows = (uint64_t)p->batch * 4;
+  const Span spans[] = {{kc->ptr, g.pool_bytes}, {vc->ptr, g.pool_bytes}, {ol->ptr, rows},
+                        {k->ptr, n * 4}, {v->ptr, n * 4}, {g.table, rows * p->max_pages}, {g.lengths, rows},
+                        {counts ? counts->ptr : nullptr, counts ? rows : 0}};
+  if ((rc = ctx_apart(ctx, who, spans, 8, 3))) return rc;
   cudaSetDevice(ctx->device);
   const bool wide = p->head_dim % 4 == 0 &&
                     (((uintptr_t)kc->ptr | (uintptr_t)vc->ptr | (uintptr_t)k->ptr | (uintptr_t)v->ptr) & 15) == 0;
@@ -407,6 +412,12 @@ int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params
     for (int j = 0; j < i; ++j)
       if (out[i] == out[j]) return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: an output is given twice", who);
   }
+  const uint64_t rows = (uint64_t)p->batch * 4;
+  const Span spans[] = {{kc->ptr, g.pool_bytes}, {vc->ptr, g.pool_bytes}, {ow->ptr, slots}, {op->ptr, slots},
+                        {ol->ptr, rows}, {ok->ptr, units * (uint64_t)p->budget * 4},
+                        {w->ptr, slots}, {g.table, rows * p->max_pages}, {g.lengths, rows},
+                        {pos ? pos->ptr : nullptr, pos ? slots : 0}, {tot ? tot->ptr : nullptr, tot ? rows : 0}};
+  if ((rc = ctx_apart(ctx, who, spans, 11, 6))) return rc;
   float *kp = (float*)kc->ptr, *vp = (float*)vc->ptr;
   EvictArgs a;
   a.weights = (const float*)w->ptr;

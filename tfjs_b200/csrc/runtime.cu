@@ -80,6 +80,15 @@ int ctx_scratch(tfjs_cuda_ctx* ctx, uint64_t bytes, void** out) {
   return TFJS_CUDA_OK;
 }
 
+int ctx_apart(tfjs_cuda_ctx* ctx, const char* who, const Span* spans, int n, int n_written) {
+  for (int i = 0; i < n_written; ++i)
+    for (int j = 0; j < n; ++j)
+      if (j != i && spans[i].meets(spans[j]))
+        return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: the call would write to memory that it also %s as another tensor",
+                        who, j < n_written ? "writes" : "reads");
+  return TFJS_CUDA_OK;
+}
+
 void ctx_mark_written(tfjs_cuda_ctx* ctx, int32_t id) {
   Buffer* b = ctx_buf(ctx, id);
   if (b) {
