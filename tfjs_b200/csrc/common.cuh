@@ -9,6 +9,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "error_word.h"
 #include "tfjs_cuda.h"
 
 struct Buffer {
@@ -101,7 +102,7 @@ struct tfjs_cuda_ctx {
   bool log_launches = false;
   std::vector<const char*> launch_log;
   int math_mode = TFJS_CUDA_MATH_TF32;
-  int* d_flag = nullptr;  // device error word written by bounded waits
+  int* d_flag = nullptr;  // device error word (error_word.h)
   int* h_flag = nullptr;  // pinned mirror
   long long* d_bad_index = nullptr;
   long long* h_bad_index = nullptr;
@@ -134,10 +135,6 @@ Buffer* ctx_buf(tfjs_cuda_ctx* ctx, int32_t id);
 int ctx_get(tfjs_cuda_ctx* ctx, int32_t id, uint64_t need, const char* name,
             Buffer** out);
 int ctx_scratch(tfjs_cuda_ctx* ctx, uint64_t bytes, void** out);
-
-// Values of the device error word from kBadInput on name inputs that only the device can
-// check; smaller ones are waits that gave up.
-enum { kBadInput = 1000, kBadPage = 1000, kBadLength = 1001 };
 
 // A workspace of one call, from the pool (or from the arena of the step being captured): it
 // goes back in stream order when the call returns, so that nothing outside the call, a

@@ -22,7 +22,7 @@ __device__ __forceinline__ int linear_length(const LinearArgs& a, int b) {
   if (!a.lengths) return a.seq;
   const int n = __ldg(a.lengths + b);
   if (n < 0 || n > a.seq) {
-    atomicExch(a.flag, kBadLength);
+    atomicOr(a.flag, kBadLength);
     return n < 0 ? 0 : a.seq;
   }
   return n;

@@ -21,7 +21,7 @@ struct PagedLayout {
 __device__ __forceinline__ int paged_length(const PagedLayout& g, int b) {
   const int n = __ldg(g.lengths + b);
   if (n < 0 || n > g.capacity) {
-    atomicExch(g.flag, kBadLength);
+    atomicOr(g.flag, kBadLength);
     return n < 0 ? 0 : g.capacity;
   }
   return n;
@@ -34,7 +34,7 @@ __device__ __forceinline__ uint32_t paged_row(const PagedLayout& g, int b, int h
   const int pi = g.page_shift >= 0 ? j >> g.page_shift : j / g.page_size;
   const int page = __ldg(g.table + (size_t)b * g.max_pages + pi);
   if ((unsigned)page >= (unsigned)g.num_pages) {
-    atomicExch(g.flag, kBadPage);
+    atomicOr(g.flag, kBadPage);
     return kNoRow;
   }
   return (uint32_t)((page * g.kv_heads + h) * g.page_size + (j - pi * g.page_size));

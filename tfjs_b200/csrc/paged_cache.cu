@@ -41,7 +41,7 @@ paged_append_kernel(const PagedLayout g, const float* __restrict__ k, const floa
   const bool bad = c < 0 || c > tokens || c > g.capacity - n;
   if (bad) c = c < 0 ? 0 : min(min(c, tokens), g.capacity - n);
   if (h == 0 && part == 0 && threadIdx.x == 0) {
-    if (bad) atomicExch(g.flag, kBadLength);
+    if (bad) atomicOr(g.flag, kBadLength);
     out_lengths[b] = n + c;
   }
   const int per_row = g.head_dim / V;

@@ -520,17 +520,14 @@ static int report_flag(tfjs_cuda_ctx* ctx, int* host_word) {
   if (*host_word != 0) {
     int v = *host_word;
     *host_word = 0;
-    if (v >= kBadInput)
-      return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s",
-                      v == kBadPage ? "a kernel needed a page that its page table does not name "
-                                      "(outside the pool); the slots of that page were left out"
-                                    : "a row's length is outside what its tensors hold; it was "
-                                      "clamped");
+    const char* input = error_word_input(v);
+    if (error_word_timeout(v) == 0) return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s", input);
     // a K-split GEMM that gave up may have left partial-tile flags raised
     if (ctx->sk_flags) cudaMemsetAsync(ctx->sk_flags, 0, 4096 * sizeof(unsigned), ctx->stream);
     return ctx_fail(ctx, TFJS_CUDA_DEVICE_TIMEOUT,
                     "a device-side wait gave up (code %d); results of the "
-                    "affected kernel are invalid", v);
+                    "affected kernel are invalid%s%s", error_word_timeout(v), input ? ".  Also: " : "",
+                    input ? input : "");
   }
   return TFJS_CUDA_OK;
 }
