@@ -235,3 +235,29 @@ def test_a_copy_writes_its_destination(backend):
     locked = backend.createTensorFromGPUData(Memory((2,), read_only=True))
     with pytest.raises(ValueError, match="read-only"):
         backend.copy(src.dataId, locked.dataId)
+
+
+def test_two_threads_get_their_own_ids(backend):
+    """The library's calls let other threads run: each caller's new id is its own."""
+    import threading
+    inside, go_on = threading.Event(), threading.Event()
+    plain, first = backend.lib.tfjs_cuda_alloc, []
+
+    def alloc(ctx, nbytes, out):
+        rc = plain(ctx, nbytes, out)
+        if not first:
+            first.append(out._obj.value)
+            inside.set()
+            go_on.wait(10)
+        return rc
+    backend.lib.tfjs_cuda_alloc = alloc
+    made = []
+    other = threading.Thread(target=lambda: made.append(backend.make_output([2000], "float32")))
+    other.start()
+    assert inside.wait(10)
+    mine = backend.make_output([2000], "float32")
+    foreign = backend.createTensorFromGPUData(Memory())
+    go_on.set()
+    other.join(10)
+    ids = [backend.data[t.dataId].dev for t in (made[0], mine, foreign)]
+    assert ids == [1, 2, 3]

@@ -515,8 +515,6 @@ class CudaBackend(object):
             raise CudaError(rc, "tfjs_cuda_create(device %d) failed with status "
                             "%d: no usable sm_100a GPU" % (device_ordinal, rc))
         self.ctx = ctx
-        self._out_id = c_int32()            # where calls leave a new id
-        self._out_id_ref = byref(self._out_id)
         self.device_ordinal = device_ordinal
         self.data = {}        # DataId -> _Record
         self._pinned = []
@@ -545,8 +543,9 @@ class CudaBackend(object):
             raise CudaError(rc, msg.decode() if msg else "status %d" % rc)
 
     def _alloc(self, nbytes):
-        self.check(self.lib.tfjs_cuda_alloc(self.ctx, nbytes, self._out_id_ref))
-        return self._out_id.value
+        out = c_int32()       # (of this call's own: ctypes lets other threads run meanwhile)
+        self.check(self.lib.tfjs_cuda_alloc(self.ctx, nbytes, byref(out)))
+        return out.value
 
     def floatPrecision(self):
         return 32
@@ -625,10 +624,10 @@ class CudaBackend(object):
         before = stream if stream is not None else info.get("stream")
         if before is not None:
             self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, before))
-        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes,
-                                                  self._out_id_ref))
+        out = c_int32()
+        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes, byref(out)))
         dataId = DataId()
-        rec = _Record(self._out_id.value, nbytes, found, 1, None)
+        rec = _Record(out.value, nbytes, found, 1, None)
         rec.foreign, rec.stream, rec.read_only = values, stream, bool(info["data"][1])
         self._exposed += 1
         self.data[dataId] = rec
