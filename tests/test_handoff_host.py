@@ -261,3 +261,15 @@ def test_two_threads_get_their_own_ids(backend):
     other.join(10)
     ids = [backend.data[t.dataId].dev for t in (made[0], mine, foreign)]
     assert ids == [1, 2, 3]
+
+
+def test_a_launch_that_fails_leaves_nothing_behind(backend):
+    t = backend.createTensorFromGPUData(Memory())
+    u = backend.make_output([2000], "float32")
+    with pytest.raises(RuntimeError):
+        backend.defer([2000], "float32", Deferred(t.dataId, u.dataId, fails=True))
+    assert backend.numDataIds() == 2 and backend.refCount(t.dataId) == backend.refCount(u.dataId) == 1
+    assert backend.data[t.dataId].held == 0
+    for x in (t, u):
+        assert backend.disposeData(x.dataId)
+    assert len(backend.data) == 0 and len(backend.lib.freed) == 3

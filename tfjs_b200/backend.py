@@ -744,7 +744,11 @@ class CudaBackend(object):
             self._matmuls_on[pending.a] = ids + [dataId]
         if self._exposed and any(self._is_exposed(self.data[d]) for d in pending.deps()):
             # somebody else may rewrite the memory at any time: what reads it launches now
-            self._resolve(rec)
+            try:
+                self._resolve(rec)
+            except Exception:
+                self.disposeData(dataId)
+                raise
         return TensorInfo(dataId, shape, dtype)
 
     @staticmethod

@@ -117,7 +117,14 @@ export class CudaBackend extends KernelBackend {
     this.pendingIds.add(dataId);
     if (pending instanceof PendingMatMul) this.noteMatMul(dataId, pending);
     // somebody else may rewrite the memory at any time: what reads it launches now
-    if (this.exposed > 0 && pending.deps().some(d => this.isExposed(this.data.get(d)))) this.resolve(r);
+    if (this.exposed > 0 && pending.deps().some(d => this.isExposed(this.data.get(d)))) {
+      try {
+        this.resolve(r);
+      } catch (e) {
+        this.disposeData(dataId);
+        throw e;
+      }
+    }
     return {dataId, shape, dtype};
   }
 
