@@ -273,3 +273,19 @@ def test_a_launch_that_fails_leaves_nothing_behind(backend):
     for x in (t, u):
         assert backend.disposeData(x.dataId)
     assert len(backend.data) == 0 and len(backend.lib.freed) == 3
+
+
+def test_a_tensors_info_is_the_callers(backend):
+    """A kernel that changes what it was given does not change the tensor, nor one that shares its data."""
+    from tfjs_b200.engine import Engine
+    engine = Engine()
+    engine.backend = backend
+    x = engine.make_tensor_from_info(backend.make_output([20, 100], "float32"))
+    first = x.info()
+    first.dtype = "int32"
+    second = x.info()
+    second.shape.append(1)
+    again = x.info()
+    assert (again.shape, again.dtype, again.dataId) == ([20, 100], "float32", x.dataId)
+    assert x.shape == [20, 100] and x.dtype == "float32"
+    x.dispose()

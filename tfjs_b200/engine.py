@@ -17,7 +17,6 @@ class Tensor(object):
 
     def __init__(self, engine, info):
         self._engine = engine
-        self._info = info
         self.dataId = info.dataId
         self.shape = list(info.shape)
         self.dtype = info.dtype
@@ -35,9 +34,7 @@ class Tensor(object):
         return n
 
     def info(self):
-        if self._info.shape != self.shape:
-            return TensorInfo(self.dataId, self.shape, self.dtype)
-        return self._info
+        return TensorInfo(self.dataId, self.shape, self.dtype)
 
     def dataSync(self):
         """engine.ts:1218-1222 -> backend.readSync."""
