@@ -26,9 +26,7 @@ linear_recurrent_kernel(const LinearArgs a, int tiles) {
   const int n = linear_length(a, b);
   const int r = threadIdx.x >> 3, c0 = tile * kTileV + (threadIdx.x & 7) * 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the decay in two parts: rounded to one, its error would grow with every step
-  const double exact = exp((double)__ldg(a.log_decay + h));
-  const float decay = (float)exact, decay_lo = isinf(decay) ? 0.0f : (float)(exact - (double)decay);
+  const Factor decay = factor_of(decay_power_exact(__ldg(a.log_decay + h), 1));
   const uint64_t s0 = (uint64_t)unit * a.dk * a.dv;
   float s[NR][4];
 #pragma unroll
@@ -59,7 +57,7 @@ linear_recurrent_kernel(const LinearArgs a, int tiles) {
       const float qq = row < a.dk ? __ldg(a.q + tok * a.dk + row) : 0.f;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        s[i][x] = fmaf(decay, s[i][x], fmaf(decay_lo, s[i][x], kk * v[x]));
+        s[i][x] = times_plus(decay, s[i][x], kk * v[x]);
         o[x] = fmaf(qq, s[i][x], o[x]);
       }
     }

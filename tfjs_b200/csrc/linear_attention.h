@@ -28,6 +28,26 @@ __device__ __forceinline__ int linear_length(const LinearArgs& a, int b) {
   return n;
 }
 
+// A factor that is applied again and again, in two parts: rounded to one float, its error would have
+// the same sign each time and grow with the steps.
+struct Factor {
+  float hi, lo;
+};
+__device__ __forceinline__ Factor factor_of(double exact) {
+  Factor f;
+  f.hi = (float)exact;
+  f.lo = isinf(f.hi) ? 0.0f : (float)(exact - (double)f.hi);
+  return f;
+}
+// f s + x.  (An infinite s times the small part would be an infinity of the other sign, or NaN.)
+__device__ __forceinline__ float times_plus(Factor f, float s, float x) {
+  return fmaf(f.hi, s, fmaf(f.lo, fabsf(s) <= 3.402823466e38f ? s : 0.0f, x));
+}
+// decay^e, in double
+__device__ __forceinline__ double decay_power_exact(float log_decay, int e) {
+  return e == 0 ? 1.0 : exp((double)log_decay * e);
+}
+
 // decay^e for a whole number e >= 0 (decay 0 included: 0^0 = 1)
 __device__ __forceinline__ float decay_power(float log_decay, int e) {
   return e == 0 ? 1.0f : expf(__fmul_rn(log_decay, (float)e));
