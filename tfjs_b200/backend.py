@@ -516,6 +516,7 @@ class CudaBackend(object):
                             "%d: no usable sm_100a GPU" % (device_ordinal, rc))
         self.ctx = ctx
         self.device_ordinal = device_ordinal
+        self._words = []      # (_word)
         self.data = {}        # DataId -> _Record
         self._pinned = []
         self._hidden = 0      # records kept alive only by pending launches
@@ -543,9 +544,20 @@ class CudaBackend(object):
             raise CudaError(rc, msg.decode() if msg else "status %d" % rc)
 
     def _alloc(self, nbytes):
-        out = c_int32()       # (of this call's own: ctypes lets other threads run meanwhile)
-        self.check(self.lib.tfjs_cuda_alloc(self.ctx, nbytes, byref(out)))
-        return out.value
+        word = self._word()
+        self.check(self.lib.tfjs_cuda_alloc(self.ctx, nbytes, word[1]))
+        out = word[0].value
+        self._words.append(word)
+        return out
+
+    def _word(self):
+        """An int32 that a call leaves a new id in, and its address.  The caller's own until it is put back
+        into `_words`: ctypes lets other threads run during a call."""
+        try:
+            return self._words.pop()
+        except IndexError:
+            word = c_int32()
+            return word, byref(word)
 
     def floatPrecision(self):
         return 32
@@ -624,10 +636,11 @@ class CudaBackend(object):
         before = stream if stream is not None else info.get("stream")
         if before is not None:
             self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, before))
-        out = c_int32()
-        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes, byref(out)))
+        word = self._word()
+        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes, word[1]))
         dataId = DataId()
-        rec = _Record(out.value, nbytes, found, 1, None)
+        rec = _Record(word[0].value, nbytes, found, 1, None)
+        self._words.append(word)
         rec.foreign, rec.stream, rec.read_only = values, stream, bool(info["data"][1])
         self._exposed += 1
         self.data[dataId] = rec
@@ -649,11 +662,14 @@ class CudaBackend(object):
     def gpu_data(self, tensor, stream):
         """readToGPU for a reference that the result takes over."""
         if self._unreleased or self._unsignalled:
-            self._release_gpu_data()
+            self._try_again()
         rec = self.data[tensor.dataId]
         # Whoever holds the memory may write to it: what is pending on its present contents launches
         # first, and there is no host copy from now on.
-        dev = self.device_id(tensor.dataId) if rec.read_only else self.device_id_for_update(tensor.dataId)
+        if rec.held and not rec.read_only:
+            self._launch_readers(tensor.dataId, rec)
+        dev = rec.dev or self.device_id(tensor.dataId)
+        rec.host = None
         ptr = c_void_p()
         self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
         if stream is not None:
@@ -670,42 +686,37 @@ class CudaBackend(object):
     def release_gpu_data(self, ref, stream):
         """Disposes the tensor that a GPUData held, behind the work on its holder's stream.  Its memory
         must not be used again before that, so a wait that is refused is tried again later."""
-        self._unreleased.append((ref, stream))
-        self._release_gpu_data()
+        # (during a capture the library would refuse the wait and discard the capture)
+        if self._capturing or (stream is not None and
+                               self.lib.tfjs_cuda_wait_stream(self.ctx, stream) != _cabi.OK):
+            self._unreleased.append((ref, stream))
+            return
+        rec = self.data.get(ref.dataId)
+        if rec is not None and rec.ref > 1 and rec.shared:      # (else the record goes as well)
+            self.check(self.lib.tfjs_cuda_device_ptr_end(self.ctx, rec.dev))
+            rec.shared -= 1
+            if rec.shared == 0 and rec.foreign is None:
+                self._exposed -= 1
+        if isinstance(ref, TensorInfo):
+            self.disposeData(ref.dataId)
+        else:
+            ref.dispose()
 
-    def _release_gpu_data(self):
-        if self._capturing:       # (the library would refuse the wait and discard the capture)
+    def _try_again(self):
+        """What could not be ordered against other streams when it went."""
+        if self._capturing:
             return
         self._unsignalled = [
             (memory, stream) for memory, stream in self._unsignalled
             if self.lib.tfjs_cuda_signal_stream(self.ctx, stream) != _cabi.OK]
-        todo, self._unreleased = self._unreleased, []
-        while todo:
-            ref, stream = todo.pop(0)
-            if stream is not None and \
-                    self.lib.tfjs_cuda_wait_stream(self.ctx, stream) != _cabi.OK:
-                self._unreleased.append((ref, stream))
-                continue
-            try:
-                rec = self.data.get(ref.dataId)
-                if rec is not None and rec.shared:
-                    rec.shared -= 1
-                    if rec.ref > 1:    # (else the buffer goes as well)
-                        self.check(self.lib.tfjs_cuda_device_ptr_end(self.ctx, rec.dev))
-                    if rec.shared == 0 and rec.foreign is None:
-                        self._exposed -= 1
-                if isinstance(ref, TensorInfo):
-                    self.disposeData(ref.dataId)
-                else:
-                    ref.dispose()
-            except Exception:
-                self._unreleased.extend(todo)
-                raise
+        late, self._unreleased = self._unreleased, []
+        for ref, stream in late:
+            self.release_gpu_data(ref, stream)
 
     def wait_stream(self, stream):
         """This backend's work from now on runs after what is queued on `stream`."""
         if self._unreleased or self._unsignalled:
-            self._release_gpu_data()
+            self._try_again()
         self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, int(stream)))
 
     def signal_stream(self, stream):
@@ -960,7 +971,7 @@ class CudaBackend(object):
         if rec.pending is not None:
             pending, rec.pending = rec.pending, None
             self._release(pending)
-        if self._is_exposed(rec):
+        if rec.shared or rec.foreign is not None:
             self._exposed -= 1
         if rec.stream is not None:     # its owner's next work waits for what read it here
             rc = self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream)
@@ -1042,7 +1053,7 @@ class CudaBackend(object):
 
     def sync(self):
         if self._unreleased or self._unsignalled:
-            self._release_gpu_data()
+            self._try_again()
         self.check(self.lib.tfjs_cuda_sync(self.ctx))
 
     def set_math_mode(self, mode):
@@ -1075,7 +1086,7 @@ class CudaBackend(object):
         finally:
             self._capturing = False
             if self._unreleased or self._unsignalled:
-                self._release_gpu_data()
+                self._try_again()
         return graph.value
 
     def graph_launch(self, graph):

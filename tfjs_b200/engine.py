@@ -34,7 +34,9 @@ class Tensor(object):
         return n
 
     def info(self):
-        return TensorInfo(self.dataId, self.shape, self.dtype)
+        info = TensorInfo.__new__(TensorInfo)     # (the shape holds ints already)
+        info.dataId, info.shape, info.dtype = self.dataId, self.shape[:], self.dtype
+        return info
 
     def dataSync(self):
         """engine.ts:1218-1222 -> backend.readSync."""
