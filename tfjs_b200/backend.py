@@ -99,15 +99,18 @@ class GPUData(object):
     def dispose(self):
         """Releases the tensor, behind the work on `stream`; where that stream cannot be waited
         for now (a step of either side is being captured), as soon as it can."""
-        ref, self.tensorRef = self.tensorRef, None
-        if ref is not None and self.backend.ctx:
-            self.backend.release_gpu_data(ref, self.stream)
+        ref = self.tensorRef
+        if ref is not None:
+            self.tensorRef = None
+            if self.backend.ctx:
+                self.backend.release_gpu_data(ref, self.stream)
 
     def __del__(self):
-        try:
-            self.dispose()
-        except Exception:      # the interpreter is going away, or the device is
-            pass
+        if self.tensorRef is not None:
+            try:
+                self.dispose()
+            except Exception:      # the interpreter is going away, or the device is
+                pass
 
 
 class _Record(object):
@@ -516,13 +519,14 @@ class CudaBackend(object):
                             "%d: no usable sm_100a GPU" % (device_ordinal, rc))
         self.ctx = ctx
         self.device_ordinal = device_ordinal
-        self._words = []      # (_word)
+        self._words = []      # (_alloc)
         self.data = {}        # DataId -> _Record
         self._pinned = []
         self._hidden = 0      # records kept alive only by pending launches
         self._capturing = False
-        self._unreleased = []   # (tensor, stream) of GPUData that went while it could not be waited for
-        self._unsignalled = []  # (foreign memory, stream) of tensors that are gone, likewise
+        # what could not be ordered against another stream when it went: tensors that GPUData held
+        # (True, tensor, stream) and memory of tensors that are gone (False, memory, stream)
+        self._late = []
         self._exposed = 0     # records whose memory others may write: foreign or shared
         self.lazy_fusion = os.environ.get("TFJS_CUDA_NO_LAZY_FUSION", "0") in ("", "0")
         # a pending 3x3 depthwise convolution consumed by a 1x1 convolution runs inside that
@@ -544,20 +548,19 @@ class CudaBackend(object):
             raise CudaError(rc, msg.decode() if msg else "status %d" % rc)
 
     def _alloc(self, nbytes):
-        word = self._word()
-        self.check(self.lib.tfjs_cuda_alloc(self.ctx, nbytes, word[1]))
+        # `_words`: int32s that calls leave a new id in, and their addresses.  A word is the caller's own
+        # until it is put back: ctypes lets other threads run during a call.
+        try:
+            word = self._words.pop()
+        except IndexError:
+            word = c_int32()
+            word = word, byref(word)
+        rc = self.lib.tfjs_cuda_alloc(self.ctx, nbytes, word[1])
+        if rc:
+            self.check(rc)
         out = word[0].value
         self._words.append(word)
         return out
-
-    def _word(self):
-        """An int32 that a call leaves a new id in, and its address.  The caller's own until it is put back
-        into `_words`: ctypes lets other threads run during a call."""
-        try:
-            return self._words.pop()
-        except IndexError:
-            word = c_int32()
-            return word, byref(word)
 
     def floatPrecision(self):
         return 32
@@ -620,7 +623,7 @@ class CudaBackend(object):
             raise ValueError("createTensorFromGPUData: dtype %s of the memory is not %s" %
                              (info["typestr"], dtype or "one of float32, int32, bool"))
         have = info["shape"]
-        n = size_from_shape(have)
+        n = int(math.prod(have))
         nbytes = n * step
         strides = info.get("strides")
         if strides is not None and n:
@@ -635,13 +638,22 @@ class CudaBackend(object):
         # handles that CUDA has for them)
         before = stream if stream is not None else info.get("stream")
         if before is not None:
-            self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, before))
-        word = self._word()
-        self.check(self.lib.tfjs_cuda_from_device(self.ctx, info["data"][0], nbytes, word[1]))
+            rc = self.lib.tfjs_cuda_wait_stream(self.ctx, before)
+            if rc:
+                self.check(rc)
+        address, read_only = info["data"]
+        try:
+            word = self._words.pop()
+        except IndexError:
+            word = c_int32()
+            word = word, byref(word)
+        rc = self.lib.tfjs_cuda_from_device(self.ctx, address, nbytes, word[1])
+        if rc:
+            self.check(rc)
         dataId = DataId()
         rec = _Record(word[0].value, nbytes, found, 1, None)
         self._words.append(word)
-        rec.foreign, rec.stream, rec.read_only = values, stream, bool(info["data"][1])
+        rec.foreign, rec.stream, rec.read_only = values, stream, read_only
         self._exposed += 1
         self.data[dataId] = rec
         return TensorInfo(dataId, have if shape is None else shape, found)
@@ -661,7 +673,7 @@ class CudaBackend(object):
 
     def gpu_data(self, tensor, stream):
         """readToGPU for a reference that the result takes over."""
-        if self._unreleased or self._unsignalled:
+        if self._late:
             self._try_again()
         rec = self.data[tensor.dataId]
         # Whoever holds the memory may write to it: what is pending on its present contents launches
@@ -671,13 +683,16 @@ class CudaBackend(object):
         dev = rec.dev or self.device_id(tensor.dataId)
         rec.host = None
         ptr = c_void_p()
-        self.check(self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr)))
+        rc = self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr))
+        if rc:
+            self.check(rc)
         if stream is not None:
-            try:
-                self.check(self.lib.tfjs_cuda_signal_stream(self.ctx, stream))
-            except CudaError:
-                self.lib.tfjs_cuda_device_ptr_end(self.ctx, dev)
-                raise
+            rc = self.lib.tfjs_cuda_signal_stream(self.ctx, stream)
+            if rc:
+                try:
+                    self.check(rc)
+                finally:
+                    self.lib.tfjs_cuda_device_ptr_end(self.ctx, dev)
         if rec.shared == 0 and rec.foreign is None:
             self._exposed += 1
         rec.shared += 1
@@ -689,7 +704,7 @@ class CudaBackend(object):
         # (during a capture the library would refuse the wait and discard the capture)
         if self._capturing or (stream is not None and
                                self.lib.tfjs_cuda_wait_stream(self.ctx, stream) != _cabi.OK):
-            self._unreleased.append((ref, stream))
+            self._late.append((True, ref, stream))
             return
         rec = self.data.get(ref.dataId)
         if rec is not None and rec.ref > 1 and rec.shared:      # (else the record goes as well)
@@ -697,7 +712,7 @@ class CudaBackend(object):
             rec.shared -= 1
             if rec.shared == 0 and rec.foreign is None:
                 self._exposed -= 1
-        if isinstance(ref, TensorInfo):
+        if type(ref) is TensorInfo:
             self.disposeData(ref.dataId)
         else:
             ref.dispose()
@@ -706,16 +721,20 @@ class CudaBackend(object):
         """What could not be ordered against other streams when it went."""
         if self._capturing:
             return
-        self._unsignalled = [
-            (memory, stream) for memory, stream in self._unsignalled
-            if self.lib.tfjs_cuda_signal_stream(self.ctx, stream) != _cabi.OK]
-        late, self._unreleased = self._unreleased, []
-        for ref, stream in late:
-            self.release_gpu_data(ref, stream)
+        late, self._late = self._late, []
+        try:
+            while late:
+                held, what, stream = late.pop()
+                if held:
+                    self.release_gpu_data(what, stream)
+                elif self.lib.tfjs_cuda_signal_stream(self.ctx, stream) != _cabi.OK:
+                    self._late.append((held, what, stream))
+        finally:
+            self._late.extend(late)
 
     def wait_stream(self, stream):
         """This backend's work from now on runs after what is queued on `stream`."""
-        if self._unreleased or self._unsignalled:
+        if self._late:
             self._try_again()
         self.check(self.lib.tfjs_cuda_wait_stream(self.ctx, int(stream)))
 
@@ -967,7 +986,9 @@ class CudaBackend(object):
             self._hidden -= 1
         del self.data[dataId]
         if rec.dev:
-            self.check(self.lib.tfjs_cuda_free(self.ctx, rec.dev))
+            rc = self.lib.tfjs_cuda_free(self.ctx, rec.dev)
+            if rc:
+                self.check(rc)
         if rec.pending is not None:
             pending, rec.pending = rec.pending, None
             self._release(pending)
@@ -977,8 +998,8 @@ class CudaBackend(object):
             rc = self.lib.tfjs_cuda_signal_stream(self.ctx, rec.stream)
             if rc == _cabi.UNSUPPORTED and not self._capturing:
                 # its owner is capturing on that stream: the memory stays referenced until it is not
-                self._unsignalled.append((rec.foreign, rec.stream))
-            else:                      # (a capture began behind all work that read it)
+                self._late.append((False, rec.foreign, rec.stream))
+            elif rc:                   # (a capture began behind all work that read it)
                 self.check(rc)
 
     def refCount(self, dataId):
@@ -1052,7 +1073,7 @@ class CudaBackend(object):
         return True
 
     def sync(self):
-        if self._unreleased or self._unsignalled:
+        if self._late:
             self._try_again()
         self.check(self.lib.tfjs_cuda_sync(self.ctx))
 
@@ -1085,7 +1106,7 @@ class CudaBackend(object):
             self.check(self.lib.tfjs_cuda_capture_end(self.ctx, 1 if abandon else 0, byref(graph)))
         finally:
             self._capturing = False
-            if self._unreleased or self._unsignalled:
+            if self._late:
                 self._try_again()
         return graph.value
 
@@ -1135,7 +1156,7 @@ class CudaBackend(object):
             self.lib.tfjs_cuda_destroy(self.ctx)
             self.ctx = None
             self.data = {}
-            self._unreleased, self._unsignalled = [], []
+            self._late = []
 
     def __del__(self):
         try:

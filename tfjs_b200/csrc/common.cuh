@@ -113,6 +113,7 @@ struct tfjs_cuda_ctx {
   // signalled and has missed nothing since is not signalled again.
   uint64_t work = 1, signalled_work = 0;
   unsigned long long signalled_stream = 0;  // cudaStreamGetId: never given out twice
+  void* signalled_handle = (void*)~(uintptr_t)0;
   std::vector<cudaEvent_t> prof_events;  // numbered events for per-kernel timing
   std::vector<cudaEvent_t> read_events;  // tickets of tfjs_cuda_read_begin (index + 1)
   std::vector<cudaEvent_t> read_order;   // per ticket: orders the read stream behind the compute stream

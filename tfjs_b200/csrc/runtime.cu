@@ -760,10 +760,9 @@ int tfjs_cuda_wait_stream(tfjs_cuda_ctx* ctx, void* stream) {
   const int rc = order_streams(ctx, (cudaStream_t)stream, ctx->stream, (cudaStream_t)stream);
   if (rc) return rc;
   // That work is in front of this context's stream now, so whoever is signalled waits for it too; the
-  // stream it came from alone has it already.
-  unsigned long long id = 0;
-  if (cudaStreamGetId((cudaStream_t)stream, &id) != cudaSuccess || id != ctx->signalled_stream) ctx->work++;
-  cudaGetLastError();
+  // stream it came from alone has it already.  (A new stream in the place of one that was signalled and
+  // destroyed has another id there, and nobody signals the old one.)
+  if (stream != ctx->signalled_handle) ctx->work++;
   return TFJS_CUDA_OK;
 }
 
@@ -777,6 +776,7 @@ int tfjs_cuda_signal_stream(tfjs_cuda_ctx* ctx, void* stream) {
   if (known && id == ctx->signalled_stream && ctx->work == ctx->signalled_work) return TFJS_CUDA_OK;
   const int rc = order_streams(ctx, ctx->stream, (cudaStream_t)stream, (cudaStream_t)stream);
   ctx->signalled_stream = id;
+  ctx->signalled_handle = stream;
   ctx->signalled_work = rc == TFJS_CUDA_OK && known ? ctx->work : 0;
   return rc;
 }

@@ -12,6 +12,9 @@ from . import kernel_registry
 from .backend import TensorInfo
 
 
+_new = object.__new__
+
+
 class Tensor(object):
     """Handle over {dataId, shape, dtype} (tfjs-core/src/tensor.ts)."""
 
@@ -34,7 +37,7 @@ class Tensor(object):
         return n
 
     def info(self):
-        info = TensorInfo.__new__(TensorInfo)     # (the shape holds ints already)
+        info = _new(TensorInfo)     # (the shape holds ints already)
         info.dataId, info.shape, info.dtype = self.dataId, self.shape[:], self.dtype
         return info
 
@@ -62,7 +65,7 @@ class Tensor(object):
         backend = engine.backend
         backend.incRef(self.dataId)
         engine.num_tensors += 1
-        ref = Tensor(engine, self.info())
+        ref = Tensor(engine, self)
         try:
             return backend.gpu_data(ref, stream)
         except Exception:
