@@ -23,3 +23,35 @@ def test_an_infinite_state_stays_infinite(tf, n, log_decay):
     assert got[0, 0, 3, 5] == np.inf and got[0, 1, 30, 31] == -np.inf
     there = np.isfinite(s)
     assert np.all(np.abs(got - ref)[there] <= off[there])
+
+
+def test_long_rows_keep_their_first_state(tf):
+    """128 chunks of tokens whose keys are zero leave exp(log_decay)^16384 times the first state.
+    A decay for a whole chunk that is one float is off the same way in every chunk, by half a unit in its
+    last place or more: 64 EPS in all and more for these.  What remains with the decay in two
+    parts is the rounding of each chunk's step, at most EPS and to either side: over 128 steps its standard
+    deviation is below 128 ** 0.5 * EPS / 3 ** 0.5 = 6.6 EPS, over the mean of 1024 elements 0.21 EPS.
+    2 EPS is over nine of those."""
+    h, n, d = 8, 16384, 32
+    r = np.random.default_rng(21)
+    q = np.zeros((1, h, n, d), np.float32)
+    s = (1.0 + r.random((1, h, d, d))).astype(np.float32)
+    ld = (-np.geomspace(1e-6, 1e-4, h)).astype(np.float32)
+    _, got = call(tf, q, q, q, ld, state=s)
+    ref = s.astype(np.float64) * np.exp(ld.astype(np.float64) * n)[None, :, None, None]
+    drift = np.mean(got / ref - 1.0, axis=(0, 2, 3)) / dc.EPS
+    assert np.all(np.abs(drift) <= 2.0), drift
+    # the largest error: 128 roundings of EPS each and the two products of a step
+    assert np.max(np.abs(got / ref - 1.0)) <= 132 * dc.EPS
+
+
+@pytest.mark.parametrize("n", [1100, 1152, 2047, 2049, 4200])
+def test_many_chunks(tf, n):
+    """9, 16, 17 and 33 chunks: beyond the first eight that the scan has in flight, its second batch,
+    and its second time around; ragged rows."""
+    b, h, dk, dv = 2, 2, 16, 32
+    q, k, v, s = inputs(n, b, h, n, dk, dv)
+    ld = np.array([-1e-4, -0.01], np.float32)
+    lengths = np.array([n, n - 700], np.int32)
+    check(call(tf, q, k, v, ld, state=s, scale=0.25, lengths=lengths),
+          dc.linear(q, k, v, ld, s, 0.25, lengths))
