@@ -497,8 +497,8 @@ int tfjs_cuda_paged_cache_append(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_param
  * over the slots of row b; query head h reads key-value head h / (heads / kv_heads).
  * q is [batch, heads, 1, head_dim], out [batch, 1, heads, head_dim]; has_scale = 0 skips the
  * product.  mask (float32 [batch, capacity], 0: none) is added to the scores; -infinity hides
- * a slot, whose key and value then do not count whatever they hold, and nothing is read of slots
- * behind a row's length.  A row that has no slot, or only hidden ones (scores of -infinity), gives
+ * a slot, whose key and value then do not count whatever they hold (a page of which every slot is hidden
+ * is not needed), and nothing is read of slots behind a row's length.  A row that has no slot, or only hidden ones (scores of -infinity), gives
  * zeros.  Finite keys, values and queries are assumed: an infinity may come out as NaN.  weights (float32 [batch, kv_heads, capacity], 0: none) accumulates
  * attention: out_weights[b, g, j] = weights[b, g, j] + the sum of p_j over the query heads of
  * key-value head g, and 0 behind the row's length. */

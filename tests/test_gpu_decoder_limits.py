@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests import decoder_cases as dc
-from tests.test_gpu_paged_cache import run_evict, tf  # noqa: F401  (tf: a fixture)
+from tests.test_gpu_paged_cache import Held, attend, check, run_evict, tf  # noqa: F401  (tf: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,31 @@ def test_memory_that_a_call_writes_is_its_own(tf, cuda_engine):
     for t in outs + [kc, vc, same, over, table, lengths, k, inside, w, w_inside, q]:
         t.dispose()
     assert float(x.sum()) == 2 * 2 * 16
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (4, 1, 128), (8, 1, 64), (16, 1, 32), (4, 2, 33)])
+def test_pages_that_the_mask_hides_are_not_needed(tf, cuda_engine, heads, kv, dim):
+    """A window over a long row: the pages in front of it have been given back, their entries name
+    none, and the mask hides their slots.  Nothing is wrong with such a call."""
+    from tfjs_b200 import _cabi
+    page, lengths = 8, [300, 40, 9]
+    r = np.random.default_rng(dim)
+    cache = dc.Cache(dim, kv, dim, page, lengths)
+    mask = np.zeros((3, cache.capacity), np.float32)
+    mask[0, :203] = mask[1, :16] = -np.inf
+    q = r.standard_normal((3, heads, 1, dim)).astype(np.float32)
+    w = r.random((3, kv, cache.capacity)).astype(np.float32)
+    ref, neww, off, woff = dc.attention(q, cache, lengths, 0.2, mask, w)
+    cache.table[0, :203 // page] = -1
+    cache.table[1, :2] = 10 ** 6
+    got, gotw = attend(tf, cache, q, 0.2, mask, w)        # (reads block: an error would be raised)
+    check(got, ref, off)
+    check(gotw, neww, woff)
+    # one slot of such a page is shown: reported
+    mask[0, 100] = 0.0
+    h = Held(tf, cache)
+    h(tf.paged_attention(h(q), h.k, h.v, h.table, h.lengths, 0.2, h(mask)))
+    with pytest.raises(_cabi.CudaError) as e:
+        cuda_engine.backend.sync()
+    h.close()
+    assert e.value.code == 1 and "page" in str(e.value)

@@ -28,13 +28,14 @@ __device__ __forceinline__ int paged_length(const PagedLayout& g, int b) {
 }
 
 // Index, in rows of head_dim values, of slot j of row b and head h in both pools; kNoRow (and
-// a report) when the table names no page of the pool for it.  The number of rows of a pool
-// is below 2^31 (checked on the host), its byte offsets are not.
+// a report, unless the caller makes it) when the table names no page of the pool for it.  The number of
+// rows of a pool is below 2^31 (checked on the host), its byte offsets are not.
+template <bool REPORT = true>
 __device__ __forceinline__ uint32_t paged_row(const PagedLayout& g, int b, int h, int j) {
   const int pi = g.page_shift >= 0 ? j >> g.page_shift : j / g.page_size;
   const int page = __ldg(g.table + (size_t)b * g.max_pages + pi);
   if ((unsigned)page >= (unsigned)g.num_pages) {
-    atomicOr(g.flag, kBadPage);
+    if (REPORT) atomicOr(g.flag, kBadPage);
     return kNoRow;
   }
   return (uint32_t)((page * g.kv_heads + h) * g.page_size + (j - pi * g.page_size));

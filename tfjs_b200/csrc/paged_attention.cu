@@ -674,8 +674,8 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
             for (int pi = page0 + lane; pi <= page1; pi += 32) {
               const int from = max(first, pi * g.page_size);
               const int to = (int)min((long long)last, (long long)(pi + 1) * g.page_size);
-              const uint32_t row = paged_row(g, pc.b, pc.h, from);
-              if (row == kNoRow) continue;
+              const uint32_t row = paged_row<false>(g, pc.b, pc.h, from);
+              if (row == kNoRow) continue;   // (reported below, if one of its slots counts)
               const uint32_t n = (uint32_t)(to - from) * (uint32_t)(D * 4);
               if (pass)
                 bulk_copy(ring + (uint32_t)slot * tile_bytes + (uint32_t)(from - first) * (uint32_t)(D * 4),
@@ -710,10 +710,10 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
     auto look = [&](int t, int& page, float& add) {
       const int mine = pc.begin + t * T + warp * TW + lane;
       page = -1;
-      add = 0.f;
+      add = -INFINITY;
       if (lane < TW && mine < pc.end) {
         page = __ldg(g.table + (size_t)pc.b * g.max_pages + (g.page_shift >= 0 ? mine >> g.page_shift : mine / g.page_size));
-        if (a.mask) add = __ldg(a.mask + (uint64_t)pc.b * g.capacity + mine);
+        add = a.mask ? __ldg(a.mask + (uint64_t)pc.b * g.capacity + mine) : 0.f;
       }
     };
     int page, next_page;
@@ -725,7 +725,9 @@ paged_attention_bulk_kernel(const PagedLayout g, const PagedAttnArgs a) {
       add = next_add;
       look(t + 1, next_page, next_add);
       // (a slot hidden by the mask does not count, whatever it holds, NaN included)
-      const uint32_t seen = __ballot_sync(0xffffffffu, (unsigned)page < (unsigned)g.num_pages && add != -INFINITY);
+      const bool counts = add != -INFINITY, there = (unsigned)page < (unsigned)g.num_pages;
+      if (counts && !there) atomicOr(g.flag, kBadPage);
+      const uint32_t seen = __ballot_sync(0xffffffffu, counts && there);
       // (a wait that gives up marks the launch as failed; the rest runs through without waiting)
       if (alive && !warp_wait(full(slot), phase)) {
         alive = false;

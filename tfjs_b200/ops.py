@@ -345,7 +345,8 @@ def paged_attention(q, kCache, vCache, pageTable, lengths, scale=None, mask=None
 
     q [batch, heads, 1, headDim]; heads is a multiple of the pools' kvHeads, and query head h
     reads key-value head h // (heads // kvHeads).  mask [batch, maxPages * pageSize] is added
-    to the scores; -infinity hides a slot.  Returns [batch, 1, heads, headDim] (as
+    to the scores; -infinity hides a slot, and pages all of whose slots are hidden need not be named by
+    the table (a window over a long row).  Returns [batch, 1, heads, headDim] (as
     fused_attention does for a sequence); a row with nothing to attend to gives zeros.  Finite
     keys, values and queries are assumed (an infinity may come out as NaN).  With
     weights [batch, kvHeads, maxPages * pageSize], which accumulates each slot's attention for
