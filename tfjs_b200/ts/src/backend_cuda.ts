@@ -6,7 +6,7 @@
  * Python twin (executed by the tests): tfjs_b200/backend.py.
  */
 import {backend_util, BackendTimingInfo, DataStorage, DataType, engine, KernelBackend,
-        TensorInfo, TypedArray, util} from '@tensorflow/tfjs-core';
+        Tensor, TensorInfo, TypedArray, util} from '@tensorflow/tfjs-core';
 
 import {binding, Ctx} from './binding';
 import {Desc, Pending, PendingConv, PendingDepthwise, PendingMatMul} from './pending';
@@ -21,6 +21,7 @@ interface Record {
   held: number;        // how many of refCount belong to pending launches that read it
   foreign?: ForeignData;  // the owner of device memory that is not the backend's
   shared?: boolean;    // its address was handed out
+  holders?: Set<bigint>;  // streams that those who have it work on
 }
 
 /** Device memory of another library (a WebGPUData-like value: an address instead of a GPUBuffer), and
@@ -28,6 +29,13 @@ interface Record {
 export interface ForeignData {
   buffer: bigint;
   stream?: bigint;
+}
+
+/** tfjs-core's GPUData with a device address in the place of a GPUBuffer; what readToGPU returns. */
+export interface CudaGPUData {
+  tensorRef: Tensor;
+  buffer: bigint;
+  bufSize: number;
 }
 
 const HOST_RESIDENT_BYTES = 4096;
@@ -270,9 +278,16 @@ export class CudaBackend extends KernelBackend {
   }
 
   // -------------------------------------------------------- other libraries' memory --
-  /** A tensor over another library's device memory, without a copy (tf.tensor({buffer, zeroCopy: true})).
-   * With a stream, this backend's work waits for what is queued there now, and what is queued there after
-   * the tensor is disposed waits for this backend's work. */
+  /** A tensor over another library's device memory, without a copy; call it on the backend, with an
+   * address.  With a stream, this backend's work waits for what is queued there now, and what is queued
+   * there after the tensor is disposed waits for this backend's work. */
+  override createTensorFromGPUData(values: ForeignData|Parameters<KernelBackend['createTensorFromGPUData']>[0],
+                                   shape: number[], dtype: DataType): Tensor {
+    const info = this.fromForeign(values as unknown as ForeignData, shape, dtype);
+    return engine().makeTensorFromTensorInfo(info, this);
+  }
+
+  /** The same as a TensorInfo. */
   fromForeign(values: ForeignData, shape: number[], dtype: DataType): TensorInfo {
     const nbytes = util.sizeFromShape(shape) * bytesPerElement(dtype);
     if (values.stream != null) binding.waitStream(this.ctx, values.stream);
@@ -283,15 +298,25 @@ export class CudaBackend extends KernelBackend {
     return {dataId, shape, dtype};
   }
 
-  /** The device address of a tensor (tensor.dataToGPU()); whoever holds it may write to it, so what is
-   * pending on its present contents launches first, and what reads it later launches when called. */
-  toForeign(t: TensorInfo, stream?: bigint): ForeignData {
+  /** The device memory of a tensor (tensor.dataToGPU({stream})), without a copy: `buffer` is the address,
+   * and `tensorRef`, a reference of its own, keeps it.  Whoever holds it may write to it, so what is pending
+   * on its present contents launches first, and what reads it later launches when called.  With a stream,
+   * what is queued there from now on runs after this backend's work, and the memory is used again behind
+   * what is queued there when its last tensor is disposed. */
+  override readToGPU(dataId: object, options?: object): ReturnType<KernelBackend['readToGPU']> {
+    const stream = (options as {stream?: bigint}|undefined)?.stream;
+    const r = this.data.get(dataId);
+    const t = {dataId, shape: [r.nbytes / bytesPerElement(r.dtype)], dtype: r.dtype};
     const buffer = binding.devicePtr(this.ctx, this.deviceIdForUpdate(t));
-    if (stream != null) binding.signalStream(this.ctx, stream);
-    const r = this.data.get(t.dataId);
-    if (!r.shared && r.foreign == null) this.exposed++;
+    if (!this.isExposed(r)) this.exposed++;
     r.shared = true;
-    return {buffer, stream};
+    if (stream != null) {
+      binding.signalStream(this.ctx, stream);
+      (r.holders ??= new Set()).add(stream);
+    }
+    this.incRef(dataId);
+    const data: CudaGPUData = {tensorRef: engine().makeTensorFromTensorInfo(t, this), buffer, bufSize: r.nbytes};
+    return data as unknown as ReturnType<KernelBackend['readToGPU']>;
   }
 
   hostValues(t: TensorInfo): TypedArray|undefined { return this.data.get(t.dataId).host; }
@@ -328,11 +353,32 @@ export class CudaBackend extends KernelBackend {
     return true;
   }
 
+  /** Frees a buffer behind the work of those who held it; a stream that cannot be waited for now (it is
+   * being captured) is tried again with the next buffer. */
+  private freeBehind(id: number, streams: bigint[]): void {
+    const todo = [...this.late, {id, streams}];
+    this.late = [];
+    for (const one of todo) {
+      try {
+        for (const stream of one.streams) binding.waitStream(this.ctx, stream);
+      } catch (_) {
+        this.late.push(one);
+        continue;
+      }
+      if (one.id !== 0) binding.free(this.ctx, one.id);
+    }
+  }
+  private late: Array<{id: number, streams: bigint[]}> = [];
+
   private drop(dataId: object, r: Record): void {
     if (r.held > 0 && r.refCount <= r.held) this.hidden--;
     this.data.delete(dataId);
     this.pendingIds.delete(dataId);
-    if (r.id !== 0) binding.free(this.ctx, r.id);
+    if (r.holders != null || this.late.length > 0) {
+      this.freeBehind(r.id, [...(r.holders ?? [])]);
+    } else if (r.id !== 0) {
+      binding.free(this.ctx, r.id);
+    }
     if (this.isExposed(r)) this.exposed--;
     if (r.foreign?.stream != null) binding.signalStream(this.ctx, r.foreign.stream);
     if (r.pending != null) {
