@@ -287,3 +287,10 @@ def test_a_tensors_info_is_the_callers(backend):
     assert (again.shape, again.dtype, again.dataId) == ([20, 100], "float32", x.dataId)
     assert x.shape == [20, 100] and x.dtype == "float32"
     x.dispose()
+
+
+def test_masked_memory_is_refused(backend):
+    with pytest.raises(ValueError, match="mask"):
+        backend.createTensorFromGPUData(Memory(mask=Memory()))
+    assert backend.numDataIds() == 0 and backend.lib.taken() == []
+    backend.createTensorFromGPUData(Memory(mask=None))

@@ -632,6 +632,8 @@ class CudaBackend(object):
                     raise ValueError("createTensorFromGPUData: the memory is not contiguous "
                                      "(shape %s, strides %s)" % (list(have), list(strides)))
                 step *= d
+        if info.get("mask") is not None:
+            raise ValueError("createTensorFromGPUData: masked memory")
         if shape is not None and size_from_shape(shape) != n:
             raise ValueError("createTensorFromGPUData: %d values for shape %s" % (n, list(shape)))
         # (the interface's numbers for the legacy and the per-thread default stream, 1 and 2, are the
