@@ -110,9 +110,9 @@ extern "C" int tfjs_cuda_linear_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_li
   if (p->batch <= 0 || p->heads <= 0 || p->seq <= 0 || p->dim_k <= 0 || p->dim_v <= 0)
     return ctx_fail(ctx, TFJS_CUDA_INVALID_ARG, "%s: dimensions must be positive", who);
   const uint64_t units = (uint64_t)p->batch * p->heads;
-  if (p->dim_k > 256 || p->dim_v > 256 || units > 0xffffffull)
+  if (p->dim_k > 256 || p->dim_v > 256 || units > 0xffffffull || p->seq > 0x7fffff00)
     return ctx_fail(ctx, TFJS_CUDA_UNSUPPORTED,
-                    "%s: heads of up to 256 values, fewer than 2^24 rows times heads", who);
+                    "%s: heads of up to 256 values, fewer than 2^24 rows times heads, tokens below 2^31 - 255", who);
   const uint64_t tokens = units * p->seq, st = units * p->dim_k * p->dim_v * 4;
   Buffer *q, *k, *v, *d, *s = nullptr, *n = nullptr, *out, *os;
   int rc;

@@ -12,6 +12,9 @@ from ..kernel_registry import KernelConfig
 from .common import BACKEND, dev
 
 
+_MOST = (1 << 31) - 1      # of a dimension: the kernels count in int32
+
+
 def _want(name, what, info, shape, dtype):
     """`shape` holds sizes, or None where any size goes."""
     got = info.shape
@@ -21,13 +24,15 @@ def _want(name, what, info, shape, dtype):
                 return
         elif len(got) == len(shape):
             for w, g in zip(shape, got):
-                if g <= 0 or (w is not None and g != w):
+                if g <= 0 or g > _MOST or (w is not None and g != w):
                     break
             else:
                 return
     if 0 in got and info.dtype == dtype and len(got) == len(shape) and \
             all(w is None or g == w for w, g in zip(shape, got)):
         raise ValueError("%s: %s has an empty dimension: %s" % (name, what, list(got)))
+    if got and max(got) > _MOST:
+        raise ValueError("%s: %s has a dimension above 2^31 - 1: %s" % (name, what, list(got)))
     raise ValueError("%s: %s must be %s %s, but got %s %s" %
                      (name, what, dtype, ["any" if w is None else w for w in shape],
                       info.dtype, list(got)))

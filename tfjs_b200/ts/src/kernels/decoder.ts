@@ -18,6 +18,9 @@ function want(name: string, what: string, t: TensorInfo, shape: Array<number|nul
   if (t.dtype !== dtype || t.shape.length !== shape.length || shape.some((w, i) => w != null && w !== t.shape[i])) {
     throw new Error(`${name}: ${what} must be ${dtype} [${shape.map(w => w ?? 'any')}], but got ${t.dtype} [${t.shape}]`);
   }
+  if (t.shape.some(d => d > 2 ** 31 - 1)) {
+    throw new Error(`${name}: ${what} has a dimension above 2^31 - 1: [${t.shape}]`);
+  }
   if (t.shape.some(d => d <= 0)) throw new Error(`${name}: ${what} has an empty dimension: [${t.shape}]`);
 }
 
