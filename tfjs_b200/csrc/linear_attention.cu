@@ -6,9 +6,9 @@
 
 namespace {
 
-// Up to here the recurrence, one dependent step a token: 8 / 16 / 32 tokens take 7 / 11 / 19 us for
-// 12 states of 64 x 64 and 69 / 123 / 229 us for 1024 of 128 x 128, where the chunked form takes
-// 17 and 295 for each of them.
+// Up to here the recurrence, one dependent step a token: 8 / 16 / 32 tokens take 9 / 14 / 25 us for
+// 12 states of 64 x 64 and 71 / 128 / 244 us for 1024 of 128 x 128 (ncu durations), where the three launches
+// of the chunked form take 24 and 311 for 33 tokens.
 constexpr int kFewTokens = 32;
 constexpr int kTileV = 32;      // columns of the state that a block holds
 constexpr int kRowGroups = 32;  // threads that share a column's rows
@@ -26,7 +26,6 @@ linear_recurrent_kernel(const LinearArgs a, int tiles) {
   const int n = linear_length(a, b);
   const int r = threadIdx.x >> 3, c0 = tile * kTileV + (threadIdx.x & 7) * 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Factor decay = factor_of(decay_power_exact(__ldg(a.log_decay + h), 1));
   const uint64_t s0 = (uint64_t)unit * a.dk * a.dv;
   float s[NR][4];
 #pragma unroll
@@ -45,22 +44,31 @@ linear_recurrent_kernel(const LinearArgs a, int tiles) {
       for (int x = 0; x < 4; ++x) s[i][x] = in && c0 + x < a.dv ? __ldg(p + x) : 0.f;
     }
   }
-  for (int t = 0; t < n; ++t) {
-    const uint64_t tok = (uint64_t)unit * a.seq + t;
-    float v[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+  // (the next token's values are on their way while a step waits for the sum over the block)
+  float v[4], kk[NR], qq[NR];
+  auto fetch = [&](uint64_t tok) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) v[x] = c0 + x < a.dv ? __ldg(a.v + tok * a.dv + c0 + x) : 0.f;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int row = i * kRowGroups + r;
-      const float kk = row < a.dk ? __ldg(a.k + tok * a.dk + row) : 0.f;
-      const float qq = row < a.dk ? __ldg(a.q + tok * a.dk + row) : 0.f;
+      kk[i] = row < a.dk ? __ldg(a.k + tok * a.dk + row) : 0.f;
+      qq[i] = row < a.dk ? __ldg(a.q + tok * a.dk + row) : 0.f;
+    }
+  };
+  if (n > 0) fetch((uint64_t)unit * a.seq);
+  const Factor decay = factor_of(decay_power_exact(__ldg(a.log_decay + h), 1));
+  for (int t = 0; t < n; ++t) {
+    const uint64_t tok = (uint64_t)unit * a.seq + t;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        s[i][x] = times_plus(decay, s[i][x], kk * v[x]);
-        o[x] = fmaf(qq, s[i][x], o[x]);
+        s[i][x] = times_plus(decay, s[i][x], kk[i] * v[x]);
+        o[x] = fmaf(qq[i], s[i][x], o[x]);
       }
-    }
+    if (t + 1 < n) fetch(tok + 1);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       o[x] += __shfl_xor_sync(0xffffffffu, o[x], 8);

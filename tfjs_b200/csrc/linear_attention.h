@@ -28,21 +28,23 @@ __device__ __forceinline__ int linear_length(const LinearArgs& a, int b) {
   return n;
 }
 
-// A factor that is applied again and again, in two parts: rounded to one float, its error would have
-// the same sign each time and grow with the steps.
+// A positive factor that is applied again and again, in two parts: rounded to one float, its error would
+// have the same sign each time and grow with the steps.  The large part is rounded down and the small one
+// is never 0 beside it (at least 2^-149), so that both keep the sign of an infinite value and it stays what
+// it is; a test of every value for that took a quarter more time (1024 states of 128 x 128, 32 tokens:
+// 299 us a call, here 236).
 struct Factor {
   float hi, lo;
 };
 __device__ __forceinline__ Factor factor_of(double exact) {
   Factor f;
-  f.hi = (float)exact;
-  f.lo = isinf(f.hi) ? 0.0f : (float)(exact - (double)f.hi);
+  f.hi = __double2float_rz(exact);
+  f.lo = (float)(exact - (double)f.hi);
+  if (f.hi > 0.0f && !(f.lo > 0.0f)) f.lo = __int_as_float(1);
   return f;
 }
-// f s + x.  (An infinite s times the small part would be an infinity of the other sign, or NaN.)
-__device__ __forceinline__ float times_plus(Factor f, float s, float x) {
-  return fmaf(f.hi, s, fmaf(f.lo, fabsf(s) <= 3.402823466e38f ? s : 0.0f, x));
-}
+// f s + x
+__device__ __forceinline__ float times_plus(Factor f, float s, float x) { return fmaf(f.hi, s, fmaf(f.lo, s, x)); }
 // decay^e, in double
 __device__ __forceinline__ double decay_power_exact(float log_decay, int e) {
   return e == 0 ? 1.0 : exp((double)log_decay * e);
