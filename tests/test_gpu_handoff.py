@@ -237,3 +237,24 @@ def test_a_copy_over_a_small_tensor(cuda_engine):
     assert np.all(z.arraySync() == 2.0) and np.all(x.arraySync() == 4.0)
     for k in (t, s, x, y, z):
         k.dispose()
+
+
+def test_a_tensor_that_its_holder_fills(cuda_engine):
+    """New memory, handed out before any kernel has written it."""
+    from tfjs_b200 import ops as tf
+    backend = cuda_engine.backend
+    before = backend.numDataIds()
+    side = torch.cuda.Stream()
+    for n in (1000, 1 << 23, 1 << 23, 3001):
+        backend.signal_stream(side.cuda_stream)
+        t = cuda_engine.make_tensor_from_info(backend.make_output([n], "float32"))
+        with torch.cuda.stream(side):
+            g = torch.as_tensor(t.dataToGPU(side.cuda_stream), device="cuda")
+            g.copy_(torch.arange(n, device="cuda"))
+        backend.wait_stream(side.cuda_stream)
+        y = tf.add(t, t)
+        assert np.array_equal(y.arraySync(), 2.0 * np.arange(n, dtype=np.float32))
+        del g
+        t.dispose()
+        y.dispose()
+    assert backend.numDataIds() == before

@@ -108,9 +108,9 @@ struct tfjs_cuda_ctx {
   long long* h_bad_index = nullptr;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;
   cudaEvent_t ev_order = nullptr;  // orders this context against a caller's stream
-  // Counts what may have put work on the stream or in front of it (every use of a tensor, every launch,
-  // every wait for another stream than the one signalled last), so that a caller's stream that was
-  // signalled and has missed nothing since is not signalled again.
+  // Counts what may have put work on the stream or in front of it (every allocation, every use of a tensor,
+  // every launch, every wait for another stream than the one signalled last), so that a caller's stream
+  // that was signalled and has missed nothing since is not signalled again.
   uint64_t work = 1, signalled_work = 0;
   unsigned long long signalled_stream = 0;  // cudaStreamGetId: never given out twice
   void* signalled_handle = (void*)~(uintptr_t)0;

@@ -339,6 +339,7 @@ int tfjs_cuda_alloc(tfjs_cuda_ctx* ctx, uint64_t nbytes, int32_t* out_id) {
   b.version++;
   ctx->in_use += padded;
   ctx->n_live++;
+  ctx->work++;   // (the block is there in stream order only: a stream that is handed it waits for that)
   if (ctx->in_use > ctx->high_water) ctx->high_water = ctx->in_use;
   *out_id = id;
   return TFJS_CUDA_OK;
