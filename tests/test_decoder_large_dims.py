@@ -24,3 +24,11 @@ def test_tokens_and_heads():
         inp = {n: info(shape) for n in "qkv"}
         refused(decoder._linear_attention, dict(inp, logDecay=info([shape[1]])), {}, "2^31")
     assert np.int32(np.int64(BIG) & 0xffffffff) == 5
+
+
+@pytest.mark.parametrize("attrs", [dict(budget=7.5), dict(budget=8, recent=2.5), dict(budget=float("inf")),
+                                   dict(budget=float("nan"))])
+def test_budgets_are_whole_numbers(attrs):
+    inp = dict(cache_inputs(), weights=info([3, 2, 64]))
+    with pytest.raises((ValueError, OverflowError)):
+        decoder._paged_cache_evict({"inputs": inp, "attrs": attrs, "backend": None})

@@ -137,9 +137,10 @@ def _paged_cache_evict(args):
         _want(name, "total", total, [p.batch], "int32")
     _not_a_pool(name, inp, ("weights",))
     budget, recent = int(at["budget"]), int(at.get("recent", 0))
-    if not 0 < budget < 1 << 30 or not 0 <= recent <= budget:
-        raise ValueError("%s: the budget must be positive and hold the recent slots, but got "
-                         "budget %d, recent %d" % (name, budget, recent))
+    if not 0 < budget < 1 << 30 or not 0 <= recent <= budget or \
+            budget != at["budget"] or recent != at.get("recent", 0):
+        raise ValueError("%s: the budget must be a positive whole number and hold the recent slots, "
+                         "but got budget %s, recent %s" % (name, at["budget"], at.get("recent", 0)))
     p.budget, p.recent = budget, recent
     reads = [dev(backend, t) for t in (weights, inp["pageTable"], inp["lengths"], positions, total)]
     pools = [backend.device_id_for_update(inp[n].dataId) for n in ("kCache", "vCache")]

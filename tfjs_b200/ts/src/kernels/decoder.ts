@@ -107,9 +107,10 @@ export const decoderConfigs: KernelConfig[] = [
     if (total != null) want(name, 'total', total, [d.batch], 'int32');
     notAPool(name, inputs, ['weights']);
     const budget = attrs['budget'] as number, recent = (attrs['recent'] as number) ?? 0;
-    if (!(budget > 0 && budget < 2 ** 30 && recent >= 0 && recent <= budget)) {
-      throw new Error(`${name}: the budget must be positive and hold the recent slots, but got budget ${budget}, ` +
-                      `recent ${recent}`);
+    if (!(budget > 0 && budget < 2 ** 30 && recent >= 0 && recent <= budget && Number.isInteger(budget) &&
+          Number.isInteger(recent))) {
+      throw new Error(`${name}: the budget must be a positive whole number and hold the recent slots, ` +
+                      `but got budget ${budget}, recent ${recent}`);
     }
     const reads = [weights, pageTable, lengths, positions, total].map(t => backend.deviceId(t));
     const [kc, vc] = [kCache, vCache].map(t => backend.deviceIdForUpdate(t));
