@@ -497,11 +497,13 @@ int tfjs_cuda_paged_cache_append(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_param
  * over the slots of row b; query head h reads key-value head h / (heads / kv_heads).
  * q is [batch, heads, 1, head_dim], out [batch, 1, heads, head_dim]; has_scale = 0 skips the
  * product.  mask (float32 [batch, capacity], 0: none) is added to the scores; -infinity hides
- * a slot, whose key and value then do not count whatever they hold (a page of which every slot is hidden
- * is not needed), and nothing is read of slots behind a row's length.  A row that has no slot, or only hidden ones (scores of -infinity), gives
- * zeros.  Finite keys, values and queries are assumed: an infinity may come out as NaN.  weights (float32 [batch, kv_heads, capacity], 0: none) accumulates
- * attention: out_weights[b, g, j] = weights[b, g, j] + the sum of p_j over the query heads of
- * key-value head g, and 0 behind the row's length. */
+ * a slot, whose key and value then do not count whatever they hold (a page of which every slot is
+ * hidden is not needed), and nothing is read of slots behind a row's length.  A row that has no
+ * slot, or only hidden ones (scores of -infinity), gives zeros.  Finite keys, values and queries of
+ * at most 2^127 are assumed: an infinity, and a float next to the largest, may come out as NaN.
+ * weights (float32 [batch, kv_heads, capacity], 0: none) accumulates attention:
+ * out_weights[b, g, j] = weights[b, g, j] + the sum of p_j over the query heads of key-value head
+ * g, and 0 behind the row's length. */
 int tfjs_cuda_paged_attention(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params* p, int32_t q_id,
                               int32_t k_cache_id, int32_t v_cache_id, int32_t page_table_id,
                               int32_t lengths_id, int32_t mask_id, int32_t weights_id,
@@ -535,9 +537,11 @@ int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params
  * out is [batch, seq, heads, dim_v] (heads merged, as tfjs_cuda_fused_attention stores it) and
  * out_state the state behind each row's last token.  lengths (int32 [batch], 0: all of seq)
  * gives the tokens of each row: what is behind them does not enter, and their out is zero.
- * has_scale = 0 skips the product.  A few tokens run as steps of the recurrence, prompts in chunks of
- * 128 tokens, within which a NaN or an infinity reaches every token.  dim_k and dim_v up to
- * 256.  No counterpart in the reference's kernel set. */
+ * has_scale = 0 skips the product.  Up to 32 tokens run as steps of the recurrence, prompts in chunks
+ * of 128 tokens.  A value of v that is NaN, infinite or above 2^127 makes its column of out NaN for all
+ * tokens of its chunk, those in front of it as well; one in the state in front of a chunk does the same.
+ * An infinite element of the state stays infinite in out_state.  dim_k and dim_v up to 256.  No
+ * counterpart in the reference's kernel set. */
 typedef struct tfjs_cuda_linear_attention_params {
   int32_t batch, heads, seq, dim_k, dim_v;
   int32_t has_scale;

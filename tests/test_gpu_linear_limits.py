@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests import decoder_cases as dc
-from tests.test_gpu_linear_attention import call, check, inputs, tf  # noqa: F401  (tf: a fixture)
+from tests.test_gpu_linear_attention import call, check, decays, inputs, tf  # noqa: F401  (tf: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,23 @@ def test_many_chunks(tf, n):
     lengths = np.array([n, n - 700], np.int32)
     check(call(tf, q, k, v, ld, state=s, scale=0.25, lengths=lengths),
           dc.linear(q, k, v, ld, s, 0.25, lengths))
+
+
+def test_what_is_not_finite_stays_in_its_column(tf):
+    """A NaN in v: its column of out is NaN from its token on, and in front of it within its chunk of 128 at
+    most; other columns, other rows and earlier chunks keep their values, and its column of the state
+    is NaN."""
+    b, h, n, d = 2, 2, 400, 64
+    q, k, v, s = inputs(17, b, h, n, d, d)
+    ld = decays(h)
+    clean = dc.linear(q, k, v, ld, s)
+    v = v.copy()
+    v[0, 1, 200, 9] = np.nan                            # in the second chunk, tokens 128 to 255
+    out, state = call(tf, q, k, v, ld, state=s)
+    assert np.all(np.isnan(out[0, 200:, 1, 9])) and np.all(np.isnan(state[0, 1, :, 9]))
+    there = np.ones(out.shape, bool)
+    there[0, 128:, 1, 9] = False
+    assert np.all(np.abs(out - clean[0])[there] <= clean[2][there])
+    there = np.ones(state.shape, bool)
+    there[0, 1, :, 9] = False
+    assert np.all(np.abs(state - clean[1])[there] <= clean[3][there])

@@ -18,11 +18,11 @@
 // Operands come through registers (load, split, swizzled store)
 // because the split has to happen on the way, so any size and alignment is a predicate there.
 //
-// 2 x 16 heads of 128 x 128 with 16384 tokens take 178 us for the states (805 MB), 88 for the scan (537 MB, 0.94
-// of a copy's bandwidth) and 407 for the outputs (1342 MB).  No unit is full in the last: DRAM, tensor and
+// 2 x 16 heads of 128 x 128 with 16384 tokens take 177 us for the states (805 MB), 90 for the scan (537 MB, 0.92
+// of a copy's bandwidth) and 410 for the outputs (1342 MB).  No unit is full in the last: DRAM, tensor and
 // shared-memory pipes are each near 0.4.  A chunk moves 1.5 MB through shared memory (the split doubles what is written,
 // and each MMA reads its operands again), some 12 k of about 28 k clocks at 128 bytes each; the rest is most
-// likely the chain of one chunk, since tensor memory has no room for a second one's scores.
+// likely the chain of one chunk: tensor memory has no room for a second one's scores (for half of them it has).
 #include "gemm_tf32_device.cuh"
 #include "linear_attention.h"
 

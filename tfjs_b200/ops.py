@@ -348,7 +348,7 @@ def paged_attention(q, kCache, vCache, pageTable, lengths, scale=None, mask=None
     to the scores; -infinity hides a slot, and pages all of whose slots are hidden need not be named by
     the table (a window over a long row).  Returns [batch, 1, heads, headDim] (as
     fused_attention does for a sequence); a row with nothing to attend to gives zeros.  Finite
-    keys, values and queries are assumed (an infinity may come out as NaN).  With
+    keys, values and queries of at most 2^127 are assumed (others may come out as NaN).  With
     weights [batch, kvHeads, maxPages * pageSize], which accumulates each slot's attention for
     paged_cache_evict, returns [out, newWeights]; newWeights is 0 behind a row's length.
     The token's own key and value are appended before.  A kernel of the 'cuda' backend with
@@ -388,9 +388,10 @@ def linear_attention(q, k, v, logDecay, state=None, scale=None, lengths=None):
     [batch, heads, dimK, dimV] (zeros if absent).  lengths [batch] int32 gives the tokens of
     each row of a padded batch; what is behind them does not enter and gives zeros.  Returns
     [out, newState] with out [batch, seq, heads, dimV].  seq = 1 is one step of generation,
-    longer inputs are prompts, in one call or in pieces that hand the state on; they run in
-    chunks of 128 tokens, within which a NaN or an infinity reaches every token.  A kernel of
-    the 'cuda' backend with no counterpart among the reference's ops."""
+    longer inputs are prompts, in one call or in pieces that hand the state on.  From 33 tokens on
+    they run in chunks of 128: a value of v that is NaN, infinite or above 2^127 makes its column of
+    out NaN for all tokens of its chunk, those in front of it as well.  A kernel of the 'cuda'
+    backend with no counterpart among the reference's ops."""
     return _run("_LinearAttention", {"q": q, "k": k, "v": v, "logDecay": logDecay,
                                      "state": state, "lengths": lengths}, {"scale": scale})
 
