@@ -86,3 +86,52 @@ def test_pages_that_the_mask_hides_are_not_needed(tf, cuda_engine, heads, kv, di
         cuda_engine.backend.sync()
     h.close()
     assert e.value.code == 1 and "page" in str(e.value)
+
+
+@pytest.mark.parametrize("kv,dim,budget", [(2, 64, 24), (1, 6, 150)])
+def test_a_captured_step_that_evicts_replays(tf, cuda_engine, kv, dim, budget):
+    """Append, attend with the weights kept, evict, with lengths, weights, positions and totals copied back:
+    replayed with eager calls in between, against the definitions; afterwards every state reads as the
+    replays left it."""
+    backend = cuda_engine.backend
+    r = np.random.default_rng(budget)
+    B, H, P, recent = 2, 2 * kv, 8, 6
+    n = np.array([budget, 5], np.int32)
+    cache = dc.Cache(budget, kv, dim, P, n, max_pages=-(-(2 * budget + 90) // P))
+    h = Held(tf, cache)
+    shape = (B, kv, cache.capacity)
+    w, pos = np.zeros(shape, np.float32), np.full(shape, -1, np.int32)
+    total = n.copy()
+    k, v = (r.standard_normal((B, kv, 1, dim)).astype(np.float32) for _ in range(2))
+    q = r.standard_normal((B, H, 1, dim)).astype(np.float32)
+    tk, tv, tq, tw, tp, tt, one = (h(x) for x in (k, v, q, w, pos, total, np.ones(1, np.int32)))
+    for t in h.all:
+        backend.device_id(t.dataId)
+    backend.sync()
+    backend.capture_begin(64 << 20)
+    long = tf.paged_cache_append(h.k, h.v, tk, tv, h.table, h.lengths)
+    seen = tf.add(tt, one)
+    out, summed = tf.paged_attention(tq, h.k, h.v, h.table, long, 0.25, None, tw)
+    parts = tf.paged_cache_evict(h.k, h.v, summed, h.table, long, budget, recent, tp, seen)
+    for new, old in zip(parts[:3] + [seen], (tw, tp, h.lengths, tt)):
+        backend.copy(new.dataId, old.dataId)
+    graph = backend.capture_end()
+    h.all += [long, seen, out, summed] + parts
+    for step in range(12):
+        backend.graph_launch(graph)
+        if step % 4 == 3:
+            h(tf.paged_attention(tq, h.k, h.v, h.table, h.lengths, 0.25))
+        for b in range(B):
+            at = cache.table[b, n[b] // P], slice(None), n[b] % P
+            cache.k[at], cache.v[at] = k[b, :, 0], v[b, :, 0]
+        n, total = n + 1, total + 1
+        ref, neww, off, woff = dc.attention(q, cache, n, 0.25, None, w)
+        check(out.arraySync(), ref, off)
+        got = summed.arraySync()
+        check(got, neww, woff + 12 * dc.EPS * neww)
+        w, pos, n, kept, cache.k, cache.v = dc.evict(cache, got, n, budget, recent, pos, total)
+        assert np.array_equal(parts[3].arraySync(), kept)
+    for t, want in ((tw, w), (tp, pos), (h.lengths, n), (tt, total), (h.k, cache.k), (h.v, cache.v)):
+        assert np.array_equal(t.arraySync(), want, equal_nan=want.dtype == np.float32)
+    backend.graph_destroy(graph)
+    h.close()
