@@ -538,10 +538,11 @@ int tfjs_cuda_paged_cache_evict(tfjs_cuda_ctx* ctx, const tfjs_cuda_paged_params
  * out_state the state behind each row's last token.  lengths (int32 [batch], 0: all of seq)
  * gives the tokens of each row: what is behind them does not enter, and their out is zero.
  * has_scale = 0 skips the product.  Up to 32 tokens run as steps of the recurrence, prompts in chunks
- * of 128 tokens.  A value of v that is NaN, infinite or above 2^127 makes its column of out NaN for all
- * tokens of its chunk, those in front of it as well; one in the state in front of a chunk does the same.
- * An infinite element of the state stays infinite in out_state.  dim_k and dim_v up to 256.  No
- * counterpart in the reference's kernel set. */
+ * of 128 tokens.  A NaN or an infinity in v enters its column of out with its token, not before; in the state
+ * it makes that column not finite, and an infinite element of the given state stays infinite.  Behind a
+ * state, and behind a chunk, that is not finite an infinity may come out as NaN, and so may a value above
+ * 2^127 (in q, k or the state, or in v behind its chunk).  dim_k and dim_v up to 256.  No counterpart
+ * in the reference's kernel set. */
 typedef struct tfjs_cuda_linear_attention_params {
   int32_t batch, heads, seq, dim_k, dim_v;
   int32_t has_scale;

@@ -57,21 +57,45 @@ def test_many_chunks(tf, n):
           dc.linear(q, k, v, ld, s, 0.25, lengths))
 
 
-def test_what_is_not_finite_stays_in_its_column(tf):
-    """A NaN in v: its column of out is NaN from its token on, and in front of it within its chunk of 128 at
-    most; other columns, other rows and earlier chunks keep their values, and its column of the state
-    is NaN."""
-    b, h, n, d = 2, 2, 400, 64
-    q, k, v, s = inputs(17, b, h, n, d, d)
+@pytest.mark.parametrize("b,h,n,dk,dv,spots", [
+    (2, 2, 400, 64, 64, [(0, 1, 200, 9)]),
+    (1, 1, 33, 64, 64, [(0, 0, 32, 63)]),
+    (2, 3, 300, 33, 50, [(0, 0, 0, 49), (1, 2, 299, 0)]),
+    (1, 2, 260, 128, 256, [(0, 0, 130, 3), (0, 1, 259, 200), (0, 1, 128, 200)]),
+    (40, 8, 150, 16, 32, [(i, i % 8, 149 - i, i % 32) for i in range(40)]),
+])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_what_is_not_finite_comes_after_its_token(tf, b, h, n, dk, dv, spots, value):
+    """A NaN or an infinity in v enters its column of out with its token and not before, in prompts as in
+    single tokens, and its column of the state; everything else keeps its value."""
+    q, k, v, s = inputs(17 + n, b, h, n, dk, dv)
     ld = decays(h)
-    clean = dc.linear(q, k, v, ld, s)
+    clean = dc.linear(q, k, v, ld, s, 0.125)
     v = v.copy()
-    v[0, 1, 200, 9] = np.nan                            # in the second chunk, tokens 128 to 255
-    out, state = call(tf, q, k, v, ld, state=s)
-    assert np.all(np.isnan(out[0, 200:, 1, 9])) and np.all(np.isnan(state[0, 1, :, 9]))
-    there = np.ones(out.shape, bool)
-    there[0, 128:, 1, 9] = False
+    there, inside = np.ones(clean[0].shape, bool), np.ones(clean[1].shape, bool)
+    for i, j, t, d in spots:
+        v[i, j, t, d] = value
+        there[i, t:, j, d] = inside[i, j, :, d] = False
+    out, state = call(tf, q, k, v, ld, state=s, scale=0.125)
     assert np.all(np.abs(out - clean[0])[there] <= clean[2][there])
-    there = np.ones(state.shape, bool)
-    there[0, 1, :, 9] = False
-    assert np.all(np.abs(state - clean[1])[there] <= clean[3][there])
+    assert np.all(np.abs(state - clean[1])[inside] <= clean[3][inside])
+    assert not np.any(np.isfinite(out[~there])) and not np.any(np.isfinite(state[~inside]))
+
+
+def test_values_next_to_the_largest(tf):
+    """Finite values of v beyond 2^127: the outputs of their chunk are right, earlier tokens' among them.
+    At decays of 1/2 such a value still counts 115 tokens later, with a weight of 5e-39: below 2^-126 the
+    operands of the tensor core are spaced 2^-136, so a weight is off by up to that, times the value."""
+    b, h, n, d = 1, 2, 300, 64
+    q, k, v, s = inputs(5, b, h, n, d, d)
+    v[0, 0, 140, 7], v[0, 1, 290, 63] = 3.4e38, np.finfo(np.float32).max
+    k[0, :, [140, 290]] *= 0.01
+    q *= np.float32(0.01)
+    ld = decays(h)
+    lengths = np.array([295], np.int32)
+    ref = dc.linear(q, k, v, ld, s, None, lengths)
+    out, state = call(tf, q, k, v, ld, state=s, lengths=lengths)
+    ref[2][:, 140:256, 0, 7] += 2.0 ** -136 * 3.4e38
+    first = np.s_[:, :256]                  # (the chunk of the first; the second's begins at 256)
+    assert np.all(np.abs(out - ref[0])[first] <= ref[2][first])
+    assert np.all(np.abs(out - ref[0])[:, 256:, 1] <= ref[2][:, 256:, 1])

@@ -45,6 +45,7 @@ __device__ __forceinline__ Factor factor_of(double exact) {
 }
 // f s + x
 __device__ __forceinline__ float times_plus(Factor f, float s, float x) { return fmaf(f.hi, s, fmaf(f.lo, s, x)); }
+constexpr float kMostFloat = 3.402823466e38f;
 // decay^e, in double
 __device__ __forceinline__ double decay_power_exact(float log_decay, int e) {
   return e == 0 ? 1.0 : exp((double)log_decay * e);

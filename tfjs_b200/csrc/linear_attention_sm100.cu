@@ -466,9 +466,45 @@ linear_chunk_scan_kernel(const ChunkArgs g, int blocks_per_unit) {
 // Eight producer warps, eight that read tensor memory.
 constexpr int kOutThreads = 512;
 
+// The second product multiplies values of v behind a token by zeros, which hides all but a NaN and an
+// infinity (a value above 2^127 becomes one when it is split).  Where a chunk has such a value its outputs are
+// computed once more, by the whole block, from the sums that the tokens have: slow, and nothing else needs it.
+__device__ __noinline__ void outputs_again(const ChunkArgs& g, int item, float* scores) {
+  const Item t = item_of(g, item);
+  const int cols = g.a.dv - t.dv0 < 128 ? g.a.dv - t.dv0 : 128;
+  const uint64_t row0 = (uint64_t)t.unit * g.a.seq + (uint64_t)t.c * kC;
+  const float* v = g.a.v + row0 * g.a.dv + t.dv0;
+  bool found = false;
+  for (int i = threadIdx.x; i < t.n * cols; i += kOutThreads)
+    found |= !(fabsf(__ldg(v + (uint64_t)(i / cols) * g.a.dv + i % cols)) <= 1.7014118e38f);
+  if (!__syncthreads_or(found)) return;
+  const float ld = __ldg(g.a.log_decay + t.h);
+  for (int i = threadIdx.x; i < t.n * kC; i += kOutThreads) {
+    const int row = i / kC, col = i % kC;
+    if (col > row) continue;
+    float sum = 0.f;
+    for (int d = 0; d < g.a.dk; ++d)
+      sum = fmaf(__ldg(g.a.q + (row0 + row) * g.a.dk + d), __ldg(g.a.k + (row0 + col) * g.a.dk + d), sum);
+    scores[i] = sum * decay_power(ld, row - col);
+  }
+  __syncthreads();
+  const float* state = g.states + (((uint64_t)t.unit * g.chunks + t.c) * g.a.dv + t.dv0) * g.a.dk;
+  for (int i = threadIdx.x; i < t.n * cols; i += kOutThreads) {
+    const int row = i / cols, col = i % cols;
+    float sum = 0.f;
+    for (int d = 0; d < g.a.dk; ++d)
+      sum = fmaf(__ldg(g.a.q + (row0 + row) * g.a.dk + d), state[(uint64_t)col * g.a.dk + d], sum);
+    sum *= decay_power(ld, row + 1);
+    for (int j = 0; j <= row; ++j) sum = fmaf(scores[row * kC + j], __ldg(v + (uint64_t)j * g.a.dv + col), sum);
+    g.a.out[(((uint64_t)t.b * g.a.seq + t.c * kC + row) * g.a.heads + t.h) * g.a.dv + t.dv0 + col] =
+        g.a.has_scale ? __fmul_rn(sum, g.a.scale) : sum;
+  }
+  __syncthreads();
+}
+
 template <bool WIDE>
 __global__ void __launch_bounds__(kOutThreads, 1)
-linear_chunk_outputs_kernel(const ChunkArgs g) {
+linear_chunk_outputs_kernel(const __grid_constant__ ChunkArgs g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t tiles = base + (uint32_t)(g.stages * g.stage_bytes);
@@ -479,8 +515,11 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
   const uint32_t tmem_slot = s_full + 16u;
   const uint32_t power_s = tmem_slot + 8u;                 // float[kC + 1]
   float* power = reinterpret_cast<float*>(smem_raw + (power_s - smem_u32(smem_raw)));
+  int* again = reinterpret_cast<int*>(power + kC + 2);     // first and last item to compute again
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    again[0] = 0x7fffffff;
+    again[1] = -1;
     for (int s = 0; s < g.stages; ++s) {
       mbar_init(full(s), kProducers);
       mbar_init(empty(s), 1);
@@ -814,6 +853,29 @@ linear_chunk_outputs_kernel(const ChunkArgs g) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
+  // A value of v that is not finite has made its column NaN for all tokens of its chunk, so the first token
+  // tells (read back here, since a look at the values on their way out took 3% of the time).
+  int from = 0x7fffffff, to = -1;
+#pragma unroll 8
+  for (int i = blockIdx.x + (int)(threadIdx.x >> 7) * gridDim.x; i < g.items; i += kOutThreads / 128 * gridDim.x) {
+    const int uc = i / g.dv_tiles, unit = uc / g.chunks, b = unit / g.a.heads;
+    const int d = (i - uc * g.dv_tiles) * 128 + (int)(threadIdx.x & 127);
+    // (behind a row's end are zeros)
+    const uint64_t at = (((uint64_t)b * g.a.seq + (uint64_t)(uc - unit * g.chunks) * kC) * g.a.heads + (unit - b * g.a.heads)) * g.a.dv + d;
+    const float x = d < g.a.dv ? __ldcg(g.a.out + at) : 0.f;
+    if (!(fabsf(x) <= kMostFloat)) {
+      from = min(from, i);
+      to = i;
+    }
+  }
+  if (to >= 0) {
+    atomicMin(again, from);
+    atomicMax(again + 1, to);
+  }
+  __syncthreads();
+  const int last = again[1];
+  for (int i = again[0]; i <= last; i += gridDim.x)
+    outputs_again(g, i, reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw))));
 }
 
 template <bool WIDE>
@@ -843,7 +905,7 @@ int launch_chunks(tfjs_cuda_ctx* ctx, ChunkArgs& g) {
   LAUNCH_CHECK(ctx, "linear_chunk_scan_kernel");
   const int qk = 32768 + 2 * (128 + g.dvp) * 128, v = 2 * 64 * g.dvp * 4;
   g.stage_bytes = qk > v ? qk : v;
-  const int o_fixed = 1024 + 8 * 4096 + 256 + (kC + 1) * 4;
+  const int o_fixed = 1024 + 8 * 4096 + 256 + (kC + 4) * 4;
   g.stages = (kSmemCap - o_fixed) / g.stage_bytes;
   if (g.stages > kMaxStages) g.stages = kMaxStages;
   const int o_smem = o_fixed + g.stages * g.stage_bytes;

@@ -388,10 +388,10 @@ def linear_attention(q, k, v, logDecay, state=None, scale=None, lengths=None):
     [batch, heads, dimK, dimV] (zeros if absent).  lengths [batch] int32 gives the tokens of
     each row of a padded batch; what is behind them does not enter and gives zeros.  Returns
     [out, newState] with out [batch, seq, heads, dimV].  seq = 1 is one step of generation,
-    longer inputs are prompts, in one call or in pieces that hand the state on.  From 33 tokens on
-    they run in chunks of 128: a value of v that is NaN, infinite or above 2^127 makes its column of
-    out NaN for all tokens of its chunk, those in front of it as well.  A kernel of the 'cuda'
-    backend with no counterpart among the reference's ops."""
+    longer inputs are prompts, in one call or in pieces that hand the state on; from 33 tokens on
+    they run in chunks of 128.  A NaN or an infinity in v enters its column of out with its token,
+    not before; further on infinities, and values above 2^127, may come out as NaN.  A kernel of the
+    'cuda' backend with no counterpart among the reference's ops."""
     return _run("_LinearAttention", {"q": q, "k": k, "v": v, "logDecay": logDecay,
                                      "state": state, "lengths": lengths}, {"scale": scale})
 
