@@ -520,6 +520,7 @@ class CudaBackend(object):
         self.ctx = ctx
         self.device_ordinal = device_ordinal
         self._words = []      # (_alloc)
+        self._addresses = []  # likewise, for addresses
         self.data = {}        # DataId -> _Record
         self._pinned = []
         self._hidden = 0      # records kept alive only by pending launches
@@ -684,10 +685,16 @@ class CudaBackend(object):
             self._launch_readers(tensor.dataId, rec)
         dev = rec.dev or self.device_id(tensor.dataId)
         rec.host = None
-        ptr = c_void_p()
-        rc = self.lib.tfjs_cuda_device_ptr(self.ctx, dev, byref(ptr))
+        try:
+            word = self._addresses.pop()
+        except IndexError:
+            word = c_void_p()
+            word = word, byref(word)
+        rc = self.lib.tfjs_cuda_device_ptr(self.ctx, dev, word[1])
         if rc:
             self.check(rc)
+        address = word[0].value or 0
+        self._addresses.append(word)
         if stream is not None:
             rc = self.lib.tfjs_cuda_signal_stream(self.ctx, stream)
             if rc:
@@ -698,7 +705,7 @@ class CudaBackend(object):
         if rec.shared == 0 and rec.foreign is None:
             self._exposed += 1
         rec.shared += 1
-        return GPUData(self, tensor, ptr.value or 0, rec.nbytes, stream, rec.read_only)
+        return GPUData(self, tensor, address, rec.nbytes, stream, rec.read_only)
 
     def release_gpu_data(self, ref, stream):
         """Disposes the tensor that a GPUData held, behind the work on its holder's stream.  Its memory
